@@ -140,7 +140,7 @@ def prepare(case, seed):
         import smat_b200 as S
         A = S.Fp4SparseMatrix.from_codes(case["M"], case["K"], w["rowptr"], (w["bcol"] * 16).int(), s["w"]["codes"], s["w"]["scales"],
                                          fmt=case["fmt"], row_scale=s["w"]["row_scale"])
-        s["plan"] = S.Fp4Plan(A, n_hint=case["N"])
+        s["plan"] = S.Fp4Plan(A)
     return s
 
 
