@@ -153,6 +153,65 @@ int smat_selftest_wait_timeout(void* stream);
  * latter kernel's other forms wait for nothing and multiply as ever; SMAT_ERR_BAD_ARG for plans of other kernels. */
 int smat_selftest_plan_wait_timeout(const smat_plan* plan, const void* B, void* C, size_t N, void* stream);
 
+/* ---- matrices in 4 bits ----------------------------------------------------------------------------------------------------
+ * Microscaled 4-bit floating point: codes are e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign in bit 3), two to a byte with the even
+ * column in the low half; groups of consecutive columns of a row share a scale.  No counterpart in the reference, which multiplies
+ * fp16 (src/cuda_hgemm/src/mma/mmaCBT.cu).
+ *   SMAT_FP4_NV  groups of 16; scale in e4m3 (bit 7 clear), times an fp32 scale of the row
+ *   SMAT_FP4_MX  groups of 32; scale 2^(byte - 127), 255 = NaN
+ * Quantisation divides by the scale and rounds to the nearest code, ties to even, magnitudes above 6 to 6, as exact arithmetic would:
+ *   SMAT_FP4_NV  row scale p = least power of two >= amax(row) / 2688, at least 2^-100, 1 for a row of zeros;
+ *                scale = e4m3(amax(group) / 6 / p) to nearest even; a group whose scale rounds to 0 is 0
+ *   SMAT_FP4_MX  2^e, e = floor(log2(amax(group))) - 2, at least -127; -127 for a group of zeros
+ * A group holding a NaN or an infinity gets the scale NaN and codes 0 (all of it reads as NaN); maxima of rows are over finite values.
+ *
+ * A dense matrix [N][K] in 4 bits (activations, the B of a product) is
+ *   codes   smat_fp4_codes_bytes(N, K) bytes: row r at r * ceil(K / 64) * 32, columns from K to the next multiple of 64 are 0
+ *   scales  smat_fp4_scales_bytes(N, K) bytes: tiles of 128 rows x 64 columns, 512 bytes each; the tile of (r, k) is number
+ *           (r / 128) * ceil(K / 64) + k / 64, the bytes of its row r at (r % 32) * 16 + (r % 128) / 32 * 4: four (SMAT_FP4_NV, one
+ *           for 16 columns), or two (SMAT_FP4_MX, one for 32 columns) and two zeros.  Those of rows N and up are not used.
+ *   row_scale  float[N] (SMAT_FP4_NV; may be NULL where it is read: ones)
+ * and a block matrix, beside rowptr and colidx as above,
+ *   codes   128 bytes a block (16 rows of 8), scales 16 bytes a block (one for each row), row_scale float[M].
+ *   Of SMAT_FP4_MX, the blocks of an aligned pair of block-columns (columns 32 c to 32 c + 31) have equal scales.
+ * All arrays 16-byte aligned in device memory; K a multiple of 16. */
+enum { SMAT_FP4_NV = 0, SMAT_FP4_MX = 1 };
+/* Element types of values. */
+enum { SMAT_F16 = 0, SMAT_BF16 = 1, SMAT_F32 = 2 };
+
+size_t smat_fp4_codes_bytes(size_t N, size_t K);
+size_t smat_fp4_scales_bytes(size_t N, size_t K);
+/* X [N][K] of fp16, bf16 or fp32, rows `ldx` elements apart (a multiple of 16 bytes), to 4 bits and back; one launch each, asynchronous
+ * on `stream`.  Values on the way back are code * scale * row_scale in fp32, rounded once. */
+int smat_fp4_quantize(const void* X, int dtype, size_t N, size_t K, size_t ldx, int fmt, void* codes, void* scales, float* row_scale,
+                      void* stream);
+int smat_fp4_dequantize(const void* codes, const void* scales, const float* row_scale, int fmt, size_t N, size_t K, void* Y, int dtype,
+                        size_t ldy, void* stream);
+/* The blocks of a matrix to 4 bits and back.  Block-rows whose row pointers are inconsistent with nonzeroBlocks are left out and
+ * reported by smat_device_status. */
+int smat_fp4_quantize_blocks(const void* vals, int dtype, const int* rowptr, const int* colidx, size_t M, size_t nonzeroBlocks, int fmt,
+                             void* codes, void* scales, float* row_scale, void* stream);
+int smat_fp4_dequantize_blocks(const void* codes, const void* scales, const float* row_scale, int fmt, const int* rowptr, size_t M,
+                               size_t nonzeroBlocks, void* vals, int dtype, void* stream);
+
+/* Plan for products of block-rows [brow_begin, brow_end) of a block matrix in 4 bits.  It looks the arrays over (block columns in
+ * strictly ascending order, multiples of 16 inside the matrix; inconsistent block-rows count as empty and are reported by
+ * smat_device_status) and keeps the pointers it was given: codes, scales and row scales may change in place between products, the
+ * structure may not.  Nothing in a plan is written by a product, so any number of streams may use it at a time.  Synchronises
+ * `stream`; K below 2^26. */
+typedef struct smat_fp4_plan smat_fp4_plan;
+int smat_fp4_plan_create(smat_fp4_plan** plan, const void* codes, const void* scales, const float* row_scale, int fmt, const int* rowptr,
+                         const int* colidx, size_t M, size_t K, size_t nonzeroBlocks, size_t brow_begin, size_t brow_end, void* stream);
+/* Rows [16*brow_begin, 16*brow_end) of C = A x B, sums in fp32, rounded once; C points at the first row of that range, row-major, N
+ * wide, any N.  B in 16 bits: B[n*K + k], C of the same type (fp16 or bf16); few columns (decoding) are what this is for: all
+ * widths work, 64 columns at a time. */
+int smat_fp4_plan_spmm(const smat_fp4_plan* plan, const void* B, int dtype, void* C, size_t N, void* stream);
+/* B in 4 bits, of the plan's format; C fp16 or bf16.  A block that is not stored may count as zeros: where B holds NaN (a group's
+ * scale), the rows of C that get one may be more than those whose stored blocks meet it. */
+int smat_fp4_plan_spmm_fp4(const smat_fp4_plan* plan, const void* codes, const void* scales, const float* row_scale, int fmt, void* C,
+                           int c_dtype, size_t N, void* stream);
+int smat_fp4_plan_destroy(smat_fp4_plan* plan);
+
 /* Number of this library's kernels launched so far by the calling process (all devices). */
 long long smat_launch_count(void);
 

@@ -36,3 +36,12 @@ from .api import (  # noqa: F401
     spmm,
     spmm_rows,
 )
+
+_FP4 = ("Fp4Matrix", "Fp4Plan", "Fp4SparseMatrix")  # need torch, which is imported with the first of them
+
+
+def __getattr__(name):
+    if name in _FP4:
+        from . import fp4
+        return getattr(fp4, name)
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

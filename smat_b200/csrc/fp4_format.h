@@ -1,0 +1,49 @@
+// Matrices in 4 bits: codes are e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign), two to a byte with the even column in the low half,
+// and consecutive columns of a row share a scale in groups.
+//   SMAT_FP4_NV  groups of 16, scale e4m3 (bit 7 clear), times an fp32 scale of the row
+//   SMAT_FP4_MX  groups of 32, scale 2^(code - 127)
+// Dense matrix (activations, [rows][K]):
+//   codes   row r at r * fp4_pitch(K) bytes; columns from K to the next multiple of 64 are zeros
+//   scales  tiles of 128 rows x 64 columns, 512 bytes each, tile (r / 128, k / 64) at index (r / 128) * fp4_quads(K) + k / 64;
+//           the four bytes of a row stand at (r % 32) * 16 + (r % 128) / 32 * 4: the order in which a block-scaled MMA finds the
+//           scales of 128 rows in tensor memory, so a tile goes there as it is.  SMAT_FP4_NV uses all four (one for 16 columns),
+//           SMAT_FP4_MX the first two (one for 32 columns), the others are zeros.
+// Block matrix: block p has its codes at p * 128 (16 rows of 8 bytes) and 16 scales at p * 16, one for each of its rows; of
+// SMAT_FP4_MX, the two blocks of an aligned pair of block-columns have equal scales.
+#pragma once
+#include <cuda_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include "smat_internal.h"
+
+namespace smat {
+
+// Columns are handled 64 at a time: K of one block-scaled MMA, 32 bytes of codes, one scale tile.
+inline size_t fp4_quads(size_t K) { return (K + 63) / 64; }
+inline size_t fp4_pitch(size_t K) { return fp4_quads(K) * 32; }
+
+// A stored matrix of 16 x 16 blocks in 4 bits and what a plan worked out about block-rows [brow_begin, brow_end).  Device memory.
+struct Fp4View {
+    const uint8_t* codes = nullptr;
+    const uint8_t* scales = nullptr;
+    const float* row_scale = nullptr;  // of the whole matrix, or null: ones
+    const int* colidx = nullptr;
+    const int2* range = nullptr;  // first and last + 1 block of every block-row of the range; empty where the arrays were inconsistent
+    int fmt = 0;
+    size_t K = 0, brow_begin = 0, block_rows = 0;
+    size_t blocks = 0, longest = 0;  // stored blocks of the range, and of its longest block-row
+};
+
+// Dense right-hand side: 16-bit values [N][K], or 4 bits as above.
+struct Fp4Rhs {
+    const void* data = nullptr;      // values, or codes
+    const uint8_t* scales = nullptr;  // 4 bits
+    const float* row_scale = nullptr;  // 4 bits; may be null
+    int dtype = 0;                   // SMAT_F16 or SMAT_BF16, or kFp4Rhs
+};
+constexpr int kFp4Rhs = 3;
+
+int launch_fp4_stream(const Fp4View& A, const Fp4Rhs& B, void* C, int c_dtype, size_t N, cudaStream_t stream);
+
+}  // namespace smat

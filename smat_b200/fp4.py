@@ -1,0 +1,301 @@
+"""Matrices in 4 bits (microscaled e2m1): quantisation, and products of a block-sparse matrix with dense ones.
+
+Formats, layouts and roundings are those of the C ABI (include/smat_b200.h, "matrices in 4 bits"):
+  "nvfp4"  groups of 16 columns share an e4m3 scale, every row has an fp32 scale (a power of two where it is computed here)
+  "mxfp4"  groups of 32 columns share a scale 2^e
+
+    A4 = Fp4SparseMatrix.quantize(A)              # A: SparseMatrix
+    plan = Fp4Plan(A4)
+    plan.spmm(x, C)                               # decoding: x [N, K] in fp16 or bf16, C [M, N] of the same type
+    plan.spmm(Fp4Matrix.quantize(x), C)           # prefilling: both in 4 bits on the tensor cores
+
+The reference multiplies fp16 only (src/cuda_hgemm/src/mma/mmaCBT.cu:13-88)."""
+import ctypes as C
+
+import torch
+
+from .api import Matrix, SmatError, SparseMatrix, _check, _stream, lib
+
+_FORMATS = {"nvfp4": 0, "mxfp4": 1}
+_GROUP = {"nvfp4": 16, "mxfp4": 32}
+_DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+_LIB = None
+
+
+def _lib():
+    global _LIB
+    if _LIB is None:
+        L = lib()
+        vp, sz, i = C.c_void_p, C.c_size_t, C.c_int
+        L.smat_fp4_quantize.argtypes = [vp, i, sz, sz, sz, i, vp, vp, vp, vp]
+        L.smat_fp4_dequantize.argtypes = [vp, vp, vp, i, sz, sz, vp, i, sz, vp]
+        L.smat_fp4_quantize_blocks.argtypes = [vp, i, vp, vp, sz, sz, i, vp, vp, vp, vp]
+        L.smat_fp4_dequantize_blocks.argtypes = [vp, vp, vp, i, vp, sz, sz, vp, i, vp]
+        L.smat_fp4_plan_create.argtypes = [C.POINTER(vp), vp, vp, vp, i, vp, vp, sz, sz, sz, sz, sz, vp]
+        L.smat_fp4_plan_spmm.argtypes = [vp, vp, i, vp, sz, vp]
+        L.smat_fp4_plan_spmm_fp4.argtypes = [vp, vp, vp, vp, i, vp, i, sz, vp]
+        L.smat_fp4_plan_destroy.argtypes = [vp]
+        _LIB = L
+    return _LIB
+
+
+def _refuse(text):
+    raise SmatError(-1, text)
+
+
+def _format(fmt):
+    if fmt not in _FORMATS:
+        _refuse(f"unknown 4-bit format {fmt!r}: 'nvfp4' or 'mxfp4'")
+    return _FORMATS[fmt]
+
+
+def _dtype(dtype, most=2):
+    code = _DTYPES.get(dtype, 3)
+    if code > most:
+        _refuse(f"element type {dtype} is not one of {[str(d) for d, c in _DTYPES.items() if c <= most]}")
+    return code
+
+
+def _on_current_device(t):
+    if not t.is_cuda or t.device.index != torch.cuda.current_device():
+        _refuse(f"tensor on {t.device}: it has to be on the current CUDA device")
+
+
+def _bytes_like(t, shape, name, device):
+    """t as uint8 (fp8 and other 8-bit types by their bits), of the given shape, contiguous."""
+    t = t if t.dtype == torch.uint8 else t.view(torch.uint8) if t.element_size() == 1 else _refuse(f"{name}: 8-bit elements expected, not {t.dtype}")
+    if tuple(t.shape) != tuple(shape):
+        _refuse(f"{name}: shape {tuple(shape)} expected, not {tuple(t.shape)}")
+    return t.to(device).contiguous()
+
+
+def _row_scales(row_scale, fmt, rows, device):
+    """float32[rows] or None; a single number stands for all rows."""
+    if row_scale is None:
+        return None
+    if fmt != "nvfp4":
+        _refuse("row scales go with nvfp4")
+    t = torch.as_tensor(row_scale, dtype=torch.float32, device=device)
+    if t.numel() == 1:
+        return t.reshape(1).expand(rows).contiguous()
+    if tuple(t.shape) != (rows,):
+        _refuse(f"row_scale: one number or {rows} expected, not shape {tuple(t.shape)}")
+    return t.contiguous()
+
+
+def _valid_scales(scales, fmt):
+    """e4m3 scales without their sign bit (no scale is negative)."""
+    return scales & 0x7F if fmt == "nvfp4" else scales
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+class Fp4Matrix:
+    """Dense matrix [N, K] in 4 bits, K a multiple of 16: the activations of a product.
+
+    ``codes`` uint8 [N, 32 * ceil(K / 64)], ``scales`` uint8 (tiled, see the C header; ``group_scales()`` gives them as
+    [N, groups]), ``row_scale`` float32 [N] or None."""
+
+    def __init__(self, N, K, fmt="nvfp4", device="cuda"):
+        _format(fmt)
+        if K % 16:
+            _refuse(f"K ({K}) must be a multiple of 16")
+        self.N, self.K, self.fmt = int(N), int(K), fmt
+        self.quads = -(-self.K // 64)
+        self.codes = torch.empty((self.N, self.quads * 32), dtype=torch.uint8, device=device)
+        self.scales = torch.empty(-(-self.N // 128) * self.quads * 512, dtype=torch.uint8, device=device)
+        self.row_scale = torch.empty(self.N, dtype=torch.float32, device=device) if fmt == "nvfp4" else None
+
+    @classmethod
+    def quantize(cls, X, fmt="nvfp4", out=None):
+        """X: Matrix or tensor [N, K] in fp16, bf16 or fp32 (rows may be strided, 16-byte aligned).  ``out``: an Fp4Matrix of this
+        size and format to write to instead of a new one."""
+        x = X.data if isinstance(X, Matrix) else X
+        f = _format(fmt)
+        d = _dtype(x.dtype)
+        if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
+            _refuse("a matrix [N, K] with consecutive columns is expected")
+        _on_current_device(x)
+        N, K = x.shape
+        if out is None:
+            out = cls(N, K, fmt, x.device)
+        elif (out.N, out.K, out.fmt, out.codes.device) != (N, K, fmt, x.device):
+            _refuse("out has another size, format or device")
+        elif f == 0 and out.row_scale is None:
+            _refuse("out has no row scales")
+        ld = x.stride(0) if N > 1 else K
+        rc = _lib().smat_fp4_quantize(x.data_ptr(), d, N, K, ld, f, out.codes.data_ptr(), out.scales.data_ptr(), _ptr(out.row_scale), _stream())
+        if rc:
+            _check(rc)
+        return out
+
+    @classmethod
+    def from_codes(cls, codes, scales, K, fmt="nvfp4", row_scale=None, device="cuda"):
+        """From arrays as checkpoints and other programs have them: codes uint8 [N, K / 2] (the even column in the low half),
+        scales 8-bit [N, ceil(K / 16 or 32)] (e4m3, or e8m0 bytes), row_scale one number or [N]."""
+        N = codes.shape[0]
+        self = cls(N, K, fmt, device)
+        dev = self.codes.device
+        self.codes.zero_()
+        self.codes[:, :K // 2] = _bytes_like(codes, (N, K // 2), "codes", dev)
+        groups, per = -(-K // _GROUP[fmt]), 64 // _GROUP[fmt]
+        s = _valid_scales(_bytes_like(scales, (N, groups), "scales", dev), fmt)
+        full = torch.zeros((-(-N // 128) * 128, self.quads, 4), dtype=torch.uint8, device=dev)
+        flat = torch.zeros((N, self.quads * per), dtype=torch.uint8, device=dev)
+        flat[:, :groups] = s
+        full[:N, :, :per] = flat.view(N, self.quads, per)
+        self.scales = full.view(-1, 4, 32, self.quads, 4).permute(0, 3, 2, 1, 4).reshape(-1).contiguous()
+        self.row_scale = _row_scales(row_scale, fmt, N, dev)
+        return self
+
+    def group_scales(self):
+        """The scales as uint8 [N, ceil(K / 16 or 32)]."""
+        per = 64 // _GROUP[self.fmt]
+        s = self.scales.view(-1, self.quads, 32, 4, 4).permute(0, 3, 2, 1, 4).reshape(-1, self.quads, 4)[:self.N, :, :per]
+        return s.reshape(self.N, -1)[:, :-(-self.K // _GROUP[self.fmt])].contiguous()
+
+    def dequantize(self, dtype=torch.float16, out=None):
+        """The values as a tensor [N, K] in fp16, bf16 or fp32, rounded once; ``out``: a tensor to write to."""
+        d = _dtype(dtype if out is None else out.dtype)
+        _on_current_device(self.codes)
+        if out is None:
+            out = torch.empty((self.N, self.K), dtype=dtype, device=self.codes.device)
+        elif tuple(out.shape) != (self.N, self.K) or (self.K > 1 and out.stride(1) != 1) or out.device != self.codes.device:
+            _refuse("out has another size, strided columns or another device")
+        ld = out.stride(0) if self.N > 1 else self.K
+        rc = _lib().smat_fp4_dequantize(self.codes.data_ptr(), self.scales.data_ptr(), _ptr(self.row_scale), _FORMATS[self.fmt], self.N,
+                                        self.K, out.data_ptr(), d, ld, _stream())
+        if rc:
+            _check(rc)
+        return out
+
+
+class Fp4SparseMatrix:
+    """Block-sparse matrix with its 16x16 blocks in 4 bits: the structure of a SparseMatrix (``bcsrRowPtr``, ``bcsrColIdx``),
+    ``codes`` uint8 [nnzb, 16, 8], ``scales`` uint8 [nnzb, 16], ``row_scale`` float32 [M] or None."""
+
+    def __init__(self):
+        self.M = self.K = self.nnzb = 0
+        self.fmt = "nvfp4"
+        self.bcsrRowPtr = self.bcsrColIdx = self.codes = self.scales = self.row_scale = None
+
+    def _allocate(self):
+        dev = self.bcsrRowPtr.device
+        self.codes = torch.empty((max(self.nnzb, 1), 16, 8), dtype=torch.uint8, device=dev)[:self.nnzb]
+        self.scales = torch.empty((max(self.nnzb, 1), 16), dtype=torch.uint8, device=dev)[:self.nnzb]
+        self.row_scale = torch.empty(self.M, dtype=torch.float32, device=dev) if self.fmt == "nvfp4" else None
+
+    @classmethod
+    def quantize(cls, A, fmt="nvfp4", check=False):
+        """The blocks of a SparseMatrix in 4 bits; the structure is shared with it."""
+        f = _format(fmt)
+        _on_current_device(A.bcsrVal)
+        self = cls()
+        self.M, self.K, self.nnzb, self.fmt = A.M, A.K, A.nnzb, fmt
+        self.bcsrRowPtr, self.bcsrColIdx = A.bcsrRowPtr, A.bcsrColIdx
+        self._allocate()
+        rc = _lib().smat_fp4_quantize_blocks(A.bcsrVal.data_ptr(), _dtype(A.bcsrVal.dtype), A.bcsrRowPtr.data_ptr(), A.bcsrColIdx.data_ptr(),
+                                             A.M, A.nnzb, f, self.codes.data_ptr(), self.scales.data_ptr(), _ptr(self.row_scale), _stream())
+        if rc:
+            _check(rc)
+        if check:
+            _check(lib().smat_device_status(_stream()))
+        return self
+
+    @classmethod
+    def from_codes(cls, M, K, bcsr_rowptr, bcsr_colidx, codes, scales, fmt="nvfp4", row_scale=None, device="cuda"):
+        """From arrays in 4 bits: codes uint8 [nnzb, 16, 8], scales 8-bit [nnzb, 16] (of mxfp4: equal for the two blocks of an
+        aligned pair), row_scale one number or [M]; rowptr and element columns as in SparseMatrix."""
+        _format(fmt)
+        self = cls()
+        self.M, self.K, self.nnzb, self.fmt = int(M), int(K), int(len(bcsr_colidx)), fmt
+        rp = torch.as_tensor(bcsr_rowptr)
+        dev = torch.empty(0, device=device).device
+        if rp.numel() != self.M // 16 + 1:
+            _refuse(f"bcsr_rowptr: {self.M // 16 + 1} numbers expected, not {rp.numel()}")
+        self.bcsrRowPtr = rp.to(dev, torch.int32).contiguous()
+        self.bcsrColIdx = torch.as_tensor(bcsr_colidx).to(dev, torch.int32).contiguous()
+        self.codes = _bytes_like(torch.as_tensor(codes), (self.nnzb, 16, 8), "codes", dev)
+        self.scales = _valid_scales(_bytes_like(torch.as_tensor(scales), (self.nnzb, 16), "scales", dev), fmt)
+        self.row_scale = _row_scales(row_scale, fmt, self.M, dev)
+        return self
+
+    def dequantize(self, check=False):
+        """A SparseMatrix of the values in fp16, rounded once; it shares the structure."""
+        _on_current_device(self.codes)
+        A = SparseMatrix()
+        A.M, A.K, A.nnzb = self.M, self.K, self.nnzb
+        A.bcsrRowPtr, A.bcsrColIdx = self.bcsrRowPtr, self.bcsrColIdx
+        A.bcsrVal = torch.empty(max(self.nnzb, 1) * 256, dtype=torch.float16, device=self.codes.device)
+        rc = _lib().smat_fp4_dequantize_blocks(self.codes.data_ptr(), self.scales.data_ptr(), _ptr(self.row_scale), _FORMATS[self.fmt],
+                                               A.bcsrRowPtr.data_ptr(), A.M, A.nnzb, A.bcsrVal.data_ptr(), 0, _stream())
+        if rc:
+            _check(rc)
+        if check:
+            _check(lib().smat_device_status(_stream()))
+        return A
+
+
+class Fp4Plan:
+    """Plan for products of block-rows [brow_begin, brow_end) of an Fp4SparseMatrix (smat_fp4_plan_*).  Codes and scales of the
+    matrix may change in place, its structure may not; products do not change the plan and may run on several streams at a time."""
+
+    def __init__(self, A, brow_begin=0, brow_end=None):
+        self.A = A
+        self.brow_begin = brow_begin
+        self.brow_end = A.M // 16 if brow_end is None else brow_end
+        self._h = None
+        _on_current_device(A.bcsrRowPtr)
+        h = C.c_void_p()
+        L = _lib()
+        _check(L.smat_fp4_plan_create(C.byref(h), A.codes.data_ptr(), A.scales.data_ptr(), _ptr(A.row_scale), _FORMATS[A.fmt],
+                                      A.bcsrRowPtr.data_ptr(), A.bcsrColIdx.data_ptr(), A.M, A.K, A.nnzb, self.brow_begin,
+                                      self.brow_end, _stream()))
+        self._h = h
+        self._rows = (self.brow_end - self.brow_begin) * 16
+        self._device = A.bcsrRowPtr.device
+
+    def spmm(self, B, Cout, check=False):
+        """C = A x B.  B: Matrix / tensor [N, K] in fp16 or bf16 with C of the same type, or an Fp4Matrix of A's format with C in
+        either; C: Matrix / tensor [rows, N], contiguous, fully overwritten."""
+        if self._h is None:
+            _refuse("the plan is closed")
+        Ct = Cout.data if isinstance(Cout, Matrix) else Cout
+        if isinstance(B, Fp4Matrix):
+            N, K, Bt = B.N, B.K, B.codes
+        else:
+            Bt = B.data if isinstance(B, Matrix) else B
+            N, K = Bt.shape
+            if Bt.dtype != Ct.dtype:
+                _refuse(f"B is {Bt.dtype}, C is {Ct.dtype}: the same type is expected")
+        if K != self.A.K or tuple(Ct.shape) != (self._rows, N):
+            _refuse(f"B [N, {self.A.K}] and C [{self._rows}, N] are expected, not [{N}, {K}] and {list(Ct.shape)}")
+        if not (Bt.is_contiguous() and Ct.is_contiguous()):
+            _refuse("B and C have to be contiguous")
+        if Bt.device != self._device or Ct.device != self._device:
+            _refuse(f"B and C have to be on {self._device}, like A")
+        d = _dtype(Ct.dtype, most=1)
+        if isinstance(B, Fp4Matrix):
+            if B.fmt != self.A.fmt:
+                _refuse(f"B is in {B.fmt}, A in {self.A.fmt}")
+            rc = _LIB.smat_fp4_plan_spmm_fp4(self._h, Bt.data_ptr(), B.scales.data_ptr(), _ptr(B.row_scale), _FORMATS[B.fmt], Ct.data_ptr(),
+                                             d, N, _stream())
+        else:
+            rc = _LIB.smat_fp4_plan_spmm(self._h, Bt.data_ptr(), d, Ct.data_ptr(), N, _stream())
+        if rc:
+            _check(rc)
+        if check:
+            _check(lib().smat_device_status(_stream()))
+
+    def close(self):
+        if self._h is not None:
+            _lib().smat_fp4_plan_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
