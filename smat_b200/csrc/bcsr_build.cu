@@ -209,6 +209,14 @@ int bitmap_words(size_t K, int* words, size_t factor) {
 }
 
 }  // namespace
+
+int scan_inplace_async(int* data, int n, cudaStream_t stream) {
+    scan_inplace_kernel<<<1, 1024, 0, stream>>>(data, n);
+    count_launch();
+    SMAT_CUDA_TRY(cudaGetLastError());
+    return SMAT_OK;
+}
+
 }  // namespace smat
 
 using namespace smat;
@@ -236,9 +244,7 @@ int smat_bcsr_count(const int* csr_rowptr, const int* csr_colidx, size_t M, size
     } else {
         SMAT_CUDA_TRY(cudaMemsetAsync(bcsr_rowptr, 0, sizeof(int), stream));
     }
-    scan_inplace_kernel<<<1, 1024, 0, stream>>>(bcsr_rowptr, Mb + 1);
-    count_launch();
-    SMAT_CUDA_TRY(cudaGetLastError());
+    if (int rc = scan_inplace_async(bcsr_rowptr, Mb + 1, stream)) return rc;
     // the total is the last entry of the scanned array (the caller's own buffer: concurrent calls do not meet)
     int total = 0;
     SMAT_CUDA_TRY(cudaMemcpyAsync(&total, bcsr_rowptr + Mb, sizeof(total), cudaMemcpyDeviceToHost, stream));

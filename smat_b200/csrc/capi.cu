@@ -80,8 +80,9 @@ int get_device_ctx(DeviceCtx** out) {
     return SMAT_OK;
 }
 
-int encode_tensor_map_2d_f16(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint64_t row_pitch_bytes,
-                             uint32_t box_inner, uint32_t box_outer, int swizzle_bytes, int l2_promo_bytes) {
+namespace {
+int encode_tensor_map_2d(CUtensorMap* map, CUtensorMapDataType type, const void* base, uint64_t inner, uint64_t outer,
+                         uint64_t row_pitch_bytes, uint32_t box_inner, uint32_t box_outer, int swizzle_bytes, int l2_promo_bytes) {
     typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -103,7 +104,7 @@ int encode_tensor_map_2d_f16(CUtensorMap* map, const void* base, uint64_t inner,
                                          : l2_promo_bytes >= 64  ? CU_TENSOR_MAP_L2_PROMOTION_L2_64B
                                                                  : CU_TENSOR_MAP_L2_PROMOTION_NONE;
     const CUresult r =
-        encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
+        encode(map, type, 2, const_cast<void*>(base), dims, strides, box, estr,
                CU_TENSOR_MAP_INTERLEAVE_NONE,
                swizzle_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B
                : swizzle_bytes == 32 ? CU_TENSOR_MAP_SWIZZLE_32B
@@ -115,6 +116,16 @@ int encode_tensor_map_2d_f16(CUtensorMap* map, const void* base, uint64_t inner,
                     (int)r, (unsigned long long)inner, (unsigned long long)outer, (unsigned long long)row_pitch_bytes,
                     box_inner, box_outer);
     return SMAT_OK;
+}
+}  // namespace
+int encode_tensor_map_2d_f16(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint64_t row_pitch_bytes,
+                             uint32_t box_inner, uint32_t box_outer, int swizzle_bytes, int l2_promo_bytes) {
+    return encode_tensor_map_2d(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, base, inner, outer, row_pitch_bytes, box_inner, box_outer,
+                                swizzle_bytes, l2_promo_bytes);
+}
+int encode_tensor_map_2d_u8(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint64_t row_pitch_bytes, uint32_t box_inner,
+                            uint32_t box_outer) {
+    return encode_tensor_map_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, inner, outer, row_pitch_bytes, box_inner, box_outer, 128, 128);
 }
 
 int check_spmm_args(const void* vals, const int* rowptr, const int* colidx, const void* B, const void* C, size_t M,

@@ -23,6 +23,16 @@ namespace smat {
 inline size_t fp4_quads(size_t K) { return (K + 63) / 64; }
 inline size_t fp4_pitch(size_t K) { return fp4_quads(K) * 32; }
 
+// Products with B in 4 bits walk groups of 8 block-rows in steps of 256 columns; steps in which a group has no block are left out (a
+// group without any has one step, with an empty mask).
+constexpr size_t kFp4GroupRows = 8, kFp4StepColumns = 256;
+struct alignas(16) Fp4Step {
+    int begin[8];      // first block of each block-row in these columns
+    uint8_t count[8];  // and their number, 0 to 16
+    uint32_t kstep;    // columns from 256 * kstep on
+    uint32_t mask;     // bit q: there are blocks in columns 64 q to 64 q + 63 of these
+};
+
 // A stored matrix of 16 x 16 blocks in 4 bits and what a plan worked out about block-rows [brow_begin, brow_end).  Device memory.
 struct Fp4View {
     const uint8_t* codes = nullptr;
@@ -32,6 +42,9 @@ struct Fp4View {
     const int2* range = nullptr;  // first and last + 1 block of every block-row of the range; empty where the arrays were inconsistent
     int fmt = 0;
     size_t K = 0, brow_begin = 0, block_rows = 0;
+    const Fp4Step* steps = nullptr;
+    const int* gsp = nullptr;  // first step of every group, and the number of all
+    size_t total_steps = 0;
     size_t blocks = 0, longest = 0;  // stored blocks of the range, and of its longest block-row
 };
 
@@ -45,5 +58,7 @@ struct Fp4Rhs {
 constexpr int kFp4Rhs = 3;
 
 int launch_fp4_stream(const Fp4View& A, const Fp4Rhs& B, void* C, int c_dtype, size_t N, cudaStream_t stream);
+
+int launch_fp4_tile(const Fp4View& A, const Fp4Rhs& B, void* C, int c_dtype, size_t N, cudaStream_t stream);
 
 }  // namespace smat

@@ -7,7 +7,8 @@
 struct smat_fp4_plan {
     smat::Fp4View v;
     int device = -1;
-    void* buffer = nullptr;
+    void* buffer = nullptr;  // totals, block ranges and first steps
+    void* steps = nullptr;
 };
 
 namespace smat {
@@ -40,6 +41,105 @@ __global__ void __launch_bounds__(kThreads) fp4_ranges_kernel(const int* __restr
     }
 }
 
+// The steps of a group (a CTA a group, a warp a block-row): a bitmap of the 256-column ranges that hold a block, counted (FILL false)
+// or turned into records.  Shared memory: `words` words of bitmap and, to fill, as many prefix counts.
+template <bool FILL>
+__global__ void __launch_bounds__(kThreads) fp4_steps_kernel(const int2* __restrict__ range, const int* __restrict__ colidx, int block_rows, int words,
+                                                             int* __restrict__ gsp, Fp4Step* __restrict__ steps) {
+    extern __shared__ uint32_t sm[];
+    uint32_t *bitmap = sm, *prefix = sm + words;
+    __shared__ int sums[kThreads];
+    const int tid = threadIdx.x, row = (int)(blockIdx.x * kFp4GroupRows) + tid / 32;
+    static_assert(kThreads == 32 * kFp4GroupRows, "a warp a block-row");
+    const int2 mine = row < block_rows ? range[row] : make_int2(0, 0);
+    for (int w = tid; w < words; w += kThreads) bitmap[w] = 0;
+    __syncthreads();
+    for (int p = mine.x + tid % 32; p < mine.y; p += 32) {
+        const int k = __ldg(colidx + p) >> 8;
+        atomicOr(&bitmap[k >> 5], 1u << (k & 31));
+    }
+    __syncthreads();
+    const int per = (words + kThreads - 1) / kThreads, w0 = min(words, tid * per), w1 = min(words, w0 + per);
+    int n = 0;
+    for (int w = w0; w < w1; w++) n += __popc(bitmap[w]);
+    sums[tid] = n;
+    __syncthreads();
+    for (int d = 1; d < kThreads; d *= 2) {
+        const int v = tid >= d ? sums[tid - d] : 0;
+        __syncthreads();
+        sums[tid] += v;
+        __syncthreads();
+    }
+    if (!FILL) {
+        if (tid == 0) gsp[blockIdx.x + 1] = max(1, sums[kThreads - 1]);
+        return;
+    }
+    int before = sums[tid] - n;
+    for (int w = w0; w < w1; w++) {
+        prefix[w] = before;
+        before += __popc(bitmap[w]);
+    }
+    __syncthreads();
+    Fp4Step* const first = steps + gsp[blockIdx.x];
+    for (int p = mine.x + tid % 32; p < mine.y; p += 32) {
+        const int k = __ldg(colidx + p) >> 8;
+        if (p > mine.x && __ldg(colidx + p - 1) >> 8 == k) continue;  // the first block of these columns speaks for all
+        uint32_t mask = 0;
+        int q = p;
+        for (int c; q < mine.y && (c = __ldg(colidx + q)) >> 8 == k; q++) mask |= 1u << (c >> 6 & 3);
+        Fp4Step* s = first + prefix[k >> 5] + __popc(bitmap[k >> 5] & ((1u << (k & 31)) - 1));
+        s->begin[tid / 32] = p;
+        s->count[tid / 32] = (uint8_t)(q - p);
+        s->kstep = (uint32_t)k;
+        atomicOr(&s->mask, mask);
+    }
+}
+
+// Ranges, totals and steps of a plan.  Synchronises the stream.
+int build_plan(smat_fp4_plan* p, const int* rowptr, const int* colidx, size_t nnzb, const DeviceCtx* ctx, cudaStream_t stream) {
+    Fp4View& v = p->v;
+    const size_t groups = (v.block_rows + kFp4GroupRows - 1) / kFp4GroupRows;
+    const size_t range_bytes = (v.block_rows * sizeof(int2) + 15) / 16 * 16;
+    SMAT_CUDA_TRY(cudaMalloc(&p->buffer, 16 + range_bytes + (groups + 1) * sizeof(int)));
+    unsigned long long* totals = static_cast<unsigned long long*>(p->buffer);
+    int2* range = reinterpret_cast<int2*>(totals + 2);
+    int* gsp = reinterpret_cast<int*>(reinterpret_cast<char*>(range) + range_bytes);
+    SMAT_CUDA_TRY(cudaMemsetAsync(p->buffer, 0, 16 + range_bytes + (groups + 1) * sizeof(int), stream));
+    fp4_ranges_kernel<<<(unsigned)v.block_rows, kThreads, 0, stream>>>(rowptr + v.brow_begin, colidx, v.K, nnzb, range, totals, ctx->d_status);
+    count_launch();
+    SMAT_CUDA_TRY(cudaGetLastError());
+    const int words = (int)((v.K + 32 * kFp4StepColumns - 1) / (32 * kFp4StepColumns));
+    SMAT_CUDA_TRY(cudaFuncSetAttribute(fp4_steps_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, words * 8));
+    fp4_steps_kernel<false><<<(unsigned)groups, kThreads, words * 4, stream>>>(range, colidx, (int)v.block_rows, words, gsp, nullptr);
+    count_launch();
+    SMAT_CUDA_TRY(cudaGetLastError());
+    if (int rc = scan_inplace_async(gsp, (int)groups + 1, stream)) return rc;
+    unsigned long long h_totals[2] = {0, 0};
+    int h_steps = 0;
+    SMAT_CUDA_TRY(cudaMemcpyAsync(h_totals, totals, sizeof(h_totals), cudaMemcpyDeviceToHost, stream));
+    SMAT_CUDA_TRY(cudaMemcpyAsync(&h_steps, gsp + groups, sizeof(int), cudaMemcpyDeviceToHost, stream));
+    SMAT_CUDA_TRY(cudaStreamSynchronize(stream));
+    v.blocks = h_totals[0];
+    v.longest = h_totals[1];
+    v.total_steps = (size_t)h_steps;
+    SMAT_CUDA_TRY(cudaMalloc(&p->steps, v.total_steps * sizeof(Fp4Step)));
+    SMAT_CUDA_TRY(cudaMemsetAsync(p->steps, 0, v.total_steps * sizeof(Fp4Step), stream));
+    fp4_steps_kernel<true><<<(unsigned)groups, kThreads, words * 8, stream>>>(range, colidx, (int)v.block_rows, words, gsp, static_cast<Fp4Step*>(p->steps));
+    count_launch();
+    SMAT_CUDA_TRY(cudaGetLastError());
+    SMAT_CUDA_TRY(cudaStreamSynchronize(stream));
+    v.range = range;
+    v.gsp = gsp;
+    v.steps = static_cast<const Fp4Step*>(p->steps);
+    return SMAT_OK;
+}
+
+cudaError_t free_plan(smat_fp4_plan* p) {
+    const cudaError_t a = cudaFree(p->buffer), b = cudaFree(p->steps);
+    delete p;
+    return a != cudaSuccess ? a : b;
+}
+
 int check_product(const smat_fp4_plan* plan, const void* B, const void* C, int c_dtype, size_t N) {
     if (!plan) return fail(SMAT_ERR_BAD_ARG, "plan is NULL");
     if (N >= ((size_t)1 << 31)) return fail(SMAT_ERR_RANGE, "N beyond 2^31");
@@ -70,6 +170,7 @@ int smat_fp4_plan_create(smat_fp4_plan** out, const void* codes, const void* sca
     if (brow_begin > brow_end || brow_end > M / 16)
         return fail(SMAT_ERR_BAD_ARG, "block-row range [%zu, %zu) outside [0, %zu]", brow_begin, brow_end, M / 16);
     if (nnzb * 16 >= ((size_t)1 << 31) || K >= ((size_t)1 << 31) || M / 16 >= ((size_t)1 << 31)) return fail(SMAT_ERR_RANGE, "size beyond 2^31");
+    if (K >= ((size_t)1 << 26)) return fail(SMAT_ERR_RANGE, "K (%zu) beyond 2^26 - 1", K);  // a bitmap of steps in shared memory
     DeviceCtx* ctx = nullptr;
     if (int rc = get_device_ctx(&ctx)) return rc;
     smat_fp4_plan* p = new (std::nothrow) smat_fp4_plan();
@@ -84,29 +185,11 @@ int smat_fp4_plan_create(smat_fp4_plan** out, const void* codes, const void* sca
     v.K = K;
     v.brow_begin = brow_begin;
     v.block_rows = brow_end - brow_begin;
-    cudaError_t e = cudaSuccess;
     if (v.block_rows) {
-        const size_t bytes = 16 + v.block_rows * sizeof(int2);
-        unsigned long long totals[2] = {0, 0};
-        e = cudaMalloc(&p->buffer, bytes);
-        if (e == cudaSuccess) e = cudaMemsetAsync(p->buffer, 0, 16, (cudaStream_t)stream);
-        if (e == cudaSuccess) {
-            int2* range = reinterpret_cast<int2*>(static_cast<char*>(p->buffer) + 16);
-            v.range = range;
-            fp4_ranges_kernel<<<(unsigned)v.block_rows, kThreads, 0, (cudaStream_t)stream>>>(
-                rowptr + brow_begin, colidx, K, nnzb, range, static_cast<unsigned long long*>(p->buffer), ctx->d_status);
-            count_launch();
-            e = cudaGetLastError();
+        if (int rc = build_plan(p, rowptr, colidx, nnzb, ctx, (cudaStream_t)stream)) {
+            free_plan(p);
+            return rc;
         }
-        if (e == cudaSuccess) e = cudaMemcpyAsync(totals, p->buffer, 16, cudaMemcpyDeviceToHost, (cudaStream_t)stream);
-        if (e == cudaSuccess) e = cudaStreamSynchronize((cudaStream_t)stream);
-        v.blocks = totals[0];
-        v.longest = totals[1];
-    }
-    if (e != cudaSuccess) {
-        cudaFree(p->buffer);
-        delete p;
-        return fail(SMAT_ERR_CUDA, "plan build failed: %s", cudaGetErrorString(e));
     }
     *out = p;
     return SMAT_OK;
@@ -130,19 +213,22 @@ int smat_fp4_plan_spmm_fp4(const smat_fp4_plan* plan, const void* codes, const v
     if (fmt != plan->v.fmt) return fail(SMAT_ERR_BAD_ARG, "B must be in the format of A");
     if (!plan->v.block_rows || !N) return SMAT_OK;
     if ((plan->v.K && !scales) || ((uintptr_t)scales & 15)) return fail(SMAT_ERR_BAD_ARG, "scales is NULL or not 16-byte aligned");
+    if (!plan->v.blocks) {
+        SMAT_CUDA_TRY(cudaMemsetAsync(C, 0, plan->v.block_rows * 16 * N * 2, (cudaStream_t)stream));
+        return SMAT_OK;
+    }
     Fp4Rhs rhs;
     rhs.data = codes;
     rhs.scales = static_cast<const uint8_t*>(scales);
     rhs.row_scale = row_scale;
     rhs.dtype = kFp4Rhs;
-    return launch_fp4_stream(plan->v, rhs, C, c_dtype, N, (cudaStream_t)stream);
+    return launch_fp4_tile(plan->v, rhs, C, c_dtype, N, (cudaStream_t)stream);
 }
 
 int smat_fp4_plan_destroy(smat_fp4_plan* plan) {
     clear_error();
     if (!plan) return SMAT_OK;
-    const cudaError_t e = plan->buffer ? cudaFree(plan->buffer) : cudaSuccess;
-    delete plan;
+    const cudaError_t e = free_plan(plan);
     if (e != cudaSuccess) return fail(SMAT_ERR_CUDA, "cudaFree failed: %s", cudaGetErrorString(e));
     return SMAT_OK;
 }

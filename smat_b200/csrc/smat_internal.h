@@ -80,6 +80,9 @@ constexpr int kOrderWindow = 16384;
 // cuTensorMapEncodeTiled through the runtime's driver entry point lookup (no link against libcuda).
 int encode_tensor_map_2d_f16(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint64_t row_pitch_bytes,
                              uint32_t box_inner, uint32_t box_outer, int swizzle_bytes, int l2_promo_bytes);
+// Bytes with a 128-byte swizzle.
+int encode_tensor_map_2d_u8(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint64_t row_pitch_bytes, uint32_t box_inner,
+                            uint32_t box_outer);
 
 // Most block-rows per work item of the SpMM kernel (one accumulator each).  A plan is built for groups of
 // `rg` <= kPlanRowsPerGroup block-rows: small matrices / shards use smaller groups to fill the SMs.
@@ -236,6 +239,8 @@ int plan_count_tall_async(const int* rowptr, const int* colidx, size_t K, size_t
 int plan_fill_tall_async(const int* rowptr, const int* colidx, size_t K, size_t nnzb, size_t brow_begin, size_t brow_end,
                          size_t rg, const int* gsp, void* steps, void* wstep, void* winfo, int* blk, cudaStream_t stream,
                          const DeviceCtx* ctx = nullptr);
+// In-place inclusive scan of device memory data[0..n), n small (bcsr_build.cu).
+int scan_inplace_async(int* data, int n, cudaStream_t stream);
 // Launch of the SpMM kernel (spmm_sm100.cu).  `ldc`: elements between rows of C (0 = N, i.e. C is exactly N wide).
 // [group_begin, group_end): the groups of the plan to multiply (default: all); C points at the first row of
 // group_begin.
