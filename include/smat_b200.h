@@ -196,12 +196,14 @@ int smat_fp4_dequantize_blocks(const void* codes, const void* scales, const floa
 
 /* Plan for products of block-rows [brow_begin, brow_end) of a block matrix in 4 bits.  It looks the arrays over (block columns in
  * strictly ascending order, multiples of 16 inside the matrix; inconsistent block-rows count as empty and are reported by
- * smat_device_status) and keeps the pointers it was given: codes, scales and row scales may change in place between products, the
- * structure may not.  Nothing in a plan is written by a product, so any number of streams may use it at a time.  Synchronises
- * `stream`; K below 2^26. */
+ * smat_device_status) and keeps the pointers it was given.  with_tiles: it also holds the blocks laid out for products with B in 4
+ * bits, 36 KB for every 256 rows x 256 columns that hold a block, unless they hold fewer than 8 on average; without, such products work
+ * but are slow.  After codes or scales changed (same structure) call smat_fp4_plan_set_values.  Nothing in a plan is written by a
+ * product, so any number of streams may use it at a time.  Creation synchronises `stream`; K below 2^26. */
 typedef struct smat_fp4_plan smat_fp4_plan;
 int smat_fp4_plan_create(smat_fp4_plan** plan, const void* codes, const void* scales, const float* row_scale, int fmt, const int* rowptr,
-                         const int* colidx, size_t M, size_t K, size_t nonzeroBlocks, size_t brow_begin, size_t brow_end, void* stream);
+                         const int* colidx, size_t M, size_t K, size_t nonzeroBlocks, size_t brow_begin, size_t brow_end, int with_tiles, void* stream);
+int smat_fp4_plan_set_values(smat_fp4_plan* plan, void* stream);
 /* Rows [16*brow_begin, 16*brow_end) of C = A x B, sums in fp32, rounded once; C points at the first row of that range, row-major, N
  * wide, any N.  B in 16 bits: B[n*K + k], C of the same type (fp16 or bf16); few columns (decoding) are what this is for: all
  * widths work, 64 columns at a time. */

@@ -23,14 +23,19 @@ namespace smat {
 inline size_t fp4_quads(size_t K) { return (K + 63) / 64; }
 inline size_t fp4_pitch(size_t K) { return fp4_quads(K) * 32; }
 
-// Products with B in 4 bits walk groups of 8 block-rows in steps of 256 columns; steps in which a group has no block are left out (a
-// group without any has one step, with an empty mask).
-constexpr size_t kFp4GroupRows = 8, kFp4StepColumns = 256;
-struct alignas(16) Fp4Step {
-    int begin[8];      // first block of each block-row in these columns
-    uint8_t count[8];  // and their number, 0 to 16
-    uint32_t kstep;    // columns from 256 * kstep on
-    uint32_t mask;     // bit q: there are blocks in columns 64 q to 64 q + 63 of these
+// Products with B in 4 bits walk groups of 16 block-rows in steps of 256 columns; steps in which a group has no block are left out (a
+// group without any has one, with an empty mask).  Every step has two tiles, one for each half of the group: 128 rows x 256 columns
+// as they lie in shared memory, 16384 bytes of codes (128 bytes a row, its 16-byte pieces in the order piece ^ row % 8) and four
+// scale tiles of 128 rows x 64 columns, zeros where no block is stored.
+constexpr size_t kFp4GroupRows = 16, kFp4StepColumns = 256;
+constexpr uint32_t kFp4TileCodes = 16384, kFp4TileBytes = kFp4TileCodes + 2048;
+struct Fp4Step {
+    uint32_t kstep;  // columns from 256 * kstep on
+    uint32_t mask;   // bit 4 h + q: half h has blocks in columns 64 q to 64 q + 63 of these
+};
+struct Fp4Where {         // of what the tiles of a step are made
+    int begin[16];        // first block of each block-row in these columns
+    uint16_t blocks[16];  // bit c: the block-row has a block in columns 16 c to 16 c + 15 of these
 };
 
 // A stored matrix of 16 x 16 blocks in 4 bits and what a plan worked out about block-rows [brow_begin, brow_end).  Device memory.
@@ -42,8 +47,9 @@ struct Fp4View {
     const int2* range = nullptr;  // first and last + 1 block of every block-row of the range; empty where the arrays were inconsistent
     int fmt = 0;
     size_t K = 0, brow_begin = 0, block_rows = 0;
-    const Fp4Step* steps = nullptr;
-    const int* gsp = nullptr;  // first step of every group, and the number of all
+    const Fp4Step* steps = nullptr;  // null: the plan has no tiles
+    const uint8_t* tiles = nullptr;  // two of a step
+    const int* gsp = nullptr;        // first step of every group, and the number of all
     size_t total_steps = 0;
     size_t blocks = 0, longest = 0;  // stored blocks of the range, and of its longest block-row
 };

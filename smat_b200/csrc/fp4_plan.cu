@@ -8,13 +8,17 @@ struct smat_fp4_plan {
     smat::Fp4View v;
     int device = -1;
     void* buffer = nullptr;  // totals, block ranges and first steps
-    void* steps = nullptr;
+    void* steps = nullptr;   // steps and what their tiles are made of
+    smat::Fp4Where* where = nullptr;
+    void* tiles = nullptr;
 };
 
 namespace smat {
 namespace {
 
 constexpr int kThreads = 256;
+// Tiles are made where a step holds so many blocks (of 256) on average.
+constexpr size_t kFp4TileFill = 8;
 
 // Looks a block-row's pointers and columns over (a CTA a block-row): they have to lie in the arrays and the matrix, the columns in
 // ascending order.  An inconsistent block-row is left out (empty) and reported.  totals: blocks, longest block-row.
@@ -43,35 +47,36 @@ __global__ void __launch_bounds__(kThreads) fp4_ranges_kernel(const int* __restr
 
 // The steps of a group (a CTA a group, a warp a block-row): a bitmap of the 256-column ranges that hold a block, counted (FILL false)
 // or turned into records.  Shared memory: `words` words of bitmap and, to fill, as many prefix counts.
+constexpr int kStepThreads = 32 * (int)kFp4GroupRows;
 template <bool FILL>
-__global__ void __launch_bounds__(kThreads) fp4_steps_kernel(const int2* __restrict__ range, const int* __restrict__ colidx, int block_rows, int words,
-                                                             int* __restrict__ gsp, Fp4Step* __restrict__ steps) {
+__global__ void __launch_bounds__(kStepThreads) fp4_steps_kernel(const int2* __restrict__ range, const int* __restrict__ colidx, int block_rows,
+                                                                 int words, int* __restrict__ gsp, Fp4Step* __restrict__ steps,
+                                                                 Fp4Where* __restrict__ where) {
     extern __shared__ uint32_t sm[];
     uint32_t *bitmap = sm, *prefix = sm + words;
-    __shared__ int sums[kThreads];
-    const int tid = threadIdx.x, row = (int)(blockIdx.x * kFp4GroupRows) + tid / 32;
-    static_assert(kThreads == 32 * kFp4GroupRows, "a warp a block-row");
+    __shared__ int sums[kStepThreads];
+    const int tid = threadIdx.x, e = tid / 32, row = (int)(blockIdx.x * kFp4GroupRows) + e;
     const int2 mine = row < block_rows ? range[row] : make_int2(0, 0);
-    for (int w = tid; w < words; w += kThreads) bitmap[w] = 0;
+    for (int w = tid; w < words; w += kStepThreads) bitmap[w] = 0;
     __syncthreads();
     for (int p = mine.x + tid % 32; p < mine.y; p += 32) {
         const int k = __ldg(colidx + p) >> 8;
         atomicOr(&bitmap[k >> 5], 1u << (k & 31));
     }
     __syncthreads();
-    const int per = (words + kThreads - 1) / kThreads, w0 = min(words, tid * per), w1 = min(words, w0 + per);
+    const int per = (words + kStepThreads - 1) / kStepThreads, w0 = min(words, tid * per), w1 = min(words, w0 + per);
     int n = 0;
     for (int w = w0; w < w1; w++) n += __popc(bitmap[w]);
     sums[tid] = n;
     __syncthreads();
-    for (int d = 1; d < kThreads; d *= 2) {
+    for (int d = 1; d < kStepThreads; d *= 2) {
         const int v = tid >= d ? sums[tid - d] : 0;
         __syncthreads();
         sums[tid] += v;
         __syncthreads();
     }
     if (!FILL) {
-        if (tid == 0) gsp[blockIdx.x + 1] = max(1, sums[kThreads - 1]);
+        if (tid == 0) gsp[blockIdx.x + 1] = max(1, sums[kStepThreads - 1]);
         return;
     }
     int before = sums[tid] - n;
@@ -80,64 +85,131 @@ __global__ void __launch_bounds__(kThreads) fp4_steps_kernel(const int2* __restr
         before += __popc(bitmap[w]);
     }
     __syncthreads();
-    Fp4Step* const first = steps + gsp[blockIdx.x];
+    const int first = gsp[blockIdx.x];
     for (int p = mine.x + tid % 32; p < mine.y; p += 32) {
         const int k = __ldg(colidx + p) >> 8;
         if (p > mine.x && __ldg(colidx + p - 1) >> 8 == k) continue;  // the first block of these columns speaks for all
-        uint32_t mask = 0;
-        int q = p;
-        for (int c; q < mine.y && (c = __ldg(colidx + q)) >> 8 == k; q++) mask |= 1u << (c >> 6 & 3);
-        Fp4Step* s = first + prefix[k >> 5] + __popc(bitmap[k >> 5] & ((1u << (k & 31)) - 1));
-        s->begin[tid / 32] = p;
-        s->count[tid / 32] = (uint8_t)(q - p);
-        s->kstep = (uint32_t)k;
-        atomicOr(&s->mask, mask);
+        uint32_t blocks = 0, mask = 0;
+        for (int q = p, c; q < mine.y && (c = __ldg(colidx + q)) >> 8 == k; q++) {
+            blocks |= 1u << (c >> 4 & 15);
+            mask |= 1u << (c >> 6 & 3);
+        }
+        const int at = first + (int)prefix[k >> 5] + __popc(bitmap[k >> 5] & ((1u << (k & 31)) - 1));
+        where[at].begin[e] = p;
+        where[at].blocks[e] = (uint16_t)blocks;
+        steps[at].kstep = (uint32_t)k;
+        atomicOr(&steps[at].mask, mask << (e / 8 * 4));
     }
 }
 
-// Ranges, totals and steps of a plan.  Synchronises the stream.
-int build_plan(smat_fp4_plan* p, const int* rowptr, const int* colidx, size_t nnzb, const DeviceCtx* ctx, cudaStream_t stream) {
+// Lays the blocks of a step out into its two tiles: a warp a block-row, a lane half a row (eight block-columns).
+template <int FMT>
+__global__ void __launch_bounds__(kStepThreads) fp4_tiles_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
+                                                                 const Fp4Where* __restrict__ where, uint8_t* __restrict__ tiles) {
+    const uint32_t e = threadIdx.x / 32, lane = threadIdx.x % 32, r = lane & 15, h = lane >> 4;
+    const Fp4Where& w = where[blockIdx.x];
+    const uint32_t blocks = w.blocks[e], mine = blocks >> (8 * h) & 0xff;
+    size_t p = (size_t)w.begin[e] + (h ? __popc(blocks & 0xff) : 0);
+    uint2 v[8];
+    uint32_t s[8];
+#pragma unroll
+    for (uint32_t j = 0; j < 8; j++) {
+        v[j] = make_uint2(0, 0);
+        s[j] = 0;
+        if (mine >> j & 1) {
+            v[j] = __ldg(reinterpret_cast<const uint2*>(codes + p * 128) + r);
+            s[j] = __ldg(scales + p * 16 + r);
+            p++;
+        }
+    }
+    const uint32_t row = (e & 7) * 16 + r;
+    uint8_t* const tile = tiles + ((size_t)blockIdx.x * 2 + e / 8) * kFp4TileBytes;
+#pragma unroll
+    for (uint32_t j = 0; j < 4; j++)
+        *reinterpret_cast<uint4*>(tile + row * 128 + (((4 * h + j) ^ (r & 7)) << 4)) = make_uint4(v[2 * j].x, v[2 * j].y, v[2 * j + 1].x, v[2 * j + 1].y);
+#pragma unroll
+    for (uint32_t j = 0; j < 2; j++) {
+        const uint32_t* q = s + 4 * j;
+        *reinterpret_cast<uint32_t*>(tile + kFp4TileCodes + (2 * h + j) * 512 + (row & 31) * 16 + (row >> 5) * 4) =
+            FMT == SMAT_FP4_NV ? q[0] | q[1] << 8 | q[2] << 16 | q[3] << 24 : (q[0] | q[1]) | (q[2] | q[3]) << 8;  // mxfp4: the blocks of a pair have equal scales
+    }
+}
+
+int fill_tiles(const smat_fp4_plan* p, cudaStream_t stream) {
+    const Fp4View& v = p->v;
+    if (!v.tiles || !v.blocks) return SMAT_OK;
+    uint8_t* tiles = static_cast<uint8_t*>(p->tiles);
+    if (v.fmt == SMAT_FP4_NV) fp4_tiles_kernel<SMAT_FP4_NV><<<(unsigned)v.total_steps, kStepThreads, 0, stream>>>(v.codes, v.scales, p->where, tiles);
+    else fp4_tiles_kernel<SMAT_FP4_MX><<<(unsigned)v.total_steps, kStepThreads, 0, stream>>>(v.codes, v.scales, p->where, tiles);
+    count_launch();
+    SMAT_CUDA_TRY(cudaGetLastError());
+    return SMAT_OK;
+}
+
+// Ranges and totals of a plan, and the steps and tiles for products with B in 4 bits.  Synchronises the stream.
+int build_plan(smat_fp4_plan* p, const int* rowptr, const int* colidx, size_t nnzb, bool with_tiles, const DeviceCtx* ctx, cudaStream_t stream) {
     Fp4View& v = p->v;
     const size_t groups = (v.block_rows + kFp4GroupRows - 1) / kFp4GroupRows;
-    const size_t range_bytes = (v.block_rows * sizeof(int2) + 15) / 16 * 16;
-    SMAT_CUDA_TRY(cudaMalloc(&p->buffer, 16 + range_bytes + (groups + 1) * sizeof(int)));
+    const size_t range_bytes = (v.block_rows * sizeof(int2) + 15) / 16 * 16, bytes = 16 + range_bytes + (groups + 1) * sizeof(int);
+    SMAT_CUDA_TRY(cudaMalloc(&p->buffer, bytes));
     unsigned long long* totals = static_cast<unsigned long long*>(p->buffer);
     int2* range = reinterpret_cast<int2*>(totals + 2);
     int* gsp = reinterpret_cast<int*>(reinterpret_cast<char*>(range) + range_bytes);
-    SMAT_CUDA_TRY(cudaMemsetAsync(p->buffer, 0, 16 + range_bytes + (groups + 1) * sizeof(int), stream));
+    SMAT_CUDA_TRY(cudaMemsetAsync(p->buffer, 0, bytes, stream));
     fp4_ranges_kernel<<<(unsigned)v.block_rows, kThreads, 0, stream>>>(rowptr + v.brow_begin, colidx, v.K, nnzb, range, totals, ctx->d_status);
     count_launch();
     SMAT_CUDA_TRY(cudaGetLastError());
     const int words = (int)((v.K + 32 * kFp4StepColumns - 1) / (32 * kFp4StepColumns));
-    SMAT_CUDA_TRY(cudaFuncSetAttribute(fp4_steps_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, words * 8));
-    fp4_steps_kernel<false><<<(unsigned)groups, kThreads, words * 4, stream>>>(range, colidx, (int)v.block_rows, words, gsp, nullptr);
-    count_launch();
-    SMAT_CUDA_TRY(cudaGetLastError());
-    if (int rc = scan_inplace_async(gsp, (int)groups + 1, stream)) return rc;
+    if (with_tiles) {
+        fp4_steps_kernel<false><<<(unsigned)groups, kStepThreads, words * 4, stream>>>(range, colidx, (int)v.block_rows, words, gsp, nullptr, nullptr);
+        count_launch();
+        SMAT_CUDA_TRY(cudaGetLastError());
+        if (int rc = scan_inplace_async(gsp, (int)groups + 1, stream)) return rc;
+    }
     unsigned long long h_totals[2] = {0, 0};
     int h_steps = 0;
     SMAT_CUDA_TRY(cudaMemcpyAsync(h_totals, totals, sizeof(h_totals), cudaMemcpyDeviceToHost, stream));
     SMAT_CUDA_TRY(cudaMemcpyAsync(&h_steps, gsp + groups, sizeof(int), cudaMemcpyDeviceToHost, stream));
     SMAT_CUDA_TRY(cudaStreamSynchronize(stream));
+    v.range = range;
     v.blocks = h_totals[0];
     v.longest = h_totals[1];
-    v.total_steps = (size_t)h_steps;
-    SMAT_CUDA_TRY(cudaMalloc(&p->steps, v.total_steps * sizeof(Fp4Step)));
-    SMAT_CUDA_TRY(cudaMemsetAsync(p->steps, 0, v.total_steps * sizeof(Fp4Step), stream));
-    fp4_steps_kernel<true><<<(unsigned)groups, kThreads, words * 8, stream>>>(range, colidx, (int)v.block_rows, words, gsp, static_cast<Fp4Step*>(p->steps));
+    const size_t steps = (size_t)h_steps;
+    if (!with_tiles || v.blocks < kFp4TileFill * steps) return SMAT_OK;
+    SMAT_CUDA_TRY(cudaMalloc(&p->steps, steps * (sizeof(Fp4Step) + sizeof(Fp4Where))));
+    Fp4Step* step = static_cast<Fp4Step*>(p->steps);
+    p->where = reinterpret_cast<Fp4Where*>(step + steps);
+    SMAT_CUDA_TRY(cudaMalloc(&p->tiles, steps * 2 * kFp4TileBytes));
+    SMAT_CUDA_TRY(cudaMemsetAsync(p->steps, 0, steps * (sizeof(Fp4Step) + sizeof(Fp4Where)), stream));
+    SMAT_CUDA_TRY(cudaFuncSetAttribute(fp4_steps_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, words * 8));
+    fp4_steps_kernel<true><<<(unsigned)groups, kStepThreads, words * 8, stream>>>(range, colidx, (int)v.block_rows, words, gsp, step, p->where);
     count_launch();
     SMAT_CUDA_TRY(cudaGetLastError());
-    SMAT_CUDA_TRY(cudaStreamSynchronize(stream));
-    v.range = range;
     v.gsp = gsp;
-    v.steps = static_cast<const Fp4Step*>(p->steps);
+    v.total_steps = steps;
+    v.steps = step;
+    v.tiles = static_cast<const uint8_t*>(p->tiles);
+    if (int rc = fill_tiles(p, stream)) return rc;
+    SMAT_CUDA_TRY(cudaStreamSynchronize(stream));
     return SMAT_OK;
 }
 
 cudaError_t free_plan(smat_fp4_plan* p) {
-    const cudaError_t a = cudaFree(p->buffer), b = cudaFree(p->steps);
+    cudaError_t e = cudaSuccess;
+    for (void* m : {p->buffer, p->steps, p->tiles}) {
+        const cudaError_t f = cudaFree(m);
+        if (e == cudaSuccess) e = f;
+    }
     delete p;
-    return a != cudaSuccess ? a : b;
+    return e;
+}
+
+int check_plan_device(const smat_fp4_plan* plan) {
+    int dev = -1;
+    SMAT_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev != plan->device)
+        return fail(SMAT_ERR_BAD_ARG, "the plan belongs to device %d but device %d is current", plan->device, dev);
+    return SMAT_OK;
 }
 
 int check_product(const smat_fp4_plan* plan, const void* B, const void* C, int c_dtype, size_t N) {
@@ -146,10 +218,7 @@ int check_product(const smat_fp4_plan* plan, const void* B, const void* C, int c
     if (c_dtype != SMAT_F16 && c_dtype != SMAT_BF16) return fail(SMAT_ERR_BAD_ARG, "C must be fp16 or bf16");
     if (plan->v.block_rows && N && (!C || (plan->v.K && !B))) return fail(SMAT_ERR_BAD_ARG, "B or C is NULL");
     if (((uintptr_t)B | (uintptr_t)C) & 15) return fail(SMAT_ERR_BAD_ARG, "B and C must be 16-byte aligned");
-    int dev = -1;
-    SMAT_CUDA_TRY(cudaGetDevice(&dev));
-    if (dev != plan->device) return fail(SMAT_ERR_BAD_ARG, "the plan belongs to device %d, the current device is %d", plan->device, dev);
-    return SMAT_OK;
+    return check_plan_device(plan);
 }
 
 }  // namespace
@@ -160,7 +229,8 @@ using namespace smat;
 extern "C" {
 
 int smat_fp4_plan_create(smat_fp4_plan** out, const void* codes, const void* scales, const float* row_scale, int fmt, const int* rowptr,
-                         const int* colidx, size_t M, size_t K, size_t nnzb, size_t brow_begin, size_t brow_end, void* stream) {
+                         const int* colidx, size_t M, size_t K, size_t nnzb, size_t brow_begin, size_t brow_end, int with_tiles,
+                         void* stream) {
     clear_error();
     if (!out || !rowptr || (nnzb && (!codes || !scales || !colidx))) return fail(SMAT_ERR_BAD_ARG, "NULL argument");
     *out = nullptr;
@@ -186,13 +256,20 @@ int smat_fp4_plan_create(smat_fp4_plan** out, const void* codes, const void* sca
     v.brow_begin = brow_begin;
     v.block_rows = brow_end - brow_begin;
     if (v.block_rows) {
-        if (int rc = build_plan(p, rowptr, colidx, nnzb, ctx, (cudaStream_t)stream)) {
+        if (int rc = build_plan(p, rowptr, colidx, nnzb, with_tiles != 0, ctx, (cudaStream_t)stream)) {
             free_plan(p);
             return rc;
         }
     }
     *out = p;
     return SMAT_OK;
+}
+
+int smat_fp4_plan_set_values(smat_fp4_plan* plan, void* stream) {
+    clear_error();
+    if (!plan) return fail(SMAT_ERR_BAD_ARG, "plan is NULL");
+    if (int rc = check_plan_device(plan)) return rc;
+    return fill_tiles(plan, (cudaStream_t)stream);
 }
 
 int smat_fp4_plan_spmm(const smat_fp4_plan* plan, const void* B, int dtype, void* C, size_t N, void* stream) {
@@ -222,7 +299,7 @@ int smat_fp4_plan_spmm_fp4(const smat_fp4_plan* plan, const void* codes, const v
     rhs.scales = static_cast<const uint8_t*>(scales);
     rhs.row_scale = row_scale;
     rhs.dtype = kFp4Rhs;
-    return launch_fp4_tile(plan->v, rhs, C, c_dtype, N, (cudaStream_t)stream);
+    return (plan->v.tiles ? launch_fp4_tile : launch_fp4_stream)(plan->v, rhs, C, c_dtype, N, (cudaStream_t)stream);
 }
 
 int smat_fp4_plan_destroy(smat_fp4_plan* plan) {

@@ -4,15 +4,16 @@
 // accumulators; the fp32 scales of rows and columns are applied to the sums.
 //
 // Why tiles.  The MMA takes 64 columns at a time and reads a panel of 128 rows of B in 32 cycles whatever it is multiplied with, so
-// single 16-row blocks (8 cycles of work) cannot feed it.  Eight block-rows form a tile of 128 rows: where blocks are absent zeros
-// are multiplied, which costs less than their absence would from a fill of 1/4 of the quads (16 x 64) on.  Steps of 256 columns in
-// which the tile holds no block at all are left out, and so are MMAs of 64 columns without one.  In memory the blocks stay
-// 144 bytes each: warps lay them out into the tile in shared memory, so that HBM and L2 see only what is stored.
+// single 16-row blocks (8 cycles of work) cannot feed it.  Eight block-rows form a tile of 128 rows, laid out by the plan: where
+// blocks are absent zeros are multiplied, which costs less than their absence would from a fill of 1/4 of the quads (16 x 64) on.
+// Steps of 256 columns in which a group of two tiles holds no block are left out, and so are MMAs of 64 columns without one.  (Laying
+// the blocks out in shared memory instead, from the 144 bytes each, was measured first: 950 us for the layer 8192 x 28672 at 20 %,
+// N = 4096; the hand-overs between copying, laying out and multiplying warps took 700 cycles a step alone.)
 //
-// Roles.  One thread fetches B (tiled TMA copies with 128-byte swizzle) and its scales; eight or sixteen warps copy the blocks of
-// their block-row (cp.async) and lay them out; one thread moves the scales to tensor memory and issues the MMAs; four warps store
-// finished tiles.  The (tile of C, step) pairs are dealt out in equal contiguous ranges, one per CTA; tiles that a range boundary
-// falls into are joined from fp32 parts in a fixed order by a second kernel.  All waits are bounded.
+// Roles.  One thread fetches the tiles (bulk copies), B (tiled TMA copies with 128-byte swizzle) and its scales; one thread moves the
+// scales to tensor memory and issues the MMAs; four warps store finished tiles of C.  The (tile of C, step) pairs are dealt out in
+// equal contiguous ranges, one per CTA; tiles that a range boundary falls into are joined from fp32 parts in a fixed order by a
+// second kernel.  All waits are bounded.
 #include "fp4_device.cuh"
 #include "ptx_sm100.cuh"
 #include "smat_internal.h"
@@ -52,33 +53,6 @@ __device__ __forceinline__ void cp_scales(uint32_t taddr, uint64_t desc) {
 __device__ __forceinline__ uint64_t desc_scales(uint32_t smem_addr) {
     return (uint64_t)((smem_addr >> 4) & 0x3FFFu) | (8ull << 16) | (8ull << 32) | (1ull << 46);
 }
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ uint2 ld_shared_v2(uint32_t addr) {
-    uint2 v;
-    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
-    return v;
-}
-__device__ __forceinline__ void st_shared_v2(uint32_t addr, uint2 v) {
-    asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(addr), "r"(v.x), "r"(v.y) : "memory");
-}
-__device__ __forceinline__ void st_shared_zero16(uint32_t addr) {
-    asm volatile("{\n\t.reg .b32 z;\n\tmov.b32 z, 0;\n\tst.shared.v4.b32 [%0], {z, z, z, z};\n\t}" ::"r"(addr) : "memory");
-}
-__device__ __forceinline__ uint32_t ld_shared_u8(uint32_t addr) {
-    uint32_t v;
-    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-    return v;
-}
-__device__ __forceinline__ void st_shared_u8(uint32_t addr, uint32_t v) { asm volatile("st.shared.u8 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
-
 // ---- schedule -------------------------------------------------------------------------------------------------------------------
 // Positions: the steps of a tile of C after one another, tiles of a group of block-rows after one another, groups after one another.
 struct Work {
@@ -137,17 +111,15 @@ struct Walk {
 };
 
 struct TileArgs {
-    const uint8_t* codes;
-    const uint8_t* scales;
-    const int* colidx;
     const Fp4Step* steps;
+    const uint8_t* tiles;
     const uint8_t* b_scales;
     const float* row_scale;  // first of the range, or null
     const float* b_row_scale;
     void* C;
     float* scratch;
     int* status;
-    int c_dtype, rows, N, quads, b_row_tiles;
+    int c_dtype, rows, N, quads, b_row_tiles, col_tiles;
 };
 
 // 16 values of row m from column n on (those below N), scaled, to C.
@@ -170,28 +142,24 @@ __device__ __forceinline__ void store_row16(const TileArgs& a, int m, int n, con
     }
 }
 
-// NT columns of C per tile.  EG groups of eight warps lay out blocks (each takes every EG-th step), RING of their copies are on their way.
+// NT columns of C per tile.
 template <int NT>
 struct Cfg {
-    static constexpr int EG = NT == 256 ? 1 : 2;
-    static constexpr int RING = NT == 256 ? 3 : 2;
-    static constexpr uint32_t S = NT == 256 ? 3 : NT == 128 ? 4 : NT == 64 ? 5 : 6;
-    static constexpr int BT = NT / 128 > 0 ? NT / 128 : 1;  // scale tiles of B
-    static constexpr uint32_t A_BYTES = 16384, B_BYTES = NT * 128, SFA_BYTES = 2048, SFB_BYTES = 2048 * BT;
-    static constexpr uint32_t OFF_B = A_BYTES, OFF_SFA = OFF_B + B_BYTES, OFF_SFB = OFF_SFA + SFA_BYTES;
+    static constexpr uint32_t S = NT == 256 ? 4 : NT == 128 ? 6 : NT == 64 ? 7 : 9;  // stages
+    static constexpr int BT = NT / 128 > 0 ? NT / 128 : 1;                           // scale tiles of B
+    static constexpr uint32_t B_BYTES = NT * 128, SFB_BYTES = 2048 * BT;
+    static constexpr uint32_t OFF_SFA = kFp4TileCodes, OFF_B = kFp4TileBytes, OFF_SFB = OFF_B + B_BYTES;
     static constexpr uint32_t STAGE = OFF_SFB + SFB_BYTES;
-    static constexpr uint32_t RAW = 2048 + 256 + 64 + 16;  // codes, scales and columns of at most 16 blocks, and their number
-    static constexpr uint32_t OFF_RAW = S * STAGE;
-    static constexpr uint32_t OFF_BAR = OFF_RAW + 8 * EG * RING * RAW;
+    static constexpr uint32_t OFF_BAR = S * STAGE;
     static constexpr uint32_t OFF_MASK = OFF_BAR + 8 * (2 * S + 2);
     static constexpr uint32_t OFF_MISC = OFF_MASK + 4 * S;
-    static constexpr uint32_t SMEM = OFF_MISC + 8 + 1024;
-    static constexpr int THREADS = 256 + EG * 256;
+    static constexpr uint32_t SMEM = OFF_MISC + 12 + 1024;
     static_assert(STAGE % 1024 == 0 && SMEM <= 232448, "shared memory");
 };
+constexpr int kTileThreads = 8 * 32;
 
 template <int NT, int FMT>
-__global__ void __launch_bounds__(Cfg<NT>::THREADS, 1) fp4_tile_kernel(const __grid_constant__ CUtensorMap mapB, const TileArgs a, const Work work) {
+__global__ void __launch_bounds__(kTileThreads, 1) fp4_tile_kernel(const __grid_constant__ CUtensorMap mapB, const TileArgs a, const Work work) {
     using G = Cfg<NT>;
     constexpr uint32_t S = G::S;
     extern __shared__ uint8_t smem_raw[];
@@ -199,12 +167,12 @@ __global__ void __launch_bounds__(Cfg<NT>::THREADS, 1) fp4_tile_kernel(const __g
     auto full = [&](uint32_t s) { return base + G::OFF_BAR + 8 * s; };
     auto empty = [&](uint32_t s) { return base + G::OFF_BAR + 8 * (S + s); };
     const uint32_t acc_full = base + G::OFF_BAR + 16 * S, acc_empty = acc_full + 8;
-    const uint32_t tmem_slot = base + G::OFF_MISC, abort_addr = tmem_slot + 4;
+    const uint32_t tmem_slot = base + G::OFF_MISC, abort_addr = tmem_slot + 4, any_addr = tmem_slot + 8;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
-        for (uint32_t s = 0; s < S; s++) { mbar_init(full(s), 1 + 8); mbar_init(empty(s), 1); }
-        mbar_init(acc_full, 1);
+        for (uint32_t s = 0; s < S; s++) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
+        mbar_init(acc_full, 2);
         mbar_init(acc_empty, 4);
         st_shared_u32(abort_addr, 0);
         fence_barrier_init();
@@ -228,57 +196,66 @@ __global__ void __launch_bounds__(Cfg<NT>::THREADS, 1) fp4_tile_kernel(const __g
         if (lane == 0) {
             bool ok = true;
             while (ok && walk.next(s)) {
-                const Fp4Step* rec = a.steps + s.gs;
-                uint32_t ks = __ldg(&rec[s.k0].kstep), mask = __ldg(&rec[s.k0].mask);
+                const int half = s.t / a.col_tiles, t = s.t - half * a.col_tiles, rt = t * G::BT;
+                const uint32_t b_tiles = (uint32_t)min(G::BT, a.b_row_tiles - rt);
+                const uint2* rec = reinterpret_cast<const uint2*>(a.steps + s.gs);
+                uint2 next = __ldg(rec + s.k0);
                 for (int k = s.k0; k < s.k1; k++, i++) {
-                    const uint32_t st = i % S, stage = base + st * G::STAGE, at = ks, m = mask;
-                    if (k + 1 < s.k1) { ks = __ldg(&rec[k + 1].kstep); mask = __ldg(&rec[k + 1].mask); }
+                    const uint32_t st = i % S, stage = base + st * G::STAGE, ks = next.x, m = next.y >> (4 * half) & 15;
+                    if (k + 1 < s.k1) next = __ldg(rec + k + 1);
                     if (!wait_bar(empty(st), ((i / S) & 1) ^ 1, abort_addr, a.status, 60)) { ok = false; break; }
                     st_shared_u32(base + G::OFF_MASK + 4 * st, m);
-                    if (m == 0) { mbar_arrive(full(st)); continue; }  // a group without blocks
-                    const uint32_t sf = (uint32_t)min(4, a.quads - (int)at * 4) * 512;
-                    const int rt = s.t * G::BT;
-                    const int tiles = min(G::BT, a.b_row_tiles - rt);
-                    mbar_arrive_expect_tx(full(st), G::B_BYTES + sf * tiles);
-                    tma_load_2d(stage + G::OFF_B, &mapB, (int)at * 128, s.t * NT, full(st));
-                    for (int j = 0; j < tiles; j++)
-                        bulk_load(stage + G::OFF_SFB + 2048 * j, a.b_scales + ((size_t)(rt + j) * a.quads + at * 4) * 512, sf, full(st));
+                    if (m == 0) { mbar_arrive(full(st)); continue; }  // nothing in this half
+                    const uint32_t sf = (uint32_t)min(4, a.quads - (int)ks * 4) * 512;
+                    mbar_arrive_expect_tx(full(st), kFp4TileBytes + G::B_BYTES + sf * b_tiles);
+                    bulk_load(stage, a.tiles + ((size_t)(s.gs + k) * 2 + half) * kFp4TileBytes, kFp4TileBytes, full(st));
+                    tma_load_2d(stage + G::OFF_B, &mapB, (int)ks * 128, t * NT, full(st));
+                    for (uint32_t j = 0; j < b_tiles; j++)
+                        bulk_load(stage + G::OFF_SFB + 2048 * j, a.b_scales + ((size_t)(rt + j) * a.quads + ks * 4) * 512, sf, full(st));
                 }
             }
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0) {
-            constexpr uint32_t idesc = idesc_fp4(128, NT, FMT == SMAT_FP4_MX);
-            bool ok = true;
-            uint32_t n = 0;
-            for (; ok && walk.next(s); n++) {
-                ok = wait_bar(acc_empty, (n & 1) ^ 1, abort_addr, a.status, 61);
+        // The whole warp walks, so that what the MMAs are given is uniform; one lane issues.
+        constexpr uint32_t idesc = idesc_fp4(128, NT, FMT == SMAT_FP4_MX);
+        bool ok = true;
+        for (uint32_t n = 0; ok && walk.next(s); n++) {
+            ok = __all_sync(~0u, wait_bar(acc_empty, (n & 1) ^ 1, abort_addr, a.status, 61));
+            tc_fence_after();
+            uint32_t acc = 0;
+            for (int k = s.k0; ok && k < s.k1; k++, i++) {
+                const uint32_t st = i % S, stage = base + st * G::STAGE;
+                ok = __all_sync(~0u, wait_bar(full(st), (i / S) & 1, abort_addr, a.status, 62));
+                if (!ok) break;
                 tc_fence_after();
-                uint32_t acc = 0;
-                for (int k = s.k0; ok && k < s.k1; k++, i++) {
-                    const uint32_t st = i % S, stage = base + st * G::STAGE;
-                    if (!(ok = wait_bar(full(st), (i / S) & 1, abort_addr, a.status, 62))) break;
-                    tc_fence_after();
-                    const uint32_t mask = ld_shared_u32(base + G::OFF_MASK + 4 * st);
-                    const uint32_t sf = tmem + 256 + (i & 1) * 48;
-                    const uint64_t da = smem_desc_k_sw128(stage), db = smem_desc_k_sw128(stage + G::OFF_B);
-                    const uint64_t dsa = desc_scales(stage + G::OFF_SFA), dsb = desc_scales(stage + G::OFF_SFB);
+                const uint32_t mask = uniform(ld_shared_u32(base + G::OFF_MASK + 4 * st));
+                const uint32_t sf = tmem + 256 + (i & 1) * 48;
+                const uint64_t da = smem_desc_k_sw128(stage), db = smem_desc_k_sw128(stage + G::OFF_B);
+                const uint64_t dsa = desc_scales(stage + G::OFF_SFA), dsb = desc_scales(stage + G::OFF_SFB);
+                if (elect_one()) {
+                    uint32_t on = acc;
 #pragma unroll
                     for (uint32_t q = 0; q < 4; q++) {
                         if (!(mask >> q & 1)) continue;
                         cp_scales(sf + q * 4, dsa + q * 32);
 #pragma unroll
                         for (int j = 0; j < G::BT; j++) cp_scales(sf + 16 + q * 8 + j * 4, dsb + q * 32 + j * 128);
-                        mma_fp4<FMT>(tmem, da + q * 2, db + q * 2, idesc, sf + q * 4, sf + 16 + q * 8, acc);
-                        acc = 1;
+                        mma_fp4<FMT>(tmem, da + q * 2, db + q * 2, idesc, sf + q * 4, sf + 16 + q * 8, on);
+                        on = 1;
                     }
                     tc_commit(empty(st));
                 }
-                if (ok) tc_commit(acc_full);
+                acc |= mask;
+                __syncwarp();
             }
+            if (ok && elect_one()) {
+                st_shared_u32(any_addr, acc);
+                tc_commit(acc_full);
+                mbar_arrive(acc_full);
+            }
+            __syncwarp();
         }
-        __syncwarp();
     } else if (warp >= 4 && warp < 8) {
         const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);
         const int row = (warp & 3) * 32 + lane;
@@ -287,8 +264,8 @@ __global__ void __launch_bounds__(Cfg<NT>::THREADS, 1) fp4_tile_kernel(const __g
             if (lane == 0) ok = wait_bar(acc_full, n & 1, abort_addr, a.status, 63);
             if (!__shfl_sync(~0u, ok, 0)) break;
             tc_fence_after();
-            const bool none = s.ns == 1 && __ldg(&a.steps[s.gs].mask) == 0;
-            const int m = s.g * 128 + row, n0 = s.t * NT, cols = min(NT, a.N - n0);
+            const bool none = ld_shared_u32(any_addr) == 0;  // no MMA wrote the accumulators
+            const int half = s.t / a.col_tiles, m = s.g * 256 + half * 128 + row, n0 = (s.t - half * a.col_tiles) * NT, cols = min(NT, a.N - n0);
             float* part = a.scratch + (size_t)s.slot * (128 * NT) + row;
             for (int c = 0; c < cols; c += 16) {
                 uint32_t u[16];
@@ -308,84 +285,6 @@ __global__ void __launch_bounds__(Cfg<NT>::THREADS, 1) fp4_tile_kernel(const __g
             __syncwarp();
             if (lane == 0) mbar_arrive(acc_empty);
         }
-    } else if (warp >= 8) {
-        const int eg = (warp - 8) / 8, e = warp % 8;  // this warp's block-row of the group
-        const uint32_t ring = base + G::OFF_RAW + (uint32_t)(warp - 8) * G::RING * G::RAW;
-        // copies, RING - 1 steps ahead of the laying out
-        Walk fw(work, (int)blockIdx.x);
-        Piece fs;
-        bool more = fw.next(fs);
-        int fk = fs.k0, skip = eg;  // the first group begins with step 0, the second with step 1
-        int nb = 0, nc = 0;
-        auto look = [&]() {  // the block-row's blocks in this warp's next step
-            while (more && fk + skip >= fs.k1) {
-                skip -= fs.k1 - fk;
-                more = fw.next(fs);
-                fk = fs.k0;
-            }
-            if (more) {
-                fk += skip;
-                const Fp4Step* r = a.steps + fs.gs + fk;
-                nb = __ldg(&r->begin[e]);
-                nc = __ldg(&r->count[e]);
-            }
-            skip = G::EG;
-        };
-        uint32_t fetched = 0;
-        auto fetch = [&]() {
-            if (more) {
-                const uint32_t slot = ring + fetched % G::RING * G::RAW;
-                const int p = nb, c = nc;
-                look();
-                const uint8_t* src = a.codes + (size_t)p * 128;
-                for (int j = lane; j < c * 8; j += 32) cp_async16(slot + j * 16, src + j * 16);
-                if (lane < c) {
-                    cp_async16(slot + 2048 + lane * 16, a.scales + ((size_t)p + lane) * 16);
-                    cp_async4(slot + 2304 + lane * 4, a.colidx + p + lane);
-                }
-                if (lane == 0) st_shared_u32(slot + 2368, (uint32_t)c);
-                fetched++;
-            }
-            cp_async_commit();
-        };
-        look();
-        for (int j = 0; j < G::RING - 1; j++) fetch();
-        uint32_t done = 0;
-        bool ok = true;
-        while (ok && walk.next(s)) {
-            for (int k = s.k0; k < s.k1; k++, i++) {
-                if (G::EG > 1 && (int)(i % G::EG) != eg) continue;
-                fetch();
-                cp_async_wait<G::RING - 1>();
-                const uint32_t st = i % S, stage = base + st * G::STAGE;
-                int go = 1;
-                if (lane == 0) go = wait_bar(empty(st), ((i / S) & 1) ^ 1, abort_addr, a.status, 64);
-                if (!__shfl_sync(~0u, go, 0)) { ok = false; break; }
-                __syncwarp();
-                const uint32_t slot = ring + done % G::RING * G::RAW;
-                const uint32_t c = ld_shared_u32(slot + 2368);
-                const uint32_t rows = stage + (uint32_t)e * 2048;                                   // 16 rows of 128 bytes
-                const uint32_t sfa = stage + G::OFF_SFA + (uint32_t)(e & 1) * 256 + (uint32_t)(e >> 1) * 4;  // of row 0: + 16 a row, + 512 a quad
-                if (c < 16) {
-#pragma unroll
-                    for (int j = 0; j < 4; j++) st_shared_zero16(rows + (j * 32 + lane) * 16);
-                    st_shared_u32(sfa + (lane & 15) * 16 + (lane >> 4) * 512, 0);
-                    st_shared_u32(sfa + (lane & 15) * 16 + (lane >> 4) * 512 + 1024, 0);
-                    __syncwarp();
-                }
-                const uint32_t r = lane & 15;
-                for (uint32_t b = lane >> 4; b < c; b += 2) {
-                    const uint32_t cb = ld_shared_u32(slot + 2304 + b * 4) >> 4 & 15;  // block-column of the step
-                    st_shared_v2(rows + r * 128 + (((cb >> 1) ^ (r & 7)) << 4) + (cb & 1) * 8, ld_shared_v2(slot + b * 128 + r * 8));
-                    st_shared_u8(sfa + r * 16 + (cb >> 2) * 512 + (FMT == SMAT_FP4_NV ? cb & 3 : cb >> 1 & 1), ld_shared_u8(slot + 2048 + b * 16 + r));
-                }
-                fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(full(st));
-                done++;
-            }
-        }
-        cp_async_wait<0>();
     }
 
     tc_fence_before();
@@ -413,7 +312,7 @@ __global__ void __launch_bounds__(256) fp4_join_kernel(const TileArgs a, const W
     const long long before = work.begin(c - 1);
     if (b >= work.total || b == u0 || before > u0) return;
     const int row = threadIdx.x % 128, h = threadIdx.x / 128;
-    const int n0 = t * NT + c0 + h * 16, m = g * 128 + row;
+    const int half = t / a.col_tiles, n0 = (t - half * a.col_tiles) * NT + c0 + h * 16, m = g * 256 + half * 128 + row;
     float v[16];
 #pragma unroll
     for (int j = 0; j < 16; j++) v[j] = 0.f;
@@ -434,7 +333,8 @@ int launch_tile(const TileArgs& args, const CUtensorMap& map, Work work, size_t 
     TileArgs a = args;
     const cudaError_t attr = cudaFuncSetAttribute(fp4_tile_kernel<NT, FMT>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM);
     if (attr != cudaSuccess) return fail(SMAT_ERR_CUDA, "cudaFuncSetAttribute failed: %s", cudaGetErrorString(attr));
-    work.tiles = (a.N + NT - 1) / NT;
+    a.col_tiles = (a.N + NT - 1) / NT;
+    work.tiles = 2 * a.col_tiles;  // of each half of a group
     work.total = (long long)total * work.tiles;
     // a CTA for every SM, but not below four steps each
     work.parts = (int)(work.total / 4 < ctx->sm_count ? (work.total / 4 > 0 ? work.total / 4 : 1) : ctx->sm_count);
@@ -443,7 +343,7 @@ int launch_tile(const TileArgs& args, const CUtensorMap& map, Work work, size_t 
         SMAT_CUDA_TRY(cudaMallocFromPoolAsync(&scratch, (size_t)work.parts * 2 * 128 * NT * sizeof(float), ctx->pool, stream));
         a.scratch = static_cast<float*>(scratch);
     }
-    fp4_tile_kernel<NT, FMT><<<work.parts, G::THREADS, G::SMEM, stream>>>(map, a, work);
+    fp4_tile_kernel<NT, FMT><<<work.parts, kTileThreads, G::SMEM, stream>>>(map, a, work);
     cudaError_t e = cudaGetLastError();
     count_launch();
     if (e == cudaSuccess && work.parts > 1) {
@@ -473,10 +373,8 @@ int launch_fp4_tile(const Fp4View& A, const Fp4Rhs& B, void* C, int c_dtype, siz
     const size_t pitch = fp4_pitch(A.K);
     if (int rc = encode_tensor_map_2d_u8(&map, B.data, pitch, N, pitch, 128, (uint32_t)nt)) return rc;
     TileArgs a = {};
-    a.codes = A.codes;
-    a.scales = A.scales;
-    a.colidx = A.colidx;
     a.steps = A.steps;
+    a.tiles = A.tiles;
     a.b_scales = B.scales;
     a.row_scale = A.row_scale ? A.row_scale + A.brow_begin * 16 : nullptr;
     a.b_row_scale = B.row_scale;
@@ -489,7 +387,7 @@ int launch_fp4_tile(const Fp4View& A, const Fp4Rhs& B, void* C, int c_dtype, siz
     a.b_row_tiles = (int)((N + 127) / 128);
     Work work = {};
     work.gsp = A.gsp;
-    work.groups = (int)((A.block_rows + 7) / 8);
+    work.groups = (int)((A.block_rows + kFp4GroupRows - 1) / kFp4GroupRows);
     switch (nt) {
         case 32: return launch_tile_format<32>(A.fmt, a, map, work, A.total_steps, ctx, stream);
         case 64: return launch_tile_format<64>(A.fmt, a, map, work, A.total_steps, ctx, stream);

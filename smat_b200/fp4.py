@@ -31,7 +31,8 @@ def _lib():
         L.smat_fp4_dequantize.argtypes = [vp, vp, vp, i, sz, sz, vp, i, sz, vp]
         L.smat_fp4_quantize_blocks.argtypes = [vp, i, vp, vp, sz, sz, i, vp, vp, vp, vp]
         L.smat_fp4_dequantize_blocks.argtypes = [vp, vp, vp, i, vp, sz, sz, vp, i, vp]
-        L.smat_fp4_plan_create.argtypes = [C.POINTER(vp), vp, vp, vp, i, vp, vp, sz, sz, sz, sz, sz, vp]
+        L.smat_fp4_plan_create.argtypes = [C.POINTER(vp), vp, vp, vp, i, vp, vp, sz, sz, sz, sz, sz, i, vp]
+        L.smat_fp4_plan_set_values.argtypes = [vp, vp]
         L.smat_fp4_plan_spmm.argtypes = [vp, vp, i, vp, sz, vp]
         L.smat_fp4_plan_spmm_fp4.argtypes = [vp, vp, vp, vp, i, vp, i, sz, vp]
         L.smat_fp4_plan_destroy.argtypes = [vp]
@@ -239,10 +240,11 @@ class Fp4SparseMatrix:
 
 
 class Fp4Plan:
-    """Plan for products of block-rows [brow_begin, brow_end) of an Fp4SparseMatrix (smat_fp4_plan_*).  Codes and scales of the
-    matrix may change in place, its structure may not; products do not change the plan and may run on several streams at a time."""
+    """Plan for products of block-rows [brow_begin, brow_end) of an Fp4SparseMatrix (smat_fp4_plan_*).  ``tiles=False``: only for
+    products with 16-bit B (decoding); those with B in 4 bits work but are slow, and the plan takes next to no memory.  Products do
+    not change the plan and may run on several streams at a time."""
 
-    def __init__(self, A, brow_begin=0, brow_end=None):
+    def __init__(self, A, brow_begin=0, brow_end=None, tiles=True):
         self.A = A
         self.brow_begin = brow_begin
         self.brow_end = A.M // 16 if brow_end is None else brow_end
@@ -252,10 +254,16 @@ class Fp4Plan:
         L = _lib()
         _check(L.smat_fp4_plan_create(C.byref(h), A.codes.data_ptr(), A.scales.data_ptr(), _ptr(A.row_scale), _FORMATS[A.fmt],
                                       A.bcsrRowPtr.data_ptr(), A.bcsrColIdx.data_ptr(), A.M, A.K, A.nnzb, self.brow_begin,
-                                      self.brow_end, _stream()))
+                                      self.brow_end, int(tiles), _stream()))
         self._h = h
         self._rows = (self.brow_end - self.brow_begin) * 16
         self._device = A.bcsrRowPtr.device
+
+    def set_values(self):
+        """After A's codes or scales changed (same structure)."""
+        if self._h is None:
+            _refuse("the plan is closed")
+        _check(_LIB.smat_fp4_plan_set_values(self._h, _stream()))
 
     def spmm(self, B, Cout, check=False):
         """C = A x B.  B: Matrix / tensor [N, K] in fp16 or bf16 with C of the same type, or an Fp4Matrix of A's format with C in

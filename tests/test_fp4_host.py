@@ -89,7 +89,7 @@ def test_c_refusals_of_blocks_and_plans():
     assert d(P, P, None, 3, P, 32, 1, P, 0, None) == BAD
     assert d(P, P, None, 0, P, 32, 1, None, 0, None) == BAD
     h = C.c_void_p()
-    good = [P, P, None, 0, P, P, 64, 64, 3, 0, 4]
+    good = [P, P, None, 0, P, P, 64, 64, 3, 0, 4, 1]
 
     def rc(**kw):
         a = list(good)
@@ -97,10 +97,11 @@ def test_c_refusals_of_blocks_and_plans():
             a[int(k[1:])] = v
         return L.smat_fp4_plan_create(C.byref(h), *a, None)
     for kw, code in [(dict(a0=None), BAD), (dict(a1=None), BAD), (dict(a0=P + 8), BAD), (dict(a3=2), BAD), (dict(a4=None), BAD), (dict(a5=None), BAD),
-                     (dict(a6=40), BAD), (dict(a7=40), BAD), (dict(a9=3, a10=2), BAD), (dict(a10=5), BAD), (dict(a8=1 << 27), RANGE), (dict(a7=1 << 31), RANGE)]:
+                     (dict(a6=40), BAD), (dict(a7=40), BAD), (dict(a9=3, a10=2), BAD), (dict(a10=5), BAD), (dict(a8=1 << 27), RANGE), (dict(a7=1 << 31), RANGE), (dict(a7=1 << 26), RANGE)]:
         assert rc(**kw) == code and not h.value, kw
     assert L.smat_fp4_plan_create(None, *good, None) == BAD
     assert L.smat_fp4_plan_spmm(None, P, 0, P, 8, None) == BAD
     assert L.smat_fp4_plan_spmm(None, P, 2, P, 8, None) == BAD
     assert L.smat_fp4_plan_spmm_fp4(None, P, P, None, 0, P, 0, 8, None) == BAD
+    assert L.smat_fp4_plan_set_values(None, None) == BAD
     assert L.smat_fp4_plan_destroy(None) == 0

@@ -86,7 +86,7 @@ def test_16bit(fmt, dtype, counts, Kb, N):
 
 @pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
-@pytest.mark.parametrize("counts,Kb", SHAPES + [([100] * 40, 130)])
+@pytest.mark.parametrize("counts,Kb", SHAPES + [([100] * 40, 130), ([16] * 3 + [0] * 40 + [13] * 10 + [0] * 30, 16), ([0] * 9 + [12], 12), ([5] * 300, 48)])
 @pytest.mark.parametrize("N", [1, 8, 31, 64, 129, 300])
 def test_4bit(fmt, dtype, counts, Kb, N):
     c = Case(N + Kb, counts, Kb, fmt)
@@ -148,15 +148,29 @@ def test_scale_nan_of_a_row_makes_nan(four):
     assert bad[5] and bad.sum() == 1 and not bool(torch.isnan(C[:5]).any())
 
 
-def test_values_change_in_place():
+@pytest.mark.parametrize("four", [False, True])
+def test_values_change(four):
     c = Case(8, [5, 9, 2], 11, "nvfp4")
     plan = S.Fp4Plan(c.A)
-    x = c.acts(5, torch.float16)
+    x = c.acts4(5)[0] if four else c.acts(5, torch.float16)
     C, D = (torch.empty((c.M, 5), dtype=torch.float16, device="cuda") for _ in range(2))
     plan.spmm(x, C)
     c.A.codes ^= 0x88  # all signs
+    plan.set_values()
     plan.spmm(x, D)
     assert torch.equal(C, -D)
+
+
+@pytest.mark.parametrize("N", [1, 9, 40, 130])
+@pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
+def test_4bit_without_tiles(N, fmt):
+    """Plans made without tiles, and those of scattered blocks, which have none either."""
+    for counts, Kb, tiles in [([3, 0, 17, 1, 40], 40, False), ([2] * 40, 2000, True)]:
+        c = Case(N, counts, Kb, fmt)
+        B, b = c.acts4(N)
+        C = torch.full((c.M, N), float("nan"), dtype=torch.bfloat16, device="cuda")
+        S.Fp4Plan(c.A, tiles=tiles).spmm(B, C, check=True)
+        _close(C, *F.multiply(c.vals, c.rowptr, c.colidx, b), c.longest)
 
 
 @pytest.mark.parametrize("four", [False, True])
