@@ -50,6 +50,7 @@ struct Fp4View {
     const Fp4Step* steps = nullptr;  // null: the plan has no tiles
     const uint8_t* tiles = nullptr;  // two of a step
     const int* gsp = nullptr;        // first step of every group, and the number of all
+    const int* h_gsp = nullptr;      // the same on the host
     size_t total_steps = 0;
     size_t blocks = 0, longest = 0;  // stored blocks of the range, and of its longest block-row
 };

@@ -11,6 +11,7 @@ struct smat_fp4_plan {
     void* steps = nullptr;   // steps and what their tiles are made of
     smat::Fp4Where* where = nullptr;
     void* tiles = nullptr;
+    int* gsp = nullptr;  // first steps on the host
 };
 
 namespace smat {
@@ -185,7 +186,11 @@ int build_plan(smat_fp4_plan* p, const int* rowptr, const int* colidx, size_t nn
     fp4_steps_kernel<true><<<(unsigned)groups, kStepThreads, words * 8, stream>>>(range, colidx, (int)v.block_rows, words, gsp, step, p->where);
     count_launch();
     SMAT_CUDA_TRY(cudaGetLastError());
+    p->gsp = new (std::nothrow) int[groups + 1];
+    if (!p->gsp) return fail(SMAT_ERR_NOMEM, "out of host memory");
+    SMAT_CUDA_TRY(cudaMemcpyAsync(p->gsp, gsp, (groups + 1) * sizeof(int), cudaMemcpyDeviceToHost, stream));
     v.gsp = gsp;
+    v.h_gsp = p->gsp;
     v.total_steps = steps;
     v.steps = step;
     v.tiles = static_cast<const uint8_t*>(p->tiles);
@@ -200,6 +205,7 @@ cudaError_t free_plan(smat_fp4_plan* p) {
         const cudaError_t f = cudaFree(m);
         if (e == cudaSuccess) e = f;
     }
+    delete[] p->gsp;
     delete p;
     return e;
 }

@@ -9,11 +9,16 @@
 // Steps of 256 columns in which a group of two tiles holds no block are left out, and so are MMAs of 64 columns without one.  (Laying
 // the blocks out in shared memory instead, from the 144 bytes each, was measured first: 950 us for the layer 8192 x 28672 at 20 %,
 // N = 4096; the hand-overs between copying, laying out and multiplying warps took 700 cycles a step alone.)
+// Beyond 128 columns of C two CTAs share a tile of 256 x 256 (cta_group::2): each holds 128 rows of A and 128 columns of B, so an SM
+// fetches 38 KB a step of 512 cycles of MMAs instead of 54; L2 delivers about 70 bytes a cycle and SM.
 //
-// Roles.  One thread fetches the tiles (bulk copies), B (tiled TMA copies with 128-byte swizzle) and its scales; one thread moves the
-// scales to tensor memory and issues the MMAs; four warps store finished tiles of C.  The (tile of C, step) pairs are dealt out in
-// equal contiguous ranges, one per CTA; tiles that a range boundary falls into are joined from fp32 parts in a fixed order by a
-// second kernel.  All waits are bounded.
+// Roles.  One thread fetches tiles of A (bulk copies), B (tiled TMA copies with 128-byte swizzle) and its scales; one moves the scales
+// to tensor memory (24 cycles for each of 12 copies a step: as long as issuing the MMAs takes, so it is not the same thread), one
+// issues the MMAs; eight warps store finished tiles of C through shared memory, whole 128-byte lines at a time.  Of a pair, the second
+// CTA only fetches and stores.  The (tile of C, step) pairs are dealt out in equal contiguous ranges, worked out on the host; tiles
+// that a range boundary falls into are joined from fp32 parts in a fixed order by a second kernel.  All waits are bounded.
+#include <algorithm>
+
 #include "fp4_device.cuh"
 #include "ptx_sm100.cuh"
 #include "smat_internal.h"
@@ -24,88 +29,126 @@ namespace {
 
 using namespace ptx;
 
-// ---- tcgen05 with block scales --------------------------------------------------------------------------------------------------
+// ---- tcgen05 with block scales; CG: CTAs of the group (cta_group::1 or ::2) -----------------------------------------------------
 // Instruction descriptor: e2m1 A and B (format 1 in bits [7,10) and [10,13)), N >> 3 in [17,23), bit 23: e8m0 scales (else e4m3),
 // M >> 4 in [24,29); bytes 0.. of the scale words are used (scale ids 0).
 __host__ __device__ constexpr uint32_t idesc_fp4(int m, int n, bool e8m0) {
     return (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((e8m0 ? 1u : 0u) << 23) | ((uint32_t)(m >> 4) << 24);
 }
-template <int FMT>
+template <int FMT, int CG>
 __device__ __forceinline__ void mma_fp4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
-    if constexpr (FMT == SMAT_FP4_NV)
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
-            "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-            : "memory");
-    else
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
-            "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-            : "memory");
+#define SMAT_MMA_FP4(cg, kind)                                                                                  \
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"                                              \
+                 "tcgen05.mma.cta_group::" cg ".kind::" kind " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d), \
+                 "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)                                \
+                 : "memory")
+    if constexpr (FMT == SMAT_FP4_NV && CG == 1) SMAT_MMA_FP4("1", "mxf4nvf4.block_scale.scale_vec::4X");
+    else if constexpr (FMT == SMAT_FP4_NV) SMAT_MMA_FP4("2", "mxf4nvf4.block_scale.scale_vec::4X");
+    else if constexpr (CG == 1) SMAT_MMA_FP4("1", "mxf4.block_scale.scale_vec::2X");
+    else SMAT_MMA_FP4("2", "mxf4.block_scale.scale_vec::2X");
+#undef SMAT_MMA_FP4
 }
-// 32 rows of 16 bytes (a scale tile of 512 bytes) to four columns of tensor memory, the same in all four lane quarters.
+// 32 rows of 16 bytes (a scale tile of 512 bytes) to four columns of tensor memory, the same in all four lane quarters; of a pair,
+// in both CTAs, from the shared memory of each.
+template <int CG>
 __device__ __forceinline__ void cp_scales(uint32_t taddr, uint64_t desc) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+    if constexpr (CG == 1) asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+    else asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
 // Descriptor of such a tile: no swizzle, groups of 8 rows x 16 bytes 128 bytes apart.
 __device__ __forceinline__ uint64_t desc_scales(uint32_t smem_addr) {
     return (uint64_t)((smem_addr >> 4) & 0x3FFFu) | (8ull << 16) | (8ull << 32) | (1ull << 46);
 }
+// Arrives on this CTA's barrier once every tcgen05 operation issued so far by this thread has completed; BOTH: on that of both CTAs.
+template <int CG, bool BOTH>
+__device__ __forceinline__ void commit(uint32_t bar) {
+    if constexpr (CG == 1) tc_commit(bar);
+    else if constexpr (!BOTH) asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .b16 m;\n\tmov.b16 m, 3;\n\t"
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], m;\n\t}" ::"r"(bar)
+            : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void alloc_all(uint32_t dst_smem) {
+    if constexpr (CG == 1) {
+        tmem_alloc(dst_smem, 512);
+        tmem_relinquish();
+    } else {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(dst_smem) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+}
+template <int CG>
+__device__ __forceinline__ void dealloc_all(uint32_t taddr) {
+    if constexpr (CG == 1) tmem_dealloc(taddr, 512);
+    else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(taddr) : "memory");
+}
+
+// ---- the two CTAs of a pair -----------------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+// Arrives on the barrier at the same place of the first CTA's shared memory.
+__device__ __forceinline__ void arrive_at_first(uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %0, 0;\n\t"
+        "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [r];\n\t}" ::"r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void fence_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
+
+__device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ uint16_t ld_shared_u16(uint32_t addr) {
+    uint16_t v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr) : "memory");
+    return v;
+}
+
 // ---- schedule -------------------------------------------------------------------------------------------------------------------
-// Positions: the steps of a tile of C after one another, tiles of a group of block-rows after one another, groups after one another.
-struct Work {
-    const int* gsp;
-    int groups, tiles, parts;
-    long long total;
-    __device__ __forceinline__ long long first(int g) const { return (long long)__ldg(gsp + g) * tiles; }
-    __device__ __forceinline__ int group_of(long long p) const {
-        int lo = 0, hi = groups - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (first(mid) <= p) lo = mid; else hi = mid - 1;
-        }
-        return lo;
-    }
-    // First position of CTA c's range.  Where a CTA has eight tiles or more its range begins with one: a cut tile goes through
-    // memory in fp32, which costs more than being off the equal share by half a tile.
-    __device__ __forceinline__ long long begin(int c) const {
-        if (c >= parts) return total;
-        const long long p = total * c / parts;
-        const int g = group_of(p), ns = __ldg(gsp + g + 1) - __ldg(gsp + g);
-        if ((long long)ns * 8 * parts > total) return p;
-        const long long off = (p - first(g)) % ns;
-        return 2 * off <= ns ? p - off : p - off + ns;
-    }
+// Units: tiles of C, those of a group of block-rows one after another.  A part is what a CTA (or pair) works on: from one start to the
+// next.  Worked out on the host and handed over as a kernel parameter: looked up on the device, five dependent loads at a time, it
+// took 7 us of every launch and 18 us of the joining kernel.
+struct Start {
+    int g, t, k;  // group, unit of the group, step of the unit
 };
-struct Piece {  // steps [k0, k1) of the ns steps of tile (g, t)
+constexpr int kMaxParts = 160;
+struct Schedule {
+    Start at[kMaxParts + 1];
+    int parts, units;  // units of a group
+};
+struct Piece {  // steps [k0, k1) of the ns steps of unit (g, t)
     int g, t, k0, k1, gs, ns, slot;
     bool cut;
 };
 struct Walk {
-    Work w;
-    long long p, p_begin, p_end;
-    int g;
-    __device__ __forceinline__ Walk(const Work& work, int c) : w(work) {
-        p = p_begin = w.begin(c);
-        p_end = w.begin(c + 1);
-        g = p < p_end ? w.group_of(p) : 0;
-    }
-    __device__ __forceinline__ bool next(Piece& s) {
-        if (p >= p_end) return false;
-        while (w.first(g + 1) <= p) g++;
-        s.g = g;
-        s.gs = __ldg(w.gsp + g);
-        s.ns = __ldg(w.gsp + g + 1) - s.gs;
-        const long long off = p - w.first(g);
-        s.t = (int)(off / s.ns);
-        s.k0 = (int)(off - (long long)s.t * s.ns);
-        const long long left = p_end - p;
-        s.k1 = left < s.ns - s.k0 ? s.k0 + (int)left : s.ns;
-        s.cut = s.k0 != 0 || s.k1 != s.ns;
-        s.slot = 2 * (int)blockIdx.x + (p_begin < p - s.k0 ? 1 : 0);
-        p += s.k1 - s.k0;
+    const int* gsp;
+    Start now, end;
+    int units, slot;
+    __device__ __forceinline__ Walk(const Schedule& s, const int* first_steps, int part)
+        : gsp(first_steps), now(s.at[part]), end(s.at[part + 1]), units(s.units), slot(2 * part) {}
+    __device__ __forceinline__ bool next(Piece& p) {
+        const bool last = now.g == end.g && now.t == end.t;
+        if (last && now.k == end.k) return false;
+        p.gs = __ldg(gsp + now.g);
+        p.ns = __ldg(gsp + now.g + 1) - p.gs;
+        p.g = now.g;
+        p.t = now.t;
+        p.k0 = now.k;
+        p.k1 = last ? end.k : p.ns;
+        p.cut = p.k0 != 0 || p.k1 != p.ns;
+        p.slot = slot;
+        slot |= 1;  // for a unit that begins inside the part
+        now.k = last ? end.k : 0;
+        if (!last && ++now.t == units) { now.t = 0; now.g++; }
         return true;
     }
 };
@@ -113,6 +156,7 @@ struct Walk {
 struct TileArgs {
     const Fp4Step* steps;
     const uint8_t* tiles;
+    const int* gsp;
     const uint8_t* b_scales;
     const float* row_scale;  // first of the range, or null
     const float* b_row_scale;
@@ -122,168 +166,248 @@ struct TileArgs {
     int c_dtype, rows, N, quads, b_row_tiles, col_tiles;
 };
 
-// 16 values of row m from column n on (those below N), scaled, to C.
-__device__ __forceinline__ void store_row16(const TileArgs& a, int m, int n, const float (&v)[16]) {
-    float o[16];
-    const float rs = a.row_scale ? __ldg(a.row_scale + m) : 1.f;
-#pragma unroll
-    for (int i = 0; i < 16; i++) {
-        o[i] = v[i] * rs;
-        if (a.b_row_scale) o[i] *= n + i < a.N ? __ldg(a.b_row_scale + n + i) : 0.f;
-    }
-    const size_t at = (size_t)m * a.N + n;
-    if (a.N % 8 == 0 && n + 16 <= a.N) {
-        if (a.c_dtype == SMAT_F16) store16<SMAT_F16>(static_cast<__half*>(a.C) + at, o);
-        else store16<SMAT_BF16>(static_cast<__nv_bfloat16*>(a.C) + at, o);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; i++)
-            if (n + i < a.N) store_c(a.C, a.c_dtype, at + i, o[i]);
-    }
-}
-
-// NT columns of C per tile.
+// NT columns of C per tile; a pair of CTAs (CG 2) for 256.
 template <int NT>
 struct Cfg {
-    static constexpr uint32_t S = NT == 256 ? 4 : NT == 128 ? 6 : NT == 64 ? 7 : 9;  // stages
-    static constexpr int BT = NT / 128 > 0 ? NT / 128 : 1;                           // scale tiles of B
-    static constexpr uint32_t B_BYTES = NT * 128, SFB_BYTES = 2048 * BT;
+    static constexpr int CG = NT == 256 ? 2 : 1;
+    static constexpr uint32_t S = NT == 64 ? 6 : NT == 32 ? 7 : 5;  // stages
+    static constexpr uint32_t NB = NT / CG;                         // columns of C whose part of B this CTA fetches
+    static constexpr int BT = NT > 128 ? NT / 128 : 1;              // scale tiles of B
+    static constexpr uint32_t B_BYTES = NB * 128, SFB_BYTES = 2048 * BT;
     static constexpr uint32_t OFF_SFA = kFp4TileCodes, OFF_B = kFp4TileBytes, OFF_SFB = OFF_B + B_BYTES;
     static constexpr uint32_t STAGE = OFF_SFB + SFB_BYTES;
-    static constexpr uint32_t OFF_BAR = S * STAGE;
-    static constexpr uint32_t OFF_MASK = OFF_BAR + 8 * (2 * S + 2);
+    static constexpr uint32_t SF_COLUMNS = 16 + 16 * BT;            // tensor memory of a stage's scales
+    static constexpr uint32_t ACC = NT == 256 ? 1 : 2;              // accumulators
+    static constexpr uint32_t OFF_OUT = S * STAGE;                  // 32 rows x 64 columns for each storing warp
+    static constexpr uint32_t OFF_COL = OFF_OUT + 8 * 4096;         // and the scales of these columns
+    static constexpr uint32_t OFF_BAR = OFF_COL + 8 * 256;
+    static constexpr uint32_t OFF_MASK = OFF_BAR + 8 * (4 * S + 4);
     static constexpr uint32_t OFF_MISC = OFF_MASK + 4 * S;
-    static constexpr uint32_t SMEM = OFF_MISC + 12 + 1024;
+    static constexpr uint32_t SMEM = OFF_MISC + 16 + 1024;
     static_assert(STAGE % 1024 == 0 && SMEM <= 232448, "shared memory");
+    static_assert(ACC * NT <= 256 && 256 + S * SF_COLUMNS <= 512, "tensor memory");
 };
-constexpr int kTileThreads = 8 * 32;
+constexpr int kTileThreads = 12 * 32;
 
 template <int NT, int FMT>
-__global__ void __launch_bounds__(kTileThreads, 1) fp4_tile_kernel(const __grid_constant__ CUtensorMap mapB, const TileArgs a, const Work work) {
+__global__ void __launch_bounds__(kTileThreads, 1)
+fp4_tile_kernel(const __grid_constant__ CUtensorMap mapB, const __grid_constant__ TileArgs a, const __grid_constant__ Schedule plan) {
     using G = Cfg<NT>;
     constexpr uint32_t S = G::S;
+    constexpr int CG = G::CG;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    auto full = [&](uint32_t s) { return base + G::OFF_BAR + 8 * s; };
-    auto empty = [&](uint32_t s) { return base + G::OFF_BAR + 8 * (S + s); };
-    const uint32_t acc_full = base + G::OFF_BAR + 16 * S, acc_empty = acc_full + 8;
+    const uint32_t bar = base + G::OFF_BAR;
+    auto full = [&](uint32_t s) { return bar + 8 * s; };              // this CTA's operands have arrived
+    auto empty = [&](uint32_t s) { return bar + 8 * (S + s); };       // ... and been used
+    auto scaled = [&](uint32_t s) { return bar + 8 * (2 * S + s); };  // the scales are in tensor memory
+    auto full2 = [&](uint32_t s) { return bar + 8 * (3 * S + s); };   // the second CTA's operands have arrived
+    auto acc_full = [&](uint32_t b) { return bar + 8 * (4 * S + b); };
+    auto acc_empty = [&](uint32_t b) { return bar + 8 * (4 * S + 2 + b); };
     const uint32_t tmem_slot = base + G::OFF_MISC, abort_addr = tmem_slot + 4, any_addr = tmem_slot + 8;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = CG == 2 ? cluster_rank() : 0;
 
     if (threadIdx.x == 0) {
-        for (uint32_t s = 0; s < S; s++) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
-        mbar_init(acc_full, 2);
-        mbar_init(acc_empty, 4);
+        for (uint32_t s = 0; s < S; s++) { mbar_init(full(s), 1); mbar_init(empty(s), 1); mbar_init(scaled(s), 1); mbar_init(full2(s), 1); }
+        for (uint32_t b = 0; b < 2; b++) { mbar_init(acc_full(b), CG == 1 ? 2 : 1); mbar_init(acc_empty(b), 8 * CG); }
         st_shared_u32(abort_addr, 0);
         fence_barrier_init();
         fence_proxy_async();
         prefetch_tensormap(&mapB);
     }
-    if (warp == 1) {
-        tmem_alloc(tmem_slot, 512);
-        tmem_relinquish();
-    }
+    if (warp == 1) alloc_all<CG>(tmem_slot);
     tc_fence_before();
     __syncthreads();
+    if (CG == 2) cluster_sync();
     tc_fence_after();
     const uint32_t tmem = ld_shared_u32(tmem_slot);
 
-    Walk walk(work, (int)blockIdx.x);
+    Walk walk(plan, a.gsp, (int)blockIdx.x / CG);
     Piece s;
     uint32_t i = 0;  // steps so far
+
+    // Half of the group and tile column of a unit; a pair takes both halves.
+    auto half_of = [&](int t) { return CG == 2 ? (int)rank : t / a.col_tiles; };
+    auto column_of = [&](int t) { return CG == 2 ? t : t % a.col_tiles; };
 
     if (warp == 0) {
         if (lane == 0) {
             bool ok = true;
             while (ok && walk.next(s)) {
-                const int half = s.t / a.col_tiles, t = s.t - half * a.col_tiles, rt = t * G::BT;
+                const int half = half_of(s.t), t = column_of(s.t), rt = t * G::BT;
                 const uint32_t b_tiles = (uint32_t)min(G::BT, a.b_row_tiles - rt);
                 const uint2* rec = reinterpret_cast<const uint2*>(a.steps + s.gs);
                 uint2 next = __ldg(rec + s.k0);
                 for (int k = s.k0; k < s.k1; k++, i++) {
-                    const uint32_t st = i % S, stage = base + st * G::STAGE, ks = next.x, m = next.y >> (4 * half) & 15;
+                    const uint32_t st = i % S, stage = base + st * G::STAGE, ks = next.x;
+                    const uint32_t m = CG == 2 ? (next.y | next.y >> 4) & 15 : next.y >> (4 * half) & 15;
                     if (k + 1 < s.k1) next = __ldg(rec + k + 1);
                     if (!wait_bar(empty(st), ((i / S) & 1) ^ 1, abort_addr, a.status, 60)) { ok = false; break; }
                     st_shared_u32(base + G::OFF_MASK + 4 * st, m);
-                    if (m == 0) { mbar_arrive(full(st)); continue; }  // nothing in this half
+                    if (m == 0) { mbar_arrive(full(st)); continue; }  // no blocks here
                     const uint32_t sf = (uint32_t)min(4, a.quads - (int)ks * 4) * 512;
                     mbar_arrive_expect_tx(full(st), kFp4TileBytes + G::B_BYTES + sf * b_tiles);
                     bulk_load(stage, a.tiles + ((size_t)(s.gs + k) * 2 + half) * kFp4TileBytes, kFp4TileBytes, full(st));
-                    tma_load_2d(stage + G::OFF_B, &mapB, (int)ks * 128, t * NT, full(st));
+                    tma_load_2d(stage + G::OFF_B, &mapB, (int)ks * 128, t * NT + (CG == 2 ? (int)(rank * G::NB) : 0), full(st));
                     for (uint32_t j = 0; j < b_tiles; j++)
                         bulk_load(stage + G::OFF_SFB + 2048 * j, a.b_scales + ((size_t)(rt + j) * a.quads + ks * 4) * 512, sf, full(st));
                 }
             }
         }
         __syncwarp();
-    } else if (warp == 1) {
+    } else if (warp == 1 && rank == 0) {
         // The whole warp walks, so that what the MMAs are given is uniform; one lane issues.
-        constexpr uint32_t idesc = idesc_fp4(128, NT, FMT == SMAT_FP4_MX);
+        constexpr uint32_t idesc = idesc_fp4(128 * CG, NT, FMT == SMAT_FP4_MX);
         bool ok = true;
         for (uint32_t n = 0; ok && walk.next(s); n++) {
-            ok = __all_sync(~0u, wait_bar(acc_empty, (n & 1) ^ 1, abort_addr, a.status, 61));
+            const uint32_t buf = n % G::ACC;
+            ok = __all_sync(~0u, wait_bar(acc_empty(buf), ((n / G::ACC) & 1) ^ 1, abort_addr, a.status, 61));
+            if (CG == 2) fence_cluster();
             tc_fence_after();
             uint32_t acc = 0;
             for (int k = s.k0; ok && k < s.k1; k++, i++) {
                 const uint32_t st = i % S, stage = base + st * G::STAGE;
-                ok = __all_sync(~0u, wait_bar(full(st), (i / S) & 1, abort_addr, a.status, 62));
+                ok = __all_sync(~0u, wait_bar(scaled(st), (i / S) & 1, abort_addr, a.status, 62));
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t mask = uniform(ld_shared_u32(base + G::OFF_MASK + 4 * st));
-                const uint32_t sf = tmem + 256 + (i & 1) * 48;
+                const uint32_t sf = tmem + 256 + st * G::SF_COLUMNS;
                 const uint64_t da = smem_desc_k_sw128(stage), db = smem_desc_k_sw128(stage + G::OFF_B);
-                const uint64_t dsa = desc_scales(stage + G::OFF_SFA), dsb = desc_scales(stage + G::OFF_SFB);
                 if (elect_one()) {
                     uint32_t on = acc;
 #pragma unroll
                     for (uint32_t q = 0; q < 4; q++) {
                         if (!(mask >> q & 1)) continue;
-                        cp_scales(sf + q * 4, dsa + q * 32);
-#pragma unroll
-                        for (int j = 0; j < G::BT; j++) cp_scales(sf + 16 + q * 8 + j * 4, dsb + q * 32 + j * 128);
-                        mma_fp4<FMT>(tmem, da + q * 2, db + q * 2, idesc, sf + q * 4, sf + 16 + q * 8, on);
+                        mma_fp4<FMT, CG>(tmem + buf * NT, da + q * 2, db + q * 2, idesc, sf + q * 4, sf + 16 + q * 4 * G::BT, on);
                         on = 1;
                     }
-                    tc_commit(empty(st));
+                    commit<CG, true>(empty(st));
                 }
                 acc |= mask;
                 __syncwarp();
             }
             if (ok && elect_one()) {
-                st_shared_u32(any_addr, acc);
-                tc_commit(acc_full);
-                mbar_arrive(acc_full);
+                if (CG == 1) st_shared_u32(any_addr + 4 * buf, acc);
+                commit<CG, true>(acc_full(buf));
+                if (CG == 1) mbar_arrive(acc_full(buf));
             }
             __syncwarp();
         }
-    } else if (warp >= 4 && warp < 8) {
-        const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);
-        const int row = (warp & 3) * 32 + lane;
-        for (uint32_t n = 0; walk.next(s); n++) {
-            int ok = 1;
-            if (lane == 0) ok = wait_bar(acc_full, n & 1, abort_addr, a.status, 63);
-            if (!__shfl_sync(~0u, ok, 0)) break;
-            tc_fence_after();
-            const bool none = ld_shared_u32(any_addr) == 0;  // no MMA wrote the accumulators
-            const int half = s.t / a.col_tiles, m = s.g * 256 + half * 128 + row, n0 = (s.t - half * a.col_tiles) * NT, cols = min(NT, a.N - n0);
-            float* part = a.scratch + (size_t)s.slot * (128 * NT) + row;
-            for (int c = 0; c < cols; c += 16) {
-                uint32_t u[16];
-                float v[16];
-                tmem_ld_x16(lanes + c, u);
-                tmem_ld_wait();
+    } else if (warp == 2 && rank == 0) {
+        bool ok = true;
+        while (ok && walk.next(s)) {
+            for (int k = s.k0; k < s.k1; k++, i++) {
+                const uint32_t st = i % S, stage = base + st * G::STAGE;
+                ok = __all_sync(~0u, wait_bar(full(st), (i / S) & 1, abort_addr, a.status, 63) &&
+                                         (CG == 1 || wait_bar(full2(st), (i / S) & 1, abort_addr, a.status, 64)));
+                if (!ok) break;
+                if (CG == 2) fence_cluster();
+                tc_fence_after();
+                const uint32_t mask = uniform(ld_shared_u32(base + G::OFF_MASK + 4 * st));
+                const uint32_t sf = tmem + 256 + st * G::SF_COLUMNS;
+                const uint64_t dsa = desc_scales(stage + G::OFF_SFA), dsb = desc_scales(stage + G::OFF_SFB);
+                if (elect_one()) {
 #pragma unroll
-                for (int j = 0; j < 16; j++) v[j] = none ? 0.f : __uint_as_float(u[j]);
-                if (s.cut) {
+                    for (uint32_t q = 0; q < 4; q++) {
+                        if (!(mask >> q & 1)) continue;
+                        cp_scales<CG>(sf + q * 4, dsa + q * 32);
 #pragma unroll
-                    for (int j = 0; j < 16; j++) part[(size_t)(c + j) * 128] = v[j];
-                } else if (m < a.rows) {
-                    store_row16(a, m, n0 + c, v);
+                        for (int j = 0; j < G::BT; j++) cp_scales<CG>(sf + 16 + q * 4 * G::BT + j * 4, dsb + q * 32 + j * 128);
+                    }
+                    commit<CG, false>(scaled(st));
                 }
+                __syncwarp();
+            }
+        }
+    } else if (warp == 3 && rank == 1) {
+        // Tells the first CTA what has arrived here.
+        bool ok = true;
+        while (ok && walk.next(s)) {
+            for (int k = s.k0; k < s.k1; k++, i++) {
+                const uint32_t st = i % S;
+                ok = __all_sync(~0u, wait_bar(full(st), (i / S) & 1, abort_addr, a.status, 65));
+                if (!ok) break;
+                if (lane == 0) arrive_at_first(full2(st));
+            }
+        }
+    } else if (warp >= 4) {
+        const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21), out = base + G::OFF_OUT + (uint32_t)(warp - 4) * 4096;
+        const uint32_t col = base + G::OFF_COL + (uint32_t)(warp - 4) * 256;
+        const int row0 = (warp & 3) * 32, c0 = (warp - 4) / 4 * 64;  // rows and first columns of this warp
+        for (uint32_t n = 0; walk.next(s); n++) {
+            const uint32_t buf = n % G::ACC;
+            const int m0 = s.g * 256 + half_of(s.t) * 128 + row0, n0 = column_of(s.t) * NT, cols = min(NT, a.N - n0);
+            const float rs = a.row_scale && m0 + lane < a.rows ? __ldg(a.row_scale + m0 + lane) : 1.f;
+            float cs[(NT + 127) / 128][2];
+#pragma unroll
+            for (int j = 0; j < (NT + 127) / 128; j++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const int c = n0 + c0 + j * 128 + lane + e * 32;
+                    cs[j][e] = a.b_row_scale && c < a.N ? __ldg(a.b_row_scale + c) : 1.f;
+                }
+            // of a pair, only the one step of an empty group has no MMA
+            bool none = CG == 2 && s.ns == 1 && __ldg(&a.steps[s.gs].mask) == 0;
+            if (!__all_sync(~0u, wait_bar(acc_full(buf), (n / G::ACC) & 1, abort_addr, a.status, 66))) break;
+            tc_fence_after();
+            if (CG == 1) none = ld_shared_u32(any_addr + 4 * buf) == 0;
+#pragma unroll
+            for (int jc = 0; jc < (NT + 127) / 128; jc++) {
+                const int c = c0 + jc * 128;
+                if (c >= cols) break;
+                if (s.cut) {
+                    float* to = a.scratch + (size_t)s.slot * (128 * CG * NT) + (CG == 2 ? (int)rank * 128 : 0) + row0 + lane;
+                    for (int j0 = c; j0 < min(c + 64, cols); j0 += 16) {
+                        uint32_t u[16];
+                        tmem_ld_x16(lanes + buf * NT + j0, u);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int j = 0; j < 16; j++) to[(size_t)(j0 + j) * (128 * CG)] = none ? 0.f : __uint_as_float(u[j]);
+                    }
+                    continue;
+                }
+                st_shared_u32(col + lane * 4, __float_as_uint(cs[jc][0]));
+                st_shared_u32(col + lane * 4 + 128, __float_as_uint(cs[jc][1]));
+                __syncwarp();
+#pragma unroll
+                for (int j0 = 0; j0 < (NT < 64 ? NT : 64); j0 += 16) {
+                    uint32_t u[16], w[8];
+                    tmem_ld_x16(lanes + buf * NT + c + j0, u);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const uint4 f = ld_shared_v4(col + (j0 + 4 * j) * 4);
+                        const float v0 = __uint_as_float(u[4 * j]) * rs * __uint_as_float(f.x), v1 = __uint_as_float(u[4 * j + 1]) * rs * __uint_as_float(f.y);
+                        const float v2 = __uint_as_float(u[4 * j + 2]) * rs * __uint_as_float(f.z), v3 = __uint_as_float(u[4 * j + 3]) * rs * __uint_as_float(f.w);
+                        w[2 * j] = none ? 0 : a.c_dtype == SMAT_F16 ? pack2<SMAT_F16>(v0, v1) : pack2<SMAT_BF16>(v0, v1);
+                        w[2 * j + 1] = none ? 0 : a.c_dtype == SMAT_F16 ? pack2<SMAT_F16>(v2, v3) : pack2<SMAT_BF16>(v2, v3);
+                    }
+                    st_shared_v4(out + lane * 128 + (((j0 / 8) ^ (lane & 7)) << 4), w[0], w[1], w[2], w[3]);
+                    st_shared_v4(out + lane * 128 + (((j0 / 8 + 1) ^ (lane & 7)) << 4), w[4], w[5], w[6], w[7]);
+                }
+                __syncwarp();
+                const int width = min(64, cols - c);
+                uint16_t* const to = static_cast<uint16_t*>(a.C) + (size_t)m0 * a.N + n0 + c;
+                if (a.N % 8 == 0) {  // eight lanes a row
+#pragma unroll
+                    for (int r0 = 0; r0 < 32; r0 += 4) {
+                        const int r = r0 + lane / 8, j = lane % 8;
+                        const uint4 v = ld_shared_v4(out + r * 128 + ((j ^ (r & 7)) << 4));
+                        if (m0 + r < a.rows && j * 8 < width) *reinterpret_cast<uint4*>(to + (size_t)r * a.N + j * 8) = v;
+                    }
+                } else {
+                    for (int r = 0; r < 32 && m0 + r < a.rows; r++)
+                        for (int j = lane; j < width; j += 32) to[(size_t)r * a.N + j] = ld_shared_u16(out + r * 128 + (((j >> 3) ^ (r & 7)) << 4) + (j & 7) * 2);
+                }
+                __syncwarp();
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(acc_empty);
+            if (lane == 0) {
+                if (CG == 2 && rank == 1) arrive_at_first(acc_empty(buf));
+                else mbar_arrive(acc_empty(buf));
+            }
         }
     }
 
@@ -293,61 +417,99 @@ __global__ void __launch_bounds__(kTileThreads, 1) fp4_tile_kernel(const __grid_
         // a wait ran out somewhere: give copies still in flight time to land before the CTA retires
         for (int j = 0; j < 64; j++) __nanosleep(1000);
     }
+    if (CG == 2) cluster_sync();  // the MMAs read both CTAs' shared memory
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc(tmem, 512);
+        dealloc_all<CG>(tmem);
     }
 }
 
-// Adds up the parts of the tiles that a range boundary falls into.  CTA (c - 1, j) looks at the boundary between the ranges of CTAs
-// c - 1 and c: if it is the first inside a tile, the tile's 32 columns from 32 j on are summed, the parts in the order of the ranges.
+// Adds up the parts of the units that a start falls into, in the order of the parts.  CTA (c - 1, j): if start c is the first inside
+// a unit, 32 columns of it from 32 j on.
 template <int NT>
-__global__ void __launch_bounds__(256) fp4_join_kernel(const TileArgs a, const Work work) {
-    const int c = (int)blockIdx.x + 1, c0 = (int)blockIdx.y * 32;
-    const long long b = work.begin(c);
-    const int g = work.group_of(b < work.total ? b : work.total - 1);
-    const int ns = __ldg(work.gsp + g + 1) - __ldg(work.gsp + g);
-    const int t = (int)((b - work.first(g)) / ns);
-    const long long u0 = work.first(g) + (long long)t * ns, u1 = u0 + ns;
-    const long long before = work.begin(c - 1);
-    if (b >= work.total || b == u0 || before > u0) return;
-    const int row = threadIdx.x % 128, h = threadIdx.x / 128;
-    const int half = t / a.col_tiles, n0 = (t - half * a.col_tiles) * NT + c0 + h * 16, m = g * 256 + half * 128 + row;
-    float v[16];
-#pragma unroll
-    for (int j = 0; j < 16; j++) v[j] = 0.f;
-    long long p = before;
-    for (int k = c - 1; p < u1; k++) {
-        const float* part = a.scratch + (size_t)(2 * k + (p < u0 ? 1 : 0)) * (128 * NT) + (size_t)(c0 + h * 16) * 128 + row;
-#pragma unroll
-        for (int j = 0; j < 16; j++)
-            if (n0 + j < a.N) v[j] += __ldg(part + (size_t)j * 128);
-        p = work.begin(k + 1);
+__global__ void __launch_bounds__(256) fp4_join_kernel(const __grid_constant__ TileArgs a, const __grid_constant__ Schedule plan) {
+    constexpr int CG = Cfg<NT>::CG, ROWS = 128 * CG;
+    const int c = (int)blockIdx.x + 1;
+    const Start b = plan.at[c], before = plan.at[c - 1];
+    const bool same = before.g == b.g && before.t == b.t;
+    if (b.k == 0 || (same && before.k != 0)) return;
+    const int n0 = (CG == 2 ? b.t : b.t % a.col_tiles) * NT + (int)blockIdx.y * 32;
+    const int m0 = b.g * 256 + (CG == 2 ? 0 : b.t / a.col_tiles * 128);
+    __shared__ float tile[32][ROWS + 1];
+    for (int j = threadIdx.x; j < 32 * ROWS; j += 256) {
+        const int row = j % ROWS, col = j / ROWS;
+        if (n0 + col >= a.N) break;
+        const float* src = a.scratch + ((size_t)blockIdx.y * 32 + col) * ROWS + row;
+        float v = __ldg(src + (size_t)(2 * (c - 1) + (same ? 0 : 1)) * (ROWS * NT));
+        int k = c;
+        do v += __ldg(src + (size_t)(2 * k) * (ROWS * NT));
+        while (++k < plan.parts && plan.at[k].g == b.g && plan.at[k].t == b.t);
+        tile[col][row] = v;
     }
-    if (m < a.rows && n0 < a.N) store_row16(a, m, n0, v);
+    __syncthreads();
+    for (int j = threadIdx.x; j < 32 * ROWS; j += 256) {
+        const int row = j / 32, col = j % 32;
+        if (m0 + row >= a.rows || n0 + col >= a.N) continue;
+        float v = tile[col][row];
+        if (a.row_scale) v *= __ldg(a.row_scale + m0 + row);
+        if (a.b_row_scale) v *= __ldg(a.b_row_scale + n0 + col);
+        store_c(a.C, a.c_dtype, (size_t)(m0 + row) * a.N + n0 + col, v);
+    }
+}
+
+// The units of `groups` groups in parts of about equal numbers of steps.  Where a part has eight units or more it begins with one: a
+// cut unit goes through memory in fp32, which costs more than being off the equal share by half a unit.  Returns whether any is cut.
+bool make_schedule(const int* gsp, int groups, int units, int sms, Schedule& s) {
+    const long long total = (long long)gsp[groups] * units;
+    s.parts = (int)std::max<long long>(std::min<long long>(std::min(sms, kMaxParts), total / 4), 1);  // not below four steps a part
+    s.units = units;
+    bool cut = false;
+    int g = 0;
+    for (int c = 0; c < s.parts; c++) {
+        const long long p = total * c / s.parts;
+        while ((long long)gsp[g + 1] * units <= p) g++;
+        const int ns = gsp[g + 1] - gsp[g];
+        const long long off = p - (long long)gsp[g] * units;
+        Start b = {g, (int)(off / ns), (int)(off % ns)};
+        if (b.k && (long long)ns * 8 * s.parts <= total) {
+            if (2 * b.k > ns && ++b.t == units) { b.t = 0; b.g++; }
+            b.k = 0;
+        }
+        cut |= b.k != 0;
+        s.at[c] = b;
+    }
+    s.at[s.parts] = {groups, 0, 0};
+    return cut;
 }
 
 template <int NT, int FMT>
-int launch_tile(const TileArgs& args, const CUtensorMap& map, Work work, size_t total, const DeviceCtx* ctx, cudaStream_t stream) {
+int launch_tile(const TileArgs& args, const CUtensorMap& map, const int* gsp, int groups, const DeviceCtx* ctx, cudaStream_t stream) {
     using G = Cfg<NT>;
     TileArgs a = args;
-    const cudaError_t attr = cudaFuncSetAttribute(fp4_tile_kernel<NT, FMT>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM);
-    if (attr != cudaSuccess) return fail(SMAT_ERR_CUDA, "cudaFuncSetAttribute failed: %s", cudaGetErrorString(attr));
+    SMAT_CUDA_TRY(cudaFuncSetAttribute(fp4_tile_kernel<NT, FMT>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM));
     a.col_tiles = (a.N + NT - 1) / NT;
-    work.tiles = 2 * a.col_tiles;  // of each half of a group
-    work.total = (long long)total * work.tiles;
-    // a CTA for every SM, but not below four steps each
-    work.parts = (int)(work.total / 4 < ctx->sm_count ? (work.total / 4 > 0 ? work.total / 4 : 1) : ctx->sm_count);
+    Schedule s;
+    const bool cut = make_schedule(gsp, groups, (G::CG == 2 ? 1 : 2) * a.col_tiles, ctx->sm_count / G::CG, s);
     void* scratch = nullptr;
-    if (work.parts > 1) {
-        SMAT_CUDA_TRY(cudaMallocFromPoolAsync(&scratch, (size_t)work.parts * 2 * 128 * NT * sizeof(float), ctx->pool, stream));
+    if (cut) {
+        SMAT_CUDA_TRY(cudaMallocFromPoolAsync(&scratch, (size_t)s.parts * 2 * 128 * G::CG * NT * sizeof(float), ctx->pool, stream));
         a.scratch = static_cast<float*>(scratch);
     }
-    fp4_tile_kernel<NT, FMT><<<work.parts, kTileThreads, G::SMEM, stream>>>(map, a, work);
-    cudaError_t e = cudaGetLastError();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(s.parts * G::CG));
+    cfg.blockDim = dim3(kTileThreads);
+    cfg.dynamicSmemBytes = G::SMEM;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = G::CG;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, fp4_tile_kernel<NT, FMT>, map, a, s);
     count_launch();
-    if (e == cudaSuccess && work.parts > 1) {
-        fp4_join_kernel<NT><<<dim3(work.parts - 1, NT / 32), 256, 0, stream>>>(a, work);
+    if (e == cudaSuccess && cut) {
+        fp4_join_kernel<NT><<<dim3(s.parts - 1, NT / 32), 256, 0, stream>>>(a, s);
         e = cudaGetLastError();
         count_launch();
     }
@@ -358,9 +520,9 @@ int launch_tile(const TileArgs& args, const CUtensorMap& map, Work work, size_t 
 }
 
 template <int NT>
-int launch_tile_format(int fmt, const TileArgs& a, const CUtensorMap& map, const Work& work, size_t total, const DeviceCtx* ctx, cudaStream_t stream) {
-    return fmt == SMAT_FP4_NV ? launch_tile<NT, SMAT_FP4_NV>(a, map, work, total, ctx, stream)
-                              : launch_tile<NT, SMAT_FP4_MX>(a, map, work, total, ctx, stream);
+int launch_tile_format(int fmt, const TileArgs& a, const CUtensorMap& map, const int* gsp, int groups, const DeviceCtx* ctx, cudaStream_t stream) {
+    return fmt == SMAT_FP4_NV ? launch_tile<NT, SMAT_FP4_NV>(a, map, gsp, groups, ctx, stream)
+                              : launch_tile<NT, SMAT_FP4_MX>(a, map, gsp, groups, ctx, stream);
 }
 
 }  // namespace
@@ -371,10 +533,11 @@ int launch_fp4_tile(const Fp4View& A, const Fp4Rhs& B, void* C, int c_dtype, siz
     const int nt = N <= 32 ? 32 : N <= 64 ? 64 : N <= 128 ? 128 : 256;
     CUtensorMap map;
     const size_t pitch = fp4_pitch(A.K);
-    if (int rc = encode_tensor_map_2d_u8(&map, B.data, pitch, N, pitch, 128, (uint32_t)nt)) return rc;
+    if (int rc = encode_tensor_map_2d_u8(&map, B.data, pitch, N, pitch, 128, (uint32_t)std::min(nt, 128))) return rc;
     TileArgs a = {};
     a.steps = A.steps;
     a.tiles = A.tiles;
+    a.gsp = A.gsp;
     a.b_scales = B.scales;
     a.row_scale = A.row_scale ? A.row_scale + A.brow_begin * 16 : nullptr;
     a.b_row_scale = B.row_scale;
@@ -385,14 +548,12 @@ int launch_fp4_tile(const Fp4View& A, const Fp4Rhs& B, void* C, int c_dtype, siz
     a.N = (int)N;
     a.quads = (int)fp4_quads(A.K);
     a.b_row_tiles = (int)((N + 127) / 128);
-    Work work = {};
-    work.gsp = A.gsp;
-    work.groups = (int)((A.block_rows + kFp4GroupRows - 1) / kFp4GroupRows);
+    const int groups = (int)((A.block_rows + kFp4GroupRows - 1) / kFp4GroupRows);
     switch (nt) {
-        case 32: return launch_tile_format<32>(A.fmt, a, map, work, A.total_steps, ctx, stream);
-        case 64: return launch_tile_format<64>(A.fmt, a, map, work, A.total_steps, ctx, stream);
-        case 128: return launch_tile_format<128>(A.fmt, a, map, work, A.total_steps, ctx, stream);
-        default: return launch_tile_format<256>(A.fmt, a, map, work, A.total_steps, ctx, stream);
+        case 32: return launch_tile_format<32>(A.fmt, a, map, A.h_gsp, groups, ctx, stream);
+        case 64: return launch_tile_format<64>(A.fmt, a, map, A.h_gsp, groups, ctx, stream);
+        case 128: return launch_tile_format<128>(A.fmt, a, map, A.h_gsp, groups, ctx, stream);
+        default: return launch_tile_format<256>(A.fmt, a, map, A.h_gsp, groups, ctx, stream);
     }
 }
 
