@@ -12,11 +12,10 @@
 // Beyond 128 columns of C two CTAs share a tile of 256 x 256 (cta_group::2): each holds 128 rows of A and 128 columns of B, so an SM
 // fetches 38 KB a step of 512 cycles of MMAs instead of 54; L2 delivers about 70 bytes a cycle and SM.
 //
-// Roles.  One thread fetches tiles of A (bulk copies), B (tiled TMA copies with 128-byte swizzle) and its scales; one moves the scales
-// to tensor memory (24 cycles for each of 12 copies a step: as long as issuing the MMAs takes, so it is not the same thread), one
-// issues the MMAs; eight warps store finished tiles of C through shared memory, whole 128-byte lines at a time.  Of a pair, the second
-// CTA only fetches and stores.  The (tile of C, step) pairs are dealt out in equal contiguous ranges, worked out on the host; tiles
-// that a range boundary falls into are joined from fp32 parts in a fixed order by a second kernel.  All waits are bounded.
+// Roles.  One thread fetches tiles of A (bulk copies), B (tiled TMA copies with 128-byte swizzle) and its scales; four warps move the
+// scales to tensor memory through registers (tcgen05.cp, 12 of them a step, took their issuer 24 cycles each in a CTA of its own and
+// 140 in a pair); one thread issues the MMAs; eight warps store finished tiles of C through shared memory, whole 128-byte lines at a
+// time.  Of a pair, the second CTA issues no MMAs.  All waits are bounded.
 #include <algorithm>
 
 #include "fp4_device.cuh"
@@ -48,22 +47,10 @@ __device__ __forceinline__ void mma_fp4(uint32_t d, uint64_t a, uint64_t b, uint
     else SMAT_MMA_FP4("2", "mxf4.block_scale.scale_vec::2X");
 #undef SMAT_MMA_FP4
 }
-// 32 rows of 16 bytes (a scale tile of 512 bytes) to four columns of tensor memory, the same in all four lane quarters; of a pair,
-// in both CTAs, from the shared memory of each.
+// Arrives on this CTA's barrier, of a pair on that of both, once every tcgen05 operation issued so far by this thread has completed.
 template <int CG>
-__device__ __forceinline__ void cp_scales(uint32_t taddr, uint64_t desc) {
-    if constexpr (CG == 1) asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-    else asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-}
-// Descriptor of such a tile: no swizzle, groups of 8 rows x 16 bytes 128 bytes apart.
-__device__ __forceinline__ uint64_t desc_scales(uint32_t smem_addr) {
-    return (uint64_t)((smem_addr >> 4) & 0x3FFFu) | (8ull << 16) | (8ull << 32) | (1ull << 46);
-}
-// Arrives on this CTA's barrier once every tcgen05 operation issued so far by this thread has completed; BOTH: on that of both CTAs.
-template <int CG, bool BOTH>
 __device__ __forceinline__ void commit(uint32_t bar) {
     if constexpr (CG == 1) tc_commit(bar);
-    else if constexpr (!BOTH) asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
     else
         asm volatile(
             "{\n\t.reg .b16 m;\n\tmov.b16 m, 3;\n\t"
@@ -95,17 +82,24 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
-// Arrives on the barrier at the same place of the first CTA's shared memory.
+// Arrives on the barrier at the same place of the first CTA's shared memory.  What it announces is tensor memory (ordered by the
+// tcgen05 fences around it), so it needs no release at cluster scope, which takes 700 to 900 cycles.
 __device__ __forceinline__ void arrive_at_first(uint32_t bar) {
     asm volatile(
         "{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %0, 0;\n\t"
-        "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [r];\n\t}" ::"r"(bar)
+        "mbarrier.arrive.shared::cluster.b64 _, [r];\n\t}" ::"r"(bar)
         : "memory");
 }
-__device__ __forceinline__ void fence_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
-
 __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+// Writes 16 consecutive columns of the calling thread's lane.
+__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint4* v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+        "r"(v[0].x), "r"(v[0].y), "r"(v[0].z), "r"(v[0].w), "r"(v[1].x), "r"(v[1].y), "r"(v[1].z), "r"(v[1].w), "r"(v[2].x), "r"(v[2].y),
+        "r"(v[2].z), "r"(v[2].w), "r"(v[3].x), "r"(v[3].y), "r"(v[3].z), "r"(v[3].w)
+        : "memory");
 }
 __device__ __forceinline__ uint16_t ld_shared_u16(uint32_t addr) {
     uint16_t v;
@@ -114,16 +108,19 @@ __device__ __forceinline__ uint16_t ld_shared_u16(uint32_t addr) {
 }
 
 // ---- schedule -------------------------------------------------------------------------------------------------------------------
-// Units: tiles of C, those of a group of block-rows one after another.  A part is what a CTA (or pair) works on: from one start to the
-// next.  Worked out on the host and handed over as a kernel parameter: looked up on the device, five dependent loads at a time, it
-// took 7 us of every launch and 18 us of the joining kernel.
+// Units: tiles of C, those of a group of block-rows one after another.  The first `rounds` units of a part (a CTA or pair) are dealt out
+// one by one, so that all parts walk the columns in step and L2 serves what several of them read (in contiguous ranges from the start,
+// the layer 8192 x 28672 at 20 %, N = 4096, fetched everything from HBM: 830 us).  What is left is one contiguous range for each part,
+// from one start to the next; units that a start falls into are joined from fp32 sums in a fixed order by a second kernel.  Worked out
+// on the host and handed over as a kernel parameter: looked up on the device, five dependent loads at a time, it took 7 us of every
+// launch and 18 us of the joining kernel.
 struct Start {
     int g, t, k;  // group, unit of the group, step of the unit
 };
 constexpr int kMaxParts = 160;
 struct Schedule {
     Start at[kMaxParts + 1];
-    int parts, units;  // units of a group
+    int parts, units, rounds;  // units: of a group
 };
 struct Piece {  // steps [k0, k1) of the ns steps of unit (g, t)
     int g, t, k0, k1, gs, ns, slot;
@@ -132,21 +129,34 @@ struct Piece {  // steps [k0, k1) of the ns steps of unit (g, t)
 struct Walk {
     const int* gsp;
     Start now, end;
-    int units, slot;
+    int units, parts, slot, unit, left;
     __device__ __forceinline__ Walk(const Schedule& s, const int* first_steps, int part)
-        : gsp(first_steps), now(s.at[part]), end(s.at[part + 1]), units(s.units), slot(2 * part) {}
+        : gsp(first_steps), now(s.at[part]), end(s.at[part + 1]), units(s.units), parts(s.parts), slot(2 * part), unit(part), left(s.rounds) {}
+    __device__ __forceinline__ void look_up(Piece& p, int g, int t) const {
+        p.g = g;
+        p.t = t;
+        p.gs = __ldg(gsp + g);
+        p.ns = __ldg(gsp + g + 1) - p.gs;
+    }
     __device__ __forceinline__ bool next(Piece& p) {
+        if (left) {
+            look_up(p, unit / units, unit % units);
+            p.k0 = 0;
+            p.k1 = p.ns;
+            p.cut = false;
+            p.slot = 0;
+            unit += parts;
+            left--;
+            return true;
+        }
         const bool last = now.g == end.g && now.t == end.t;
         if (last && now.k == end.k) return false;
-        p.gs = __ldg(gsp + now.g);
-        p.ns = __ldg(gsp + now.g + 1) - p.gs;
-        p.g = now.g;
-        p.t = now.t;
+        look_up(p, now.g, now.t);
         p.k0 = now.k;
         p.k1 = last ? end.k : p.ns;
         p.cut = p.k0 != 0 || p.k1 != p.ns;
         p.slot = slot;
-        slot |= 1;  // for a unit that begins inside the part
+        slot |= 1;  // for a unit that begins inside the range
         now.k = last ? end.k : 0;
         if (!last && ++now.t == units) { now.t = 0; now.g++; }
         return true;
@@ -181,13 +191,13 @@ struct Cfg {
     static constexpr uint32_t OFF_OUT = S * STAGE;                  // 32 rows x 64 columns for each storing warp
     static constexpr uint32_t OFF_COL = OFF_OUT + 8 * 4096;         // and the scales of these columns
     static constexpr uint32_t OFF_BAR = OFF_COL + 8 * 256;
-    static constexpr uint32_t OFF_MASK = OFF_BAR + 8 * (4 * S + 4);
+    static constexpr uint32_t OFF_MASK = OFF_BAR + 8 * (3 * S + 4);
     static constexpr uint32_t OFF_MISC = OFF_MASK + 4 * S;
     static constexpr uint32_t SMEM = OFF_MISC + 16 + 1024;
     static_assert(STAGE % 1024 == 0 && SMEM <= 232448, "shared memory");
     static_assert(ACC * NT <= 256 && 256 + S * SF_COLUMNS <= 512, "tensor memory");
 };
-constexpr int kTileThreads = 12 * 32;
+constexpr int kTileThreads = 16 * 32;
 
 template <int NT, int FMT>
 __global__ void __launch_bounds__(kTileThreads, 1)
@@ -200,16 +210,15 @@ fp4_tile_kernel(const __grid_constant__ CUtensorMap mapB, const __grid_constant_
     const uint32_t bar = base + G::OFF_BAR;
     auto full = [&](uint32_t s) { return bar + 8 * s; };              // this CTA's operands have arrived
     auto empty = [&](uint32_t s) { return bar + 8 * (S + s); };       // ... and been used
-    auto scaled = [&](uint32_t s) { return bar + 8 * (2 * S + s); };  // the scales are in tensor memory
-    auto full2 = [&](uint32_t s) { return bar + 8 * (3 * S + s); };   // the second CTA's operands have arrived
-    auto acc_full = [&](uint32_t b) { return bar + 8 * (4 * S + b); };
-    auto acc_empty = [&](uint32_t b) { return bar + 8 * (4 * S + 2 + b); };
+    auto scaled = [&](uint32_t s) { return bar + 8 * (2 * S + s); };  // ... and their scales are in tensor memory (of both CTAs)
+    auto acc_full = [&](uint32_t b) { return bar + 8 * (3 * S + b); };
+    auto acc_empty = [&](uint32_t b) { return bar + 8 * (3 * S + 2 + b); };
     const uint32_t tmem_slot = base + G::OFF_MISC, abort_addr = tmem_slot + 4, any_addr = tmem_slot + 8;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = CG == 2 ? cluster_rank() : 0;
 
     if (threadIdx.x == 0) {
-        for (uint32_t s = 0; s < S; s++) { mbar_init(full(s), 1); mbar_init(empty(s), 1); mbar_init(scaled(s), 1); mbar_init(full2(s), 1); }
+        for (uint32_t s = 0; s < S; s++) { mbar_init(full(s), 1); mbar_init(empty(s), 1); mbar_init(scaled(s), 4 * CG); }
         for (uint32_t b = 0; b < 2; b++) { mbar_init(acc_full(b), CG == 1 ? 2 : 1); mbar_init(acc_empty(b), 8 * CG); }
         st_shared_u32(abort_addr, 0);
         fence_barrier_init();
@@ -263,7 +272,6 @@ fp4_tile_kernel(const __grid_constant__ CUtensorMap mapB, const __grid_constant_
         for (uint32_t n = 0; ok && walk.next(s); n++) {
             const uint32_t buf = n % G::ACC;
             ok = __all_sync(~0u, wait_bar(acc_empty(buf), ((n / G::ACC) & 1) ^ 1, abort_addr, a.status, 61));
-            if (CG == 2) fence_cluster();
             tc_fence_after();
             uint32_t acc = 0;
             for (int k = s.k0; ok && k < s.k1; k++, i++) {
@@ -282,53 +290,45 @@ fp4_tile_kernel(const __grid_constant__ CUtensorMap mapB, const __grid_constant_
                         mma_fp4<FMT, CG>(tmem + buf * NT, da + q * 2, db + q * 2, idesc, sf + q * 4, sf + 16 + q * 4 * G::BT, on);
                         on = 1;
                     }
-                    commit<CG, true>(empty(st));
+                    commit<CG>(empty(st));
                 }
                 acc |= mask;
                 __syncwarp();
             }
             if (ok && elect_one()) {
                 if (CG == 1) st_shared_u32(any_addr + 4 * buf, acc);
-                commit<CG, true>(acc_full(buf));
+                commit<CG>(acc_full(buf));
                 if (CG == 1) mbar_arrive(acc_full(buf));
             }
             __syncwarp();
         }
-    } else if (warp == 2 && rank == 0) {
+    } else if (warp >= 12) {
+        // Scales to tensor memory: four words a lane and scale tile, the same in all lane quarters.
+        const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21) + 256;
         bool ok = true;
         while (ok && walk.next(s)) {
             for (int k = s.k0; k < s.k1; k++, i++) {
-                const uint32_t st = i % S, stage = base + st * G::STAGE;
-                ok = __all_sync(~0u, wait_bar(full(st), (i / S) & 1, abort_addr, a.status, 63) &&
-                                         (CG == 1 || wait_bar(full2(st), (i / S) & 1, abort_addr, a.status, 64)));
+                const uint32_t st = i % S, from = base + st * G::STAGE + lane * 16;
+                ok = __all_sync(~0u, wait_bar(full(st), (i / S) & 1, abort_addr, a.status, 63));
                 if (!ok) break;
-                if (CG == 2) fence_cluster();
                 tc_fence_after();
-                const uint32_t mask = uniform(ld_shared_u32(base + G::OFF_MASK + 4 * st));
-                const uint32_t sf = tmem + 256 + st * G::SF_COLUMNS;
-                const uint64_t dsa = desc_scales(stage + G::OFF_SFA), dsb = desc_scales(stage + G::OFF_SFB);
-                if (elect_one()) {
+                uint4 v[4 + 4 * G::BT];
 #pragma unroll
-                    for (uint32_t q = 0; q < 4; q++) {
-                        if (!(mask >> q & 1)) continue;
-                        cp_scales<CG>(sf + q * 4, dsa + q * 32);
+                for (int q = 0; q < 4; q++) v[q] = ld_shared_v4(from + G::OFF_SFA + q * 512);
 #pragma unroll
-                        for (int j = 0; j < G::BT; j++) cp_scales<CG>(sf + 16 + q * 4 * G::BT + j * 4, dsb + q * 32 + j * 128);
-                    }
-                    commit<CG, false>(scaled(st));
-                }
+                for (int q = 0; q < 4; q++)
+#pragma unroll
+                    for (int j = 0; j < G::BT; j++) v[4 + q * G::BT + j] = ld_shared_v4(from + G::OFF_SFB + j * 2048 + q * 512);
+                const uint32_t to = lanes + st * G::SF_COLUMNS;
+#pragma unroll
+                for (int j = 0; j < 1 + G::BT; j++) tmem_st_x16(to + 16 * j, v + 4 * j);
+                tmem_st_wait();
+                tc_fence_before();
                 __syncwarp();
-            }
-        }
-    } else if (warp == 3 && rank == 1) {
-        // Tells the first CTA what has arrived here.
-        bool ok = true;
-        while (ok && walk.next(s)) {
-            for (int k = s.k0; k < s.k1; k++, i++) {
-                const uint32_t st = i % S;
-                ok = __all_sync(~0u, wait_bar(full(st), (i / S) & 1, abort_addr, a.status, 65));
-                if (!ok) break;
-                if (lane == 0) arrive_at_first(full2(st));
+                if (lane == 0) {
+                    if (CG == 2 && rank == 1) arrive_at_first(scaled(st));
+                    else mbar_arrive(scaled(st));
+                }
             }
         }
     } else if (warp >= 4) {
@@ -436,15 +436,33 @@ __global__ void __launch_bounds__(256) fp4_join_kernel(const __grid_constant__ T
     const int n0 = (CG == 2 ? b.t : b.t % a.col_tiles) * NT + (int)blockIdx.y * 32;
     const int m0 = b.g * 256 + (CG == 2 ? 0 : b.t / a.col_tiles * 128);
     __shared__ float tile[32][ROWS + 1];
-    for (int j = threadIdx.x; j < 32 * ROWS; j += 256) {
-        const int row = j % ROWS, col = j / ROWS;
-        if (n0 + col >= a.N) break;
-        const float* src = a.scratch + ((size_t)blockIdx.y * 32 + col) * ROWS + row;
-        float v = __ldg(src + (size_t)(2 * (c - 1) + (same ? 0 : 1)) * (ROWS * NT));
+    __shared__ int slots[kMaxParts + 1], n_slots;
+    if (threadIdx.x == 0) {
+        int n = 0;
+        slots[n++] = 2 * (c - 1) + (same ? 0 : 1);
         int k = c;
-        do v += __ldg(src + (size_t)(2 * k) * (ROWS * NT));
-        while (++k < plan.parts && plan.at[k].g == b.g && plan.at[k].t == b.t);
-        tile[col][row] = v;
+        do {
+            const Start from = plan.at[k], to = plan.at[k + 1];
+            if (from.k != to.k || from.g != to.g || from.t != to.t) slots[n++] = 2 * k;  // not an empty range
+        } while (++k < plan.parts && plan.at[k].g == b.g && plan.at[k].t == b.t);
+        n_slots = n;
+    }
+    __syncthreads();
+    // 16 independent sums a thread: one after the other, each a chain of loads, they took 48 us
+    const int row = threadIdx.x % ROWS, cols = min(32, a.N - n0);
+    for (int c0 = threadIdx.x / ROWS * 16; c0 < 32; c0 += 256 / ROWS * 16) {
+        float v[16];
+#pragma unroll
+        for (int j = 0; j < 16; j++) v[j] = 0.f;
+        const float* src = a.scratch + ((size_t)blockIdx.y * 32 + c0) * ROWS + row;
+        for (int k = 0; k < n_slots; k++) {
+            const float* p = src + (size_t)slots[k] * (ROWS * NT);
+#pragma unroll
+            for (int j = 0; j < 16; j++)
+                if (c0 + j < cols) v[j] += __ldg(p + j * ROWS);
+        }
+#pragma unroll
+        for (int j = 0; j < 16; j++) tile[c0 + j][row] = v[j];
     }
     __syncthreads();
     for (int j = threadIdx.x; j < 32 * ROWS; j += 256) {
@@ -457,23 +475,53 @@ __global__ void __launch_bounds__(256) fp4_join_kernel(const __grid_constant__ T
     }
 }
 
-// The units of `groups` groups in parts of about equal numbers of steps.  Where a part has eight units or more it begins with one: a
-// cut unit goes through memory in fp32, which costs more than being off the equal share by half a unit.  Returns whether any is cut.
+// Returns whether any unit is cut.
 bool make_schedule(const int* gsp, int groups, int units, int sms, Schedule& s) {
-    const long long total = (long long)gsp[groups] * units;
-    s.parts = (int)std::max<long long>(std::min<long long>(std::min(sms, kMaxParts), total / 4), 1);  // not below four steps a part
+    constexpr long long kLeast = 8;  // steps of a range: below, joining costs more than the time saved
+    const long long total = (long long)gsp[groups] * units, all = (long long)groups * units;
+    s.parts = (int)std::max<long long>(std::min<long long>(std::min(sms, kMaxParts), std::max(total / kLeast, all)), 1);
     s.units = units;
-    bool cut = false;
-    int g = 0;
+    s.rounds = (int)(all / s.parts);
+    long long load[kMaxParts];
+    auto steps_of = [&](long long unit) { return (long long)(gsp[unit / units + 1] - gsp[unit / units]); };
+    auto deal = [&]() {
+        long long most = 0;
+        for (int c = 0; c < s.parts; c++) load[c] = 0;
+        for (int r = 0; r < s.rounds; r++)
+            for (int c = 0; c < s.parts; c++) load[c] += steps_of((long long)r * s.parts + c);
+        for (int c = 0; c < s.parts; c++) most = std::max(most, load[c]);
+        return most;
+    };
+    // Units of very different lengths: everything in ranges.
+    if (deal() * s.parts > total + total / 4) { s.rounds = 0; deal(); }
+    const long long first = (long long)s.rounds * s.parts;  // the first unit of the ranges
+    int g = (int)(first / units);
+    const long long begin = (long long)gsp[g] * units + (first - (long long)g * units) * (g < groups ? gsp[g + 1] - gsp[g] : 0);
+    const long long rest = total - begin;
+    // A part gets of the rest what it is short of an equal share; ranges of long units may cut them, others hold whole ones.
+    const bool may_cut = rest >= 2 * kLeast * (all - first);
+    long long want[kMaxParts], sum = 0, given = 0;
     for (int c = 0; c < s.parts; c++) {
-        const long long p = total * c / s.parts;
-        while ((long long)gsp[g + 1] * units <= p) g++;
-        const int ns = gsp[g + 1] - gsp[g];
-        const long long off = p - (long long)gsp[g] * units;
-        Start b = {g, (int)(off / ns), (int)(off % ns)};
-        if (b.k && (long long)ns * 8 * s.parts <= total) {
-            if (2 * b.k > ns && ++b.t == units) { b.t = 0; b.g++; }
-            b.k = 0;
+        want[c] = std::max<long long>(total / s.parts + 1 - load[c], 0);
+        if (want[c] < kLeast && may_cut) want[c] = 0;
+        sum += want[c];
+    }
+    if (!sum) { want[0] = sum = 1; }
+    bool cut = false;
+    for (int c = 0; c < s.parts; c++) {
+        const long long p = begin + rest * given / sum;
+        given += want[c];
+        while (g < groups && (long long)gsp[g + 1] * units <= p) g++;
+        Start b = {g, 0, 0};
+        if (g < groups) {
+            const int ns = gsp[g + 1] - gsp[g];
+            const long long off = p - (long long)gsp[g] * units;
+            b.t = (int)(off / ns);
+            b.k = (int)(off % ns);
+            if (b.k && !may_cut) {
+                if (2 * b.k > ns && ++b.t == units) { b.t = 0; b.g++; }
+                b.k = 0;
+            }
         }
         cut |= b.k != 0;
         s.at[c] = b;
