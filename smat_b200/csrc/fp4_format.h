@@ -29,10 +29,8 @@ inline size_t fp4_pitch(size_t K) { return fp4_quads(K) * 32; }
 // scale tiles of 128 rows x 64 columns, zeros where no block is stored.
 constexpr size_t kFp4GroupRows = 16, kFp4StepColumns = 256;
 constexpr uint32_t kFp4TileCodes = 16384, kFp4TileBytes = kFp4TileCodes + 2048;
-struct Fp4Step {
-    uint32_t kstep;  // columns from 256 * kstep on
-    uint32_t mask;   // bit 4 h + q: half h has blocks in columns 64 q to 64 q + 63 of these
-};
+// A step is one word: bits [8, 32) say that its columns begin at 256 times that number (K below 2^26), bit 4 h + q that half h of the
+// group has blocks in columns 64 q to 64 q + 63 of them.
 struct Fp4Where {         // of what the tiles of a step are made
     int begin[16];        // first block of each block-row in these columns
     uint16_t blocks[16];  // bit c: the block-row has a block in columns 16 c to 16 c + 15 of these
@@ -47,7 +45,7 @@ struct Fp4View {
     const int2* range = nullptr;  // first and last + 1 block of every block-row of the range; empty where the arrays were inconsistent
     int fmt = 0;
     size_t K = 0, brow_begin = 0, block_rows = 0;
-    const Fp4Step* steps = nullptr;  // null: the plan has no tiles
+    const uint32_t* steps = nullptr;  // null: the plan has no tiles
     const uint8_t* tiles = nullptr;  // two of a step
     const int* gsp = nullptr;        // first step of every group, and the number of all
     const int* h_gsp = nullptr;      // the same on the host

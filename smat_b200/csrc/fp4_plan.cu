@@ -51,7 +51,7 @@ __global__ void __launch_bounds__(kThreads) fp4_ranges_kernel(const int* __restr
 constexpr int kStepThreads = 32 * (int)kFp4GroupRows;
 template <bool FILL>
 __global__ void __launch_bounds__(kStepThreads) fp4_steps_kernel(const int2* __restrict__ range, const int* __restrict__ colidx, int block_rows,
-                                                                 int words, int* __restrict__ gsp, Fp4Step* __restrict__ steps,
+                                                                 int words, int* __restrict__ gsp, uint32_t* __restrict__ steps,
                                                                  Fp4Where* __restrict__ where) {
     extern __shared__ uint32_t sm[];
     uint32_t *bitmap = sm, *prefix = sm + words;
@@ -98,8 +98,7 @@ __global__ void __launch_bounds__(kStepThreads) fp4_steps_kernel(const int2* __r
         const int at = first + (int)prefix[k >> 5] + __popc(bitmap[k >> 5] & ((1u << (k & 31)) - 1));
         where[at].begin[e] = p;
         where[at].blocks[e] = (uint16_t)blocks;
-        steps[at].kstep = (uint32_t)k;
-        atomicOr(&steps[at].mask, mask << (e / 8 * 4));
+        atomicOr(&steps[at], (uint32_t)k << 8 | mask << (e / 8 * 4));
     }
 }
 
@@ -177,11 +176,11 @@ int build_plan(smat_fp4_plan* p, const int* rowptr, const int* colidx, size_t nn
     v.longest = h_totals[1];
     const size_t steps = (size_t)h_steps;
     if (!with_tiles || v.blocks < kFp4TileFill * steps) return SMAT_OK;
-    SMAT_CUDA_TRY(cudaMalloc(&p->steps, steps * (sizeof(Fp4Step) + sizeof(Fp4Where))));
-    Fp4Step* step = static_cast<Fp4Step*>(p->steps);
+    SMAT_CUDA_TRY(cudaMalloc(&p->steps, steps * (sizeof(uint32_t) + sizeof(Fp4Where))));
+    uint32_t* step = static_cast<uint32_t*>(p->steps);
     p->where = reinterpret_cast<Fp4Where*>(step + steps);
     SMAT_CUDA_TRY(cudaMalloc(&p->tiles, steps * 2 * kFp4TileBytes));
-    SMAT_CUDA_TRY(cudaMemsetAsync(p->steps, 0, steps * (sizeof(Fp4Step) + sizeof(Fp4Where)), stream));
+    SMAT_CUDA_TRY(cudaMemsetAsync(p->steps, 0, steps * (sizeof(uint32_t) + sizeof(Fp4Where)), stream));
     SMAT_CUDA_TRY(cudaFuncSetAttribute(fp4_steps_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, words * 8));
     fp4_steps_kernel<true><<<(unsigned)groups, kStepThreads, words * 8, stream>>>(range, colidx, (int)v.block_rows, words, gsp, step, p->where);
     count_launch();

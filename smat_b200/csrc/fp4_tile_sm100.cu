@@ -35,11 +35,13 @@ __host__ __device__ constexpr uint32_t idesc_fp4(int m, int n, bool e8m0) {
     return (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((e8m0 ? 1u : 0u) << 23) | ((uint32_t)(m >> 4) << 24);
 }
 template <int FMT, int CG>
-__device__ __forceinline__ void mma_fp4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+__device__ __forceinline__ void mma_fp4(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t sfa,
+                                        uint32_t sfb, uint32_t accumulate) {
 #define SMAT_MMA_FP4(cg, kind)                                                                                  \
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"                                              \
-                 "tcgen05.mma.cta_group::" cg ".kind::" kind " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d), \
-                 "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)                                \
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tmov.b64 da, {%1, %2};\n\tmov.b64 db, {%3, %4};\n\t"     \
+                 "setp.ne.b32 p, %8, 0;\n\t"                                                                     \
+                 "tcgen05.mma.cta_group::" cg ".kind::" kind " [%0], da, db, %5, [%6], [%7], p;\n\t}" ::"r"(d),  \
+                 "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)     \
                  : "memory")
     if constexpr (FMT == SMAT_FP4_NV && CG == 1) SMAT_MMA_FP4("1", "mxf4nvf4.block_scale.scale_vec::4X");
     else if constexpr (FMT == SMAT_FP4_NV) SMAT_MMA_FP4("2", "mxf4nvf4.block_scale.scale_vec::4X");
@@ -163,8 +165,30 @@ struct Walk {
     }
 };
 
+// Step words, read by a warp 32 at a time and 32 ahead: one at a time, each iteration of a loop waited 800 cycles for its own.
+struct Records {
+    const uint32_t* p;
+    int last, base;
+    uint32_t cur, next;
+    __device__ __forceinline__ Records(const uint32_t* steps, int n) : p(steps), last(n - 1), base(-64) {}
+    __device__ __forceinline__ uint32_t load(int b) const { return __ldg(p + min(b + (int)(threadIdx.x & 31), last)); }
+    __device__ __forceinline__ uint32_t get(int at) {  // by all lanes; uniform
+        if ((unsigned)(at - base) >= 32) {
+            if ((unsigned)(at - base) < 64) {
+                cur = next;
+                base += 32;
+            } else {
+                base = at;
+                cur = load(base);
+            }
+            next = load(base + 32);
+        }
+        return uniform((int)(threadIdx.x & 31) == at - base ? cur : 0);
+    }
+};
+
 struct TileArgs {
-    const Fp4Step* steps;
+    const uint32_t* steps;
     const uint8_t* tiles;
     const int* gsp;
     const uint8_t* b_scales;
@@ -173,31 +197,30 @@ struct TileArgs {
     void* C;
     float* scratch;
     int* status;
-    int c_dtype, rows, N, quads, b_row_tiles, col_tiles;
+    int c_dtype, rows, N, quads, b_row_tiles, col_tiles, total_steps;
 };
 
 // NT columns of C per tile; a pair of CTAs (CG 2) for 256.
 template <int NT>
 struct Cfg {
     static constexpr int CG = NT == 256 ? 2 : 1;
-    static constexpr uint32_t S = NT == 64 ? 6 : NT == 32 ? 7 : 5;  // stages
+    static constexpr uint32_t S = NT == 64 ? 6 : NT == 32 ? 7 : 5;  // stages of codes
+    static constexpr uint32_t Q = NT == 256 ? 4 : 6;                // stages of scales on their way to tensor memory; see `arrived`
     static constexpr uint32_t NB = NT / CG;                         // columns of C whose part of B this CTA fetches
     static constexpr int BT = NT > 128 ? NT / 128 : 1;              // scale tiles of B
-    static constexpr uint32_t B_BYTES = NB * 128, SFB_BYTES = 2048 * BT;
-    static constexpr uint32_t OFF_SFA = kFp4TileCodes, OFF_B = kFp4TileBytes, OFF_SFB = OFF_B + B_BYTES;
-    static constexpr uint32_t STAGE = OFF_SFB + SFB_BYTES;
-    static constexpr uint32_t SF_COLUMNS = 16 + 16 * BT;            // tensor memory of a stage's scales
+    static constexpr uint32_t OFF_B = kFp4TileCodes, STAGE = OFF_B + NB * 128;
+    static constexpr uint32_t SF_STAGE = 2048 + 2048 * BT, SF_COLUMNS = 16 + 16 * BT;  // in shared and in tensor memory
     static constexpr uint32_t ACC = NT == 256 ? 1 : 2;              // accumulators
-    static constexpr uint32_t OFF_OUT = S * STAGE;                  // 32 rows x 64 columns for each storing warp
+    static constexpr uint32_t OFF_SF = S * STAGE;
+    static constexpr uint32_t OFF_OUT = OFF_SF + Q * SF_STAGE;      // 32 rows x 64 columns for each storing warp
     static constexpr uint32_t OFF_COL = OFF_OUT + 8 * 4096;         // and the scales of these columns
     static constexpr uint32_t OFF_BAR = OFF_COL + 8 * 256;
-    static constexpr uint32_t OFF_MASK = OFF_BAR + 8 * (3 * S + 4);
-    static constexpr uint32_t OFF_MISC = OFF_MASK + 4 * S;
+    static constexpr uint32_t OFF_MISC = OFF_BAR + 8 * (3 * S + 2 * Q + 4);
     static constexpr uint32_t SMEM = OFF_MISC + 16 + 1024;
-    static_assert(STAGE % 1024 == 0 && SMEM <= 232448, "shared memory");
+    static_assert(STAGE % 1024 == 0 && Q % 2 == 0 && SMEM <= 232448, "shared memory");
     static_assert(ACC * NT <= 256 && 256 + S * SF_COLUMNS <= 512, "tensor memory");
 };
-constexpr int kTileThreads = 16 * 32;
+constexpr int kTileThreads = 20 * 32;
 
 template <int NT, int FMT>
 __global__ void __launch_bounds__(kTileThreads, 1)
@@ -208,17 +231,24 @@ fp4_tile_kernel(const __grid_constant__ CUtensorMap mapB, const __grid_constant_
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t bar = base + G::OFF_BAR;
-    auto full = [&](uint32_t s) { return bar + 8 * s; };              // this CTA's operands have arrived
-    auto empty = [&](uint32_t s) { return bar + 8 * (S + s); };       // ... and been used
-    auto scaled = [&](uint32_t s) { return bar + 8 * (2 * S + s); };  // ... and their scales are in tensor memory (of both CTAs)
-    auto acc_full = [&](uint32_t b) { return bar + 8 * (3 * S + b); };
-    auto acc_empty = [&](uint32_t b) { return bar + 8 * (3 * S + 2 + b); };
+    // A step's codes have arrived and its scales are in tensor memory, of both CTAs: one barrier, since each wait takes the MMAs' thread
+    // 130 cycles.  `full` counts the second CTA's codes.
+    auto ready = [&](uint32_t s) { return bar + 8 * s; };
+    auto full = [&](uint32_t s) { return bar + 8 * (S + s); };
+    auto empty = [&](uint32_t s) { return bar + 8 * (2 * S + s); };  // ... and have been used
+    // Scales in shared memory.  Two sets of warps wait for them in turn, and each must see every phase of a barrier that it waits for
+    // by parity, so the stages are an even number.
+    auto arrived = [&](uint32_t s) { return bar + 8 * (3 * S + s); };
+    auto taken = [&](uint32_t s) { return bar + 8 * (3 * S + G::Q + s); };
+    auto acc_full = [&](uint32_t b) { return bar + 8 * (3 * S + 2 * G::Q + b); };
+    auto acc_empty = [&](uint32_t b) { return bar + 8 * (3 * S + 2 * G::Q + 2 + b); };
     const uint32_t tmem_slot = base + G::OFF_MISC, abort_addr = tmem_slot + 4, any_addr = tmem_slot + 8;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t rank = CG == 2 ? cluster_rank() : 0;
+    const uint32_t rank = CG == 2 ? uniform(cluster_rank()) : 0;
 
     if (threadIdx.x == 0) {
-        for (uint32_t s = 0; s < S; s++) { mbar_init(full(s), 1); mbar_init(empty(s), 1); mbar_init(scaled(s), 4 * CG); }
+        for (uint32_t s = 0; s < S; s++) { mbar_init(ready(s), 1 + 4 * CG + (CG - 1)); mbar_init(full(s), 1); mbar_init(empty(s), 1); }
+        for (uint32_t s = 0; s < G::Q; s++) { mbar_init(arrived(s), 1); mbar_init(taken(s), 4); }
         for (uint32_t b = 0; b < 2; b++) { mbar_init(acc_full(b), CG == 1 ? 2 : 1); mbar_init(acc_empty(b), 8 * CG); }
         st_shared_u32(abort_addr, 0);
         fence_barrier_init();
@@ -230,7 +260,7 @@ fp4_tile_kernel(const __grid_constant__ CUtensorMap mapB, const __grid_constant_
     __syncthreads();
     if (CG == 2) cluster_sync();
     tc_fence_after();
-    const uint32_t tmem = ld_shared_u32(tmem_slot);
+    const uint32_t tmem = uniform(ld_shared_u32(tmem_slot));
 
     Walk walk(plan, a.gsp, (int)blockIdx.x / CG);
     Piece s;
@@ -240,59 +270,99 @@ fp4_tile_kernel(const __grid_constant__ CUtensorMap mapB, const __grid_constant_
     auto half_of = [&](int t) { return CG == 2 ? (int)rank : t / a.col_tiles; };
     auto column_of = [&](int t) { return CG == 2 ? t : t % a.col_tiles; };
 
+    // Quads of a step that hold blocks, for a pair in either half.
+    auto quads_of = [&](uint32_t rec, int half) { return CG == 2 ? (rec | rec >> 4) & 15 : rec >> (4 * half) & 15; };
+
+    // What decides on addresses is made uniform, and one elected lane issues: otherwise every copy costs its warp 100 cycles for
+    // bringing its operands into uniform registers lane by lane, and the loops below take 800 cycles a step.
     if (warp == 0) {
-        if (lane == 0) {
-            bool ok = true;
-            while (ok && walk.next(s)) {
-                const int half = half_of(s.t), t = column_of(s.t), rt = t * G::BT;
-                const uint32_t b_tiles = (uint32_t)min(G::BT, a.b_row_tiles - rt);
-                const uint2* rec = reinterpret_cast<const uint2*>(a.steps + s.gs);
-                uint2 next = __ldg(rec + s.k0);
-                for (int k = s.k0; k < s.k1; k++, i++) {
-                    const uint32_t st = i % S, stage = base + st * G::STAGE, ks = next.x;
-                    const uint32_t m = CG == 2 ? (next.y | next.y >> 4) & 15 : next.y >> (4 * half) & 15;
-                    if (k + 1 < s.k1) next = __ldg(rec + k + 1);
-                    if (!wait_bar(empty(st), ((i / S) & 1) ^ 1, abort_addr, a.status, 60)) { ok = false; break; }
-                    st_shared_u32(base + G::OFF_MASK + 4 * st, m);
-                    if (m == 0) { mbar_arrive(full(st)); continue; }  // no blocks here
-                    const uint32_t sf = (uint32_t)min(4, a.quads - (int)ks * 4) * 512;
-                    mbar_arrive_expect_tx(full(st), kFp4TileBytes + G::B_BYTES + sf * b_tiles);
-                    bulk_load(stage, a.tiles + ((size_t)(s.gs + k) * 2 + half) * kFp4TileBytes, kFp4TileBytes, full(st));
-                    tma_load_2d(stage + G::OFF_B, &mapB, (int)ks * 128, t * NT + (CG == 2 ? (int)(rank * G::NB) : 0), full(st));
-                    for (uint32_t j = 0; j < b_tiles; j++)
-                        bulk_load(stage + G::OFF_SFB + 2048 * j, a.b_scales + ((size_t)(rt + j) * a.quads + ks * 4) * 512, sf, full(st));
+        // Codes.
+        Records records(a.steps, a.total_steps);
+        bool ok = true;
+        uint32_t st = 0, phase = 1;
+        while (ok && walk.next(s)) {
+            const int half = (int)uniform(half_of(s.t)), gs = (int)uniform(s.gs), k1 = (int)uniform(s.k1);
+            const int row = (int)uniform(column_of(s.t)) * NT + (CG == 2 ? (int)(rank * G::NB) : 0);
+            const uint8_t* tile = a.tiles + ((size_t)(gs + (int)uniform(s.k0)) * 2 + half) * kFp4TileBytes;
+            for (int k = (int)uniform(s.k0); k < k1; k++, tile += 2 * kFp4TileBytes) {
+                const uint32_t rec = records.get(gs + k), stage = base + st * G::STAGE, arrives = rank == 0 ? ready(st) : full(st);
+                ok = __all_sync(~0u, wait_bar(empty(st), phase, abort_addr, a.status, 60));
+                if (!ok) break;
+                if (elect_one()) {
+                    if (quads_of(rec, half) == 0) {  // no blocks here
+                        mbar_arrive(arrives);
+                    } else {
+                        mbar_arrive_expect_tx(arrives, G::STAGE);
+                        bulk_load(stage, tile, kFp4TileCodes, arrives);
+                        tma_load_2d(stage + G::OFF_B, &mapB, (int)(rec >> 8) * 128, row, arrives);
+                    }
                 }
+                __syncwarp();
+                if (++st == S) { st = 0; phase ^= 1; }
             }
         }
-        __syncwarp();
+    } else if (warp == 2) {
+        // Scales.
+        Records records(a.steps, a.total_steps);
+        bool ok = true;
+        uint32_t st = 0, phase = 1;
+        while (ok && walk.next(s)) {
+            const int half = (int)uniform(half_of(s.t)), gs = (int)uniform(s.gs), k1 = (int)uniform(s.k1), rt = (int)uniform(column_of(s.t)) * G::BT;
+            const uint32_t b_tiles = (uint32_t)min(G::BT, a.b_row_tiles - rt);
+            const uint8_t* tile = a.tiles + ((size_t)(gs + (int)uniform(s.k0)) * 2 + half) * kFp4TileBytes + kFp4TileCodes;
+            const uint8_t* panel = a.b_scales + (size_t)rt * a.quads * 512;
+            for (int k = (int)uniform(s.k0); k < k1; k++, tile += 2 * kFp4TileBytes) {
+                const uint32_t rec = records.get(gs + k), stage = base + G::OFF_SF + st * G::SF_STAGE, quad = (rec >> 8) * 4;
+                const uint32_t bytes = min(4u, (uint32_t)a.quads - quad) * 512;
+                ok = __all_sync(~0u, wait_bar(taken(st), phase, abort_addr, a.status, 61));
+                if (!ok) break;
+                if (elect_one()) {
+                    if (quads_of(rec, half) == 0) {
+                        mbar_arrive(arrived(st));
+                    } else {
+                        mbar_arrive_expect_tx(arrived(st), 2048 + bytes * b_tiles);
+                        bulk_load(stage, tile, 2048, arrived(st));
+                        bulk_load(stage + 2048, panel + (size_t)quad * 512, bytes, arrived(st));
+                        if (G::BT == 2 && b_tiles == 2) bulk_load(stage + 4096, panel + ((size_t)a.quads + quad) * 512, bytes, arrived(st));
+                    }
+                }
+                __syncwarp();
+                if (++st == G::Q) { st = 0; phase ^= 1; }
+            }
+        }
     } else if (warp == 1 && rank == 0) {
         // The whole warp walks, so that what the MMAs are given is uniform; one lane issues.
         constexpr uint32_t idesc = idesc_fp4(128 * CG, NT, FMT == SMAT_FP4_MX);
+        const uint64_t da0 = smem_desc_k_sw128(base), db0 = smem_desc_k_sw128(base + G::OFF_B);
+        const uint32_t da_hi = (uint32_t)(da0 >> 32), db_hi = (uint32_t)(db0 >> 32);
+        Records records(a.steps, a.total_steps);
         bool ok = true;
-        for (uint32_t n = 0; ok && walk.next(s); n++) {
+        uint32_t st = 0, phase = 0, n = 0;
+        for (; ok && walk.next(s); n++) {
             const uint32_t buf = n % G::ACC;
-            ok = __all_sync(~0u, wait_bar(acc_empty(buf), ((n / G::ACC) & 1) ^ 1, abort_addr, a.status, 61));
+            const int half = (int)uniform(half_of(s.t)), gs = (int)uniform(s.gs), k1 = (int)uniform(s.k1);
+            ok = __all_sync(~0u, wait_bar(acc_empty(buf), ((n / G::ACC) & 1) ^ 1, abort_addr, a.status, 62));
             tc_fence_after();
             uint32_t acc = 0;
-            for (int k = s.k0; ok && k < s.k1; k++, i++) {
-                const uint32_t st = i % S, stage = base + st * G::STAGE;
-                ok = __all_sync(~0u, wait_bar(scaled(st), (i / S) & 1, abort_addr, a.status, 62));
+            for (int k = (int)uniform(s.k0); ok && k < k1; k++) {
+                const uint32_t mask = quads_of(records.get(gs + k), half);
+                const uint32_t sf = tmem + 256 + st * G::SF_COLUMNS;
+                const uint32_t da = (uint32_t)da0 + st * (G::STAGE >> 4), db = (uint32_t)db0 + st * (G::STAGE >> 4);
+                ok = __all_sync(~0u, wait_bar(ready(st), phase, abort_addr, a.status, 63));
                 if (!ok) break;
                 tc_fence_after();
-                const uint32_t mask = uniform(ld_shared_u32(base + G::OFF_MASK + 4 * st));
-                const uint32_t sf = tmem + 256 + st * G::SF_COLUMNS;
-                const uint64_t da = smem_desc_k_sw128(stage), db = smem_desc_k_sw128(stage + G::OFF_B);
                 if (elect_one()) {
                     uint32_t on = acc;
 #pragma unroll
                     for (uint32_t q = 0; q < 4; q++) {
                         if (!(mask >> q & 1)) continue;
-                        mma_fp4<FMT, CG>(tmem + buf * NT, da + q * 2, db + q * 2, idesc, sf + q * 4, sf + 16 + q * 4 * G::BT, on);
+                        mma_fp4<FMT, CG>(tmem + buf * NT, da + q * 2, da_hi, db + q * 2, db_hi, idesc, sf + q * 4, sf + 16 + q * 4 * G::BT, on);
                         on = 1;
                     }
                     commit<CG>(empty(st));
                 }
                 acc |= mask;
+                if (++st == S) { st = 0; phase ^= 1; }
                 __syncwarp();
             }
             if (ok && elect_one()) {
@@ -302,33 +372,47 @@ fp4_tile_kernel(const __grid_constant__ CUtensorMap mapB, const __grid_constant_
             }
             __syncwarp();
         }
-    } else if (warp >= 12) {
-        // Scales to tensor memory: four words a lane and scale tile, the same in all lane quarters.
-        const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21) + 256;
+    } else if (warp == 3 && rank == 1) {
+        // Tells the first CTA what has arrived here.
         bool ok = true;
+        uint32_t st = 0, phase = 0;
         while (ok && walk.next(s)) {
-            for (int k = s.k0; k < s.k1; k++, i++) {
-                const uint32_t st = i % S, from = base + st * G::STAGE + lane * 16;
-                ok = __all_sync(~0u, wait_bar(full(st), (i / S) & 1, abort_addr, a.status, 63));
+            for (int k = s.k0; k < s.k1; k++) {
+                ok = __all_sync(~0u, wait_bar(full(st), phase, abort_addr, a.status, 66));
                 if (!ok) break;
-                tc_fence_after();
-                uint4 v[4 + 4 * G::BT];
+                if (lane == 0) arrive_at_first(ready(st));
+                if (++st == S) { st = 0; phase ^= 1; }
+            }
+        }
+    } else if (warp >= 12) {
+        // Scales to tensor memory, as soon as the MMAs have used what is there: four words a lane and scale tile, the same in all lane
+        // quarters.  A set of four warps takes every other step.
+        const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21) + 256;
+        uint32_t steps = 0;
+        while (walk.next(s)) steps += (uint32_t)(s.k1 - s.k0);
+        for (i = (uint32_t)(warp - 12) / 4; i < steps; i += 2) {
+            const uint32_t st = i % S, from = base + G::OFF_SF + i % G::Q * G::SF_STAGE + lane * 16;
+            if (!__all_sync(~0u, wait_bar(arrived(i % G::Q), (i / G::Q) & 1, abort_addr, a.status, 67) &&
+                                     wait_bar(empty(st), ((i / S) & 1) ^ 1, abort_addr, a.status, 68)))
+                break;
+            tc_fence_after();
+            uint4 v[4 + 4 * G::BT];
 #pragma unroll
-                for (int q = 0; q < 4; q++) v[q] = ld_shared_v4(from + G::OFF_SFA + q * 512);
+            for (int q = 0; q < 4; q++) v[q] = ld_shared_v4(from + q * 512);
 #pragma unroll
-                for (int q = 0; q < 4; q++)
+            for (int q = 0; q < 4; q++)
 #pragma unroll
-                    for (int j = 0; j < G::BT; j++) v[4 + q * G::BT + j] = ld_shared_v4(from + G::OFF_SFB + j * 2048 + q * 512);
-                const uint32_t to = lanes + st * G::SF_COLUMNS;
+                for (int j = 0; j < G::BT; j++) v[4 + q * G::BT + j] = ld_shared_v4(from + 2048 * (1 + j) + q * 512);
+            const uint32_t to = lanes + st * G::SF_COLUMNS;
 #pragma unroll
-                for (int j = 0; j < 1 + G::BT; j++) tmem_st_x16(to + 16 * j, v + 4 * j);
-                tmem_st_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) {
-                    if (CG == 2 && rank == 1) arrive_at_first(scaled(st));
-                    else mbar_arrive(scaled(st));
-                }
+            for (int j = 0; j < 1 + G::BT; j++) tmem_st_x16(to + 16 * j, v + 4 * j);
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if (CG == 2 && rank == 1) arrive_at_first(ready(st));
+                else mbar_arrive(ready(st));
+                mbar_arrive(taken(i % G::Q));
             }
         }
     } else if (warp >= 4) {
@@ -348,16 +432,21 @@ fp4_tile_kernel(const __grid_constant__ CUtensorMap mapB, const __grid_constant_
                     cs[j][e] = a.b_row_scale && c < a.N ? __ldg(a.b_row_scale + c) : 1.f;
                 }
             // of a pair, only the one step of an empty group has no MMA
-            bool none = CG == 2 && s.ns == 1 && __ldg(&a.steps[s.gs].mask) == 0;
-            if (!__all_sync(~0u, wait_bar(acc_full(buf), (n / G::ACC) & 1, abort_addr, a.status, 66))) break;
+            bool none = CG == 2 && s.ns == 1 && (__ldg(a.steps + s.gs) & 0xff) == 0;
+            if (!__all_sync(~0u, wait_bar(acc_full(buf), (n / G::ACC) & 1, abort_addr, a.status, 69))) break;
             tc_fence_after();
             if (CG == 1) none = ld_shared_u32(any_addr + 4 * buf) == 0;
-#pragma unroll
-            for (int jc = 0; jc < (NT + 127) / 128; jc++) {
-                const int c = c0 + jc * 128;
-                if (c >= cols) break;
-                if (s.cut) {
-                    float* to = a.scratch + (size_t)s.slot * (128 * CG * NT) + (CG == 2 ? (int)rank * 128 : 0) + row0 + lane;
+            auto release = [&]() {  // all of this warp's accumulators are read
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if (CG == 2 && rank == 1) arrive_at_first(acc_empty(buf));
+                    else mbar_arrive(acc_empty(buf));
+                }
+            };
+            if (s.cut) {
+                float* to = a.scratch + (size_t)s.slot * (128 * CG * NT) + (CG == 2 ? (int)rank * 128 : 0) + row0 + lane;
+                for (int c = c0; c < cols; c += 128)
                     for (int j0 = c; j0 < min(c + 64, cols); j0 += 16) {
                         uint32_t u[16];
                         tmem_ld_x16(lanes + buf * NT + j0, u);
@@ -365,14 +454,19 @@ fp4_tile_kernel(const __grid_constant__ CUtensorMap mapB, const __grid_constant_
 #pragma unroll
                         for (int j = 0; j < 16; j++) to[(size_t)(j0 + j) * (128 * CG)] = none ? 0.f : __uint_as_float(u[j]);
                     }
-                    continue;
-                }
+                release();
+                continue;
+            }
+            // 64 columns at a time: scaled, rounded, through shared memory and out.  Of 256 columns (one accumulator) the second half
+            // is taken into registers before the first is stored, so that the next unit's MMAs need not wait for that.
+            auto take = [&](int jc, uint32_t (&w)[NT < 64 ? NT / 2 : 32]) {
+                const int c = c0 + jc * 128;
                 st_shared_u32(col + lane * 4, __float_as_uint(cs[jc][0]));
                 st_shared_u32(col + lane * 4 + 128, __float_as_uint(cs[jc][1]));
                 __syncwarp();
 #pragma unroll
                 for (int j0 = 0; j0 < (NT < 64 ? NT : 64); j0 += 16) {
-                    uint32_t u[16], w[8];
+                    uint32_t u[16];
                     tmem_ld_x16(lanes + buf * NT + c + j0, u);
                     tmem_ld_wait();
 #pragma unroll
@@ -380,12 +474,17 @@ fp4_tile_kernel(const __grid_constant__ CUtensorMap mapB, const __grid_constant_
                         const uint4 f = ld_shared_v4(col + (j0 + 4 * j) * 4);
                         const float v0 = __uint_as_float(u[4 * j]) * rs * __uint_as_float(f.x), v1 = __uint_as_float(u[4 * j + 1]) * rs * __uint_as_float(f.y);
                         const float v2 = __uint_as_float(u[4 * j + 2]) * rs * __uint_as_float(f.z), v3 = __uint_as_float(u[4 * j + 3]) * rs * __uint_as_float(f.w);
-                        w[2 * j] = none ? 0 : a.c_dtype == SMAT_F16 ? pack2<SMAT_F16>(v0, v1) : pack2<SMAT_BF16>(v0, v1);
-                        w[2 * j + 1] = none ? 0 : a.c_dtype == SMAT_F16 ? pack2<SMAT_F16>(v2, v3) : pack2<SMAT_BF16>(v2, v3);
+                        w[j0 / 2 + 2 * j] = none ? 0 : a.c_dtype == SMAT_F16 ? pack2<SMAT_F16>(v0, v1) : pack2<SMAT_BF16>(v0, v1);
+                        w[j0 / 2 + 2 * j + 1] = none ? 0 : a.c_dtype == SMAT_F16 ? pack2<SMAT_F16>(v2, v3) : pack2<SMAT_BF16>(v2, v3);
                     }
-                    st_shared_v4(out + lane * 128 + (((j0 / 8) ^ (lane & 7)) << 4), w[0], w[1], w[2], w[3]);
-                    st_shared_v4(out + lane * 128 + (((j0 / 8 + 1) ^ (lane & 7)) << 4), w[4], w[5], w[6], w[7]);
                 }
+                __syncwarp();
+            };
+            auto store = [&](int jc, const uint32_t (&w)[NT < 64 ? NT / 2 : 32]) {
+                const int c = c0 + jc * 128;
+#pragma unroll
+                for (int j = 0; j < (NT < 64 ? NT / 8 : 8); j++)
+                    st_shared_v4(out + lane * 128 + ((j ^ (lane & 7)) << 4), w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
                 __syncwarp();
                 const int width = min(64, cols - c);
                 uint16_t* const to = static_cast<uint16_t*>(a.C) + (size_t)m0 * a.N + n0 + c;
@@ -401,13 +500,15 @@ fp4_tile_kernel(const __grid_constant__ CUtensorMap mapB, const __grid_constant_
                         for (int j = lane; j < width; j += 32) to[(size_t)r * a.N + j] = ld_shared_u16(out + r * 128 + (((j >> 3) ^ (r & 7)) << 4) + (j & 7) * 2);
                 }
                 __syncwarp();
-            }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-                if (CG == 2 && rank == 1) arrive_at_first(acc_empty(buf));
-                else mbar_arrive(acc_empty(buf));
-            }
+            };
+            uint32_t w[(NT + 127) / 128][NT < 64 ? NT / 2 : 32];
+#pragma unroll
+            for (int jc = 0; jc < (NT + 127) / 128; jc++)
+                if (c0 + jc * 128 < cols) take(jc, w[jc]);
+            release();
+#pragma unroll
+            for (int jc = 0; jc < (NT + 127) / 128; jc++)
+                if (c0 + jc * 128 < cols) store(jc, w[jc]);
         }
     }
 
@@ -595,6 +696,7 @@ int launch_fp4_tile(const Fp4View& A, const Fp4Rhs& B, void* C, int c_dtype, siz
     a.rows = (int)(A.block_rows * 16);
     a.N = (int)N;
     a.quads = (int)fp4_quads(A.K);
+    a.total_steps = (int)A.total_steps;
     a.b_row_tiles = (int)((N + 127) / 128);
     const int groups = (int)((A.block_rows + kFp4GroupRows - 1) / kFp4GroupRows);
     switch (nt) {
