@@ -44,12 +44,13 @@ __device__ __forceinline__ void e2m1x4_to_f16(uint16_t w, uint32_t& h0, uint32_t
     asm("{\n\t.reg .b8 b0, b1;\n\tmov.b16 {b0, b1}, %2;\n\tcvt.rn.f16x2.e2m1x2 %0, b0;\n\tcvt.rn.f16x2.e2m1x2 %1, b1;\n\t}"
         : "=r"(h0), "=r"(h1) : "h"(w));
 }
-// A pair of fp16 that came from e2m1 -> the same pair in bf16.  The magnitude shifted down by the three bits that the exponent
-// field is wider reads as the value times 2^-112 (0 stays 0, all others are normal); a product in bf16 takes that back, exactly.
-__device__ __forceinline__ uint32_t f16_code_to_bf16(uint32_t h2) {
+// A pair of fp16 that came from e2m1 -> the same pair times `scale` in bf16, exact where the product fits bf16.  The magnitude shifted
+// down by the three bits that the exponent field is wider reads as the value times 2^-112 (0 stays 0, all others are normal); the
+// factor takes that back.  scale * 2^112 has to be finite in bf16.
+__device__ __forceinline__ uint32_t f16_code_to_bf16(uint32_t h2, float scale) {
     const uint32_t small = (h2 & 0x80008000u) | ((h2 & 0x7fff7fffu) >> 3);
-    const __nv_bfloat162 up = __floats2bfloat162_rn(5192296858534827628530496329220096.f, 5192296858534827628530496329220096.f);  // 2^112
-    const __nv_bfloat162 v = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&small), up);
+    const float up = scale * 5192296858534827628530496329220096.f;  // 2^112
+    const __nv_bfloat162 v = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&small), __floats2bfloat162_rn(up, up));
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 // Eight fp32 -> eight codes, to nearest, ties to even, saturating at 6 (no NaN comes here).

@@ -36,13 +36,23 @@ struct Fp4Where {         // of what the tiles of a step are made
     uint16_t blocks[16];  // bit c: the block-row has a block in columns 16 c to 16 c + 15 of these
 };
 
+// Products with B in 16 bits walk a block-row four blocks at a time, kept by the plan in the order in which a warp's lanes use them:
+// 512 bytes of codes (lane l: 16 bytes, a word for each block: columns 4 (l % 4) to + 3 of rows 2 (l / 4) and 2 (l / 4) + 1), 64 bytes
+// of scales (8 for each pair of rows: two a block) and four block columns.  The last four of a block-row may be fewer; the rest is
+// zeros, with the column of the last block.
+constexpr size_t kFp4FourBytes = 512 + 64 + 16;
+struct Fp4Row {
+    int first, blocks;  // four to begin with, number of blocks
+};
+
 // A stored matrix of 16 x 16 blocks in 4 bits and what a plan worked out about block-rows [brow_begin, brow_end).  Device memory.
 struct Fp4View {
     const uint8_t* codes = nullptr;
     const uint8_t* scales = nullptr;
     const float* row_scale = nullptr;  // of the whole matrix, or null: ones
     const int* colidx = nullptr;
-    const int2* range = nullptr;  // first and last + 1 block of every block-row of the range; empty where the arrays were inconsistent
+    const Fp4Row* rows = nullptr;    // of the range; empty where the arrays were inconsistent
+    const uint8_t* fours = nullptr;
     int fmt = 0;
     size_t K = 0, brow_begin = 0, block_rows = 0;
     const uint32_t* steps = nullptr;  // null: the plan has no tiles

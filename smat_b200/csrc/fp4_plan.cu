@@ -1,4 +1,5 @@
 // Plans for products of a block-sparse matrix in 4 bits (smat_fp4_plan_*).
+#include <algorithm>
 #include <new>
 
 #include "fp4_format.h"
@@ -7,7 +8,11 @@
 struct smat_fp4_plan {
     smat::Fp4View v;
     int device = -1;
-    void* buffer = nullptr;  // totals, block ranges and first steps
+    void* buffer = nullptr;  // totals, block ranges, rows and first steps
+    const int2* range = nullptr;
+    const int* four_first = nullptr;
+    smat::Fp4Row* rows = nullptr;
+    void* fours = nullptr;
     void* steps = nullptr;   // steps and what their tiles are made of
     smat::Fp4Where* where = nullptr;
     void* tiles = nullptr;
@@ -24,7 +29,8 @@ constexpr size_t kFp4TileFill = 8;
 // Looks a block-row's pointers and columns over (a CTA a block-row): they have to lie in the arrays and the matrix, the columns in
 // ascending order.  An inconsistent block-row is left out (empty) and reported.  totals: blocks, longest block-row.
 __global__ void __launch_bounds__(kThreads) fp4_ranges_kernel(const int* __restrict__ rowptr, const int* __restrict__ colidx, size_t K, size_t nnzb,
-                                                              int2* __restrict__ range, unsigned long long* __restrict__ totals, int* status) {
+                                                              int2* __restrict__ range, int* __restrict__ fours,
+                                                              unsigned long long* __restrict__ totals, int* status) {
     const size_t r = blockIdx.x;
     const int lo = __ldg(rowptr + r), hi = __ldg(rowptr + r + 1);
     int bad = lo < 0 || hi < lo || (size_t)hi > nnzb ? kStatusBadRowptr : 0;
@@ -39,10 +45,34 @@ __global__ void __launch_bounds__(kThreads) fp4_ranges_kernel(const int* __restr
     if (threadIdx.x == 0) {
         if (bad) atomicCAS(status, 0, bad);
         range[r] = bad ? make_int2(0, 0) : make_int2(lo, hi);
+        fours[r + 1] = bad ? 0 : (hi - lo + 3) / 4;
         if (!bad) {
             atomicAdd(totals, (unsigned long long)(hi - lo));
             atomicMax(totals + 1, (unsigned long long)(hi - lo));
         }
+    }
+}
+
+// Fours of a block-row (a CTA a block-row, a warp a four); `first` is scanned.
+__global__ void __launch_bounds__(kThreads) fp4_fours_kernel(const int2* __restrict__ range, const int* __restrict__ first, const int* __restrict__ colidx,
+                                                             const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
+                                                             Fp4Row* __restrict__ rows, uint8_t* __restrict__ fours) {
+    const int2 mine = range[blockIdx.x];
+    const int f0 = first[blockIdx.x], lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
+    if (threadIdx.x == 0) rows[blockIdx.x] = {f0, mine.y - mine.x};
+    for (int f = threadIdx.x / 32; f * 4 < mine.y - mine.x; f += kThreads / 32) {
+        uint8_t* const to = fours + (size_t)(f0 + f) * kFp4FourBytes;
+        uint32_t w[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int p = mine.x + 4 * f + u;
+            const uint16_t* row = reinterpret_cast<const uint16_t*>(codes + (size_t)p * 128 + g * 16);  // rows 2g and 2g + 1, four codes an element
+            w[u] = p < mine.y ? __ldg(row + t) | (uint32_t)__ldg(row + 4 + t) << 16 : 0;
+        }
+        *reinterpret_cast<uint4*>(to + lane * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+        const int p = mine.x + 4 * f + t;  // lane (g, t): scales of rows 2g and 2g + 1 of block t
+        *reinterpret_cast<uint16_t*>(to + 512 + g * 8 + t * 2) = p < mine.y ? __ldg(reinterpret_cast<const uint16_t*>(scales + (size_t)p * 16) + g) : 0;
+        if (lane < 4) *reinterpret_cast<int*>(to + 576 + lane * 4) = __ldg(colidx + min(mine.x + 4 * f + lane, mine.y - 1));
     }
 }
 
@@ -135,8 +165,14 @@ __global__ void __launch_bounds__(kStepThreads) fp4_tiles_kernel(const uint8_t* 
     }
 }
 
-int fill_tiles(const smat_fp4_plan* p, cudaStream_t stream) {
+// What a plan holds of codes and scales.
+int fill_values(const smat_fp4_plan* p, cudaStream_t stream) {
     const Fp4View& v = p->v;
+    if (!v.block_rows) return SMAT_OK;
+    fp4_fours_kernel<<<(unsigned)v.block_rows, kThreads, 0, stream>>>(p->range, p->four_first, v.colidx, v.codes, v.scales, p->rows,
+                                                                      static_cast<uint8_t*>(p->fours));
+    count_launch();
+    SMAT_CUDA_TRY(cudaGetLastError());
     if (!v.tiles || !v.blocks) return SMAT_OK;
     uint8_t* tiles = static_cast<uint8_t*>(p->tiles);
     if (v.fmt == SMAT_FP4_NV) fp4_tiles_kernel<SMAT_FP4_NV><<<(unsigned)v.total_steps, kStepThreads, 0, stream>>>(v.codes, v.scales, p->where, tiles);
@@ -150,15 +186,19 @@ int fill_tiles(const smat_fp4_plan* p, cudaStream_t stream) {
 int build_plan(smat_fp4_plan* p, const int* rowptr, const int* colidx, size_t nnzb, bool with_tiles, const DeviceCtx* ctx, cudaStream_t stream) {
     Fp4View& v = p->v;
     const size_t groups = (v.block_rows + kFp4GroupRows - 1) / kFp4GroupRows;
-    const size_t range_bytes = (v.block_rows * sizeof(int2) + 15) / 16 * 16, bytes = 16 + range_bytes + (groups + 1) * sizeof(int);
+    // totals, ranges and rows of block-rows, first fours of block-rows, first steps of groups
+    const size_t bytes = 16 + v.block_rows * (sizeof(int2) + sizeof(Fp4Row)) + (v.block_rows + 1 + groups + 1) * sizeof(int);
     SMAT_CUDA_TRY(cudaMalloc(&p->buffer, bytes));
     unsigned long long* totals = static_cast<unsigned long long*>(p->buffer);
     int2* range = reinterpret_cast<int2*>(totals + 2);
-    int* gsp = reinterpret_cast<int*>(reinterpret_cast<char*>(range) + range_bytes);
+    p->rows = reinterpret_cast<Fp4Row*>(range + v.block_rows);
+    int* fours = reinterpret_cast<int*>(p->rows + v.block_rows);
+    int* gsp = fours + v.block_rows + 1;
     SMAT_CUDA_TRY(cudaMemsetAsync(p->buffer, 0, bytes, stream));
-    fp4_ranges_kernel<<<(unsigned)v.block_rows, kThreads, 0, stream>>>(rowptr + v.brow_begin, colidx, v.K, nnzb, range, totals, ctx->d_status);
+    fp4_ranges_kernel<<<(unsigned)v.block_rows, kThreads, 0, stream>>>(rowptr + v.brow_begin, colidx, v.K, nnzb, range, fours, totals, ctx->d_status);
     count_launch();
     SMAT_CUDA_TRY(cudaGetLastError());
+    if (int rc = scan_inplace_async(fours, (int)v.block_rows + 1, stream)) return rc;
     const int words = (int)((v.K + 32 * kFp4StepColumns - 1) / (32 * kFp4StepColumns));
     if (with_tiles) {
         fp4_steps_kernel<false><<<(unsigned)groups, kStepThreads, words * 4, stream>>>(range, colidx, (int)v.block_rows, words, gsp, nullptr, nullptr);
@@ -167,40 +207,46 @@ int build_plan(smat_fp4_plan* p, const int* rowptr, const int* colidx, size_t nn
         if (int rc = scan_inplace_async(gsp, (int)groups + 1, stream)) return rc;
     }
     unsigned long long h_totals[2] = {0, 0};
-    int h_steps = 0;
+    int h_steps = 0, h_fours = 0;
     SMAT_CUDA_TRY(cudaMemcpyAsync(h_totals, totals, sizeof(h_totals), cudaMemcpyDeviceToHost, stream));
+    SMAT_CUDA_TRY(cudaMemcpyAsync(&h_fours, fours + v.block_rows, sizeof(int), cudaMemcpyDeviceToHost, stream));
     SMAT_CUDA_TRY(cudaMemcpyAsync(&h_steps, gsp + groups, sizeof(int), cudaMemcpyDeviceToHost, stream));
     SMAT_CUDA_TRY(cudaStreamSynchronize(stream));
-    v.range = range;
+    p->range = range;
+    p->four_first = fours;
+    v.rows = p->rows;
     v.blocks = h_totals[0];
     v.longest = h_totals[1];
+    SMAT_CUDA_TRY(cudaMalloc(&p->fours, std::max<size_t>(h_fours, 1) * kFp4FourBytes));
+    v.fours = static_cast<const uint8_t*>(p->fours);
     const size_t steps = (size_t)h_steps;
-    if (!with_tiles || v.blocks < kFp4TileFill * steps) return SMAT_OK;
-    SMAT_CUDA_TRY(cudaMalloc(&p->steps, steps * (sizeof(uint32_t) + sizeof(Fp4Where))));
-    uint32_t* step = static_cast<uint32_t*>(p->steps);
-    p->where = reinterpret_cast<Fp4Where*>(step + steps);
-    SMAT_CUDA_TRY(cudaMalloc(&p->tiles, steps * 2 * kFp4TileBytes));
-    SMAT_CUDA_TRY(cudaMemsetAsync(p->steps, 0, steps * (sizeof(uint32_t) + sizeof(Fp4Where)), stream));
-    SMAT_CUDA_TRY(cudaFuncSetAttribute(fp4_steps_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, words * 8));
-    fp4_steps_kernel<true><<<(unsigned)groups, kStepThreads, words * 8, stream>>>(range, colidx, (int)v.block_rows, words, gsp, step, p->where);
-    count_launch();
-    SMAT_CUDA_TRY(cudaGetLastError());
-    p->gsp = new (std::nothrow) int[groups + 1];
-    if (!p->gsp) return fail(SMAT_ERR_NOMEM, "out of host memory");
-    SMAT_CUDA_TRY(cudaMemcpyAsync(p->gsp, gsp, (groups + 1) * sizeof(int), cudaMemcpyDeviceToHost, stream));
-    v.gsp = gsp;
-    v.h_gsp = p->gsp;
-    v.total_steps = steps;
-    v.steps = step;
-    v.tiles = static_cast<const uint8_t*>(p->tiles);
-    if (int rc = fill_tiles(p, stream)) return rc;
+    if (with_tiles && v.blocks >= kFp4TileFill * steps) {
+        SMAT_CUDA_TRY(cudaMalloc(&p->steps, steps * (sizeof(uint32_t) + sizeof(Fp4Where))));
+        uint32_t* step = static_cast<uint32_t*>(p->steps);
+        p->where = reinterpret_cast<Fp4Where*>(step + steps);
+        SMAT_CUDA_TRY(cudaMalloc(&p->tiles, steps * 2 * kFp4TileBytes));
+        SMAT_CUDA_TRY(cudaMemsetAsync(p->steps, 0, steps * (sizeof(uint32_t) + sizeof(Fp4Where)), stream));
+        SMAT_CUDA_TRY(cudaFuncSetAttribute(fp4_steps_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, words * 8));
+        fp4_steps_kernel<true><<<(unsigned)groups, kStepThreads, words * 8, stream>>>(range, colidx, (int)v.block_rows, words, gsp, step, p->where);
+        count_launch();
+        SMAT_CUDA_TRY(cudaGetLastError());
+        p->gsp = new (std::nothrow) int[groups + 1];
+        if (!p->gsp) return fail(SMAT_ERR_NOMEM, "out of host memory");
+        SMAT_CUDA_TRY(cudaMemcpyAsync(p->gsp, gsp, (groups + 1) * sizeof(int), cudaMemcpyDeviceToHost, stream));
+        v.gsp = gsp;
+        v.h_gsp = p->gsp;
+        v.total_steps = steps;
+        v.steps = step;
+        v.tiles = static_cast<const uint8_t*>(p->tiles);
+    }
+    if (int rc = fill_values(p, stream)) return rc;
     SMAT_CUDA_TRY(cudaStreamSynchronize(stream));
     return SMAT_OK;
 }
 
 cudaError_t free_plan(smat_fp4_plan* p) {
     cudaError_t e = cudaSuccess;
-    for (void* m : {p->buffer, p->steps, p->tiles}) {
+    for (void* m : {p->buffer, p->fours, p->steps, p->tiles}) {
         const cudaError_t f = cudaFree(m);
         if (e == cudaSuccess) e = f;
     }
@@ -274,7 +320,7 @@ int smat_fp4_plan_set_values(smat_fp4_plan* plan, void* stream) {
     clear_error();
     if (!plan) return fail(SMAT_ERR_BAD_ARG, "plan is NULL");
     if (int rc = check_plan_device(plan)) return rc;
-    return fill_tiles(plan, (cudaStream_t)stream);
+    return fill_values(plan, (cudaStream_t)stream);
 }
 
 int smat_fp4_plan_spmm(const smat_fp4_plan* plan, const void* B, int dtype, void* C, size_t N, void* stream) {

@@ -1,12 +1,17 @@
 // C = A x B with A in 4-bit blocks and few columns of B: warps walk the blocks of a block-row.
 //
-// Mathematics.  A block is 16 x 16 and a scale covers a whole row of it, so the block's product P = codes(A) x B is formed with the
-// codes as they are (exact in fp16 and bf16) by one m16n8k16 MMA per 8 columns, and C += scale(row) * P is one fp32 FMA per
-// element: any scale format, nothing rounded on the way in.  B in 4 bits has one scale for the block's 16 rows as well.
+// Mathematics.  A block is 16 x 16 and a scale covers a whole row of it.  e2m1 times e4m3 has at most six significant bits and fits
+// fp16 and bf16, so with SMAT_FP4_NV the scaled values go into m16n8k16 MMAs that accumulate in fp32, nothing rounded on the way in.
+// Powers of two beyond the range of 16 bits (SMAT_FP4_MX) and scales of B in 4 bits are applied to a block's product instead, one
+// fp32 FMA per element.
 //
-// Layout.  The 128 bytes of a block are read as they lie, one word per lane.  Word l holds half of row l / 2; MMA rows g and g + 8
-// stand for rows 2g and 2g + 1 of the block, which lie in the words of lanes 4g .. 4g + 3, so one exchange with lane l ^ 2 gives
-// each lane four columns of both rows.  The k order inside a block is permuted by that, in the same way for A and B.
+// Layout.  Plans keep the blocks in fours in the order in which a warp's lanes take them (fp4_format.h): read as they are stored, a
+// word a lane and block, they cost twice the instructions.  MMA rows g and g + 8 stand for rows 2g and 2g + 1 of the block, the k
+// order inside a block is permuted in the same way for A and B.
+//
+// What bounds it: instructions (some 20 a block and 8 columns) and, from 16 columns on, the rows of B that every block gathers through
+// L2.  The next four are on their way while a four is multiplied, without branches: a load behind one is waited for before the next
+// is issued (39 us for one token and the layer 8192 x 28672 at 20 %, 22 without).
 #include "fp4_device.cuh"
 #include "smat_internal.h"
 
@@ -18,21 +23,21 @@ namespace {
 constexpr int kWarps = 8;
 
 template <bool BF16>
-__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
     if constexpr (BF16)
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
-            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
     else
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
-            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 
 struct StreamArgs {
-    const uint8_t* codes;
-    const uint8_t* scales;
+    const uint8_t* fours;
+    const Fp4Row* rows;
     const float* row_scale;  // first of the range, or null
-    const int* colidx;
-    const int2* range;
     const void* B;
     const uint8_t* b_scales;
     const float* b_row_scale;
@@ -42,10 +47,22 @@ struct StreamArgs {
     size_t K;
 };
 
+// Four blocks, and U of them with their rows of B.
+struct Four {
+    uint4 w;     // codes
+    uint2 s;     // scales
+    int4 col;
+};
+template <int BT, int NT, int U>
+struct Panel {
+    uint2 b[U][NT];                            // 16 bits: four values; 4 bits: four codes in x
+    uint16_t q[BT == kFp4Rhs ? U : 1][NT][2];  // 4 bits: scales of columns 2t and 2t + 1
+};
+
 // BT: SMAT_F16, SMAT_BF16 or kFp4Rhs.  NT: 8-column tiles of C per warp.  WR warps of a CTA (times the CTAs of a cluster) share a
 // block-row; a CTA holds kWarps / WR block-rows.
 template <int BT, int FMT, int NT, int U>
-__global__ void __launch_bounds__(kWarps * 32) fp4_stream_kernel(const StreamArgs a, int wr) {
+__global__ void __launch_bounds__(kWarps * 32, NT <= 2 ? 3 : 2) fp4_stream_kernel(const StreamArgs a, int wr) {
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
     const int cl = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
@@ -54,8 +71,8 @@ __global__ void __launch_bounds__(kWarps * 32) fp4_stream_kernel(const StreamArg
     const int row_ctas = (a.block_rows + rows_per_cta - 1) / rows_per_cta;
     const int r0 = (int)(blockIdx.x / cl % row_ctas) * rows_per_cta, r = r0 + warp / wr;
     const int n0 = (int)(blockIdx.x / cl / row_ctas) * NT * 8;
-    const int kbase = (t & 1) * 8 + (t >> 1) * 4;
     const size_t quads = (a.K + 63) / 64;
+    constexpr bool FOLD = FMT == SMAT_FP4_NV && BT != kFp4Rhs;  // scales go into the values of A
 
     float acc[NT][4];
 #pragma unroll
@@ -64,64 +81,86 @@ __global__ void __launch_bounds__(kWarps * 32) fp4_stream_kernel(const StreamArg
         for (int e = 0; e < 4; e++) acc[j][e] = 0.f;
 
     if (r < a.block_rows) {
-        const int2 range = a.range[r];
-        const int n = range.y - range.x, parts = wr * cl, part = rank * wr + warp % wr;
-        const int lo = range.x + (int)((long long)n * part / parts), hi = range.x + (int)((long long)n * (part + 1) / parts);
-        for (int p0 = lo; p0 < hi; p0 += 32) {
-            const int mine = p0 + lane < hi ? __ldg(a.colidx + p0 + lane) : 0;
-            const int cnt = min(32, hi - p0);
-            for (int u0 = 0; u0 < cnt; u0 += U) {
-                uint32_t w[U], sc[U], b[U][NT][2];
-                uint32_t bs[U][NT][2];
+        const Fp4Row row = a.rows[r];
+        const int n = (row.blocks + 3) / 4, parts = wr * cl, part = rank * wr + warp % wr;
+        const int lo = (int)((long long)n * part / parts), hi = (int)((long long)n * (part + 1) / parts);
+        const uint8_t* at = a.fours + (size_t)(row.first + lo) * kFp4FourBytes;
+        const uint8_t* b0[NT];  // this lane's columns of C; those beyond N are computed from the last one and not stored
 #pragma unroll
-                for (int u = 0; u < U; u++) {
-                    const int col = __shfl_sync(~0u, mine, (u0 + u) & 31);
-                    const bool in = u0 + u < cnt;
-                    const size_t p = (size_t)(p0 + u0 + u);
-                    w[u] = in ? __ldg(reinterpret_cast<const uint32_t*>(a.codes + p * 128) + lane) : 0;
-                    sc[u] = in ? __ldg(reinterpret_cast<const uint16_t*>(a.scales + p * 16) + g) : 0;
+        for (int j = 0; j < NT; j++) {
+            const size_t c = (size_t)min(n0 + j * 8 + g, a.N - 1);
+            b0[j] = static_cast<const uint8_t*>(a.B) + (BT == kFp4Rhs ? c * (quads * 32) + 2 * t : (c * a.K + 4 * t) * 2);
+        }
+        auto load = [&](Four& x) {
+            x.w = __ldg(reinterpret_cast<const uint4*>(at) + lane);
+            x.s = __ldg(reinterpret_cast<const uint2*>(at + 512) + g);
+            x.col = __ldg(reinterpret_cast<const int4*>(at + 576));
+            at += kFp4FourBytes;
+        };
+        auto panel = [&](const Four& x, Panel<BT, NT, U>& y, int u0) {
 #pragma unroll
-                    for (int j = 0; j < NT; j++) {
-                        const int c = n0 + j * 8 + g;
-                        const bool ok = in && c < a.N;
-                        if constexpr (BT == kFp4Rhs) {
-                            b[u][j][0] = ok ? __ldg(reinterpret_cast<const uint16_t*>(static_cast<const uint8_t*>(a.B) + c * (quads * 32) + (col + kbase) / 2)) : 0;
+            for (int u = 0; u < U; u++) {
+                const int k = u0 + u, col = k == 0 ? x.col.x : k == 1 ? x.col.y : k == 2 ? x.col.z : x.col.w;
 #pragma unroll
-                            for (int e = 0; e < 2; e++) {
-                                const int cc = n0 + j * 8 + 2 * t + e;
-                                bs[u][j][e] = in && cc < a.N ? __ldg(a.b_scales + dense_scale_at<FMT>(cc, col, quads)) : 0;
-                            }
-                        } else {
-                            const uint2 v = ok ? __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.B) + (size_t)c * a.K + col + kbase)) : make_uint2(0, 0);
-                            b[u][j][0] = v.x;
-                            b[u][j][1] = v.y;
-                        }
+                for (int j = 0; j < NT; j++) {
+                    if constexpr (BT == kFp4Rhs) {
+                        y.b[u][j].x = __ldg(reinterpret_cast<const uint16_t*>(b0[j] + col / 2));
+#pragma unroll
+                        for (int e = 0; e < 2; e++)
+                            y.q[u][j][e] = __ldg(a.b_scales + dense_scale_at<FMT>((size_t)min(n0 + j * 8 + 2 * t + e, a.N - 1), col, quads));
+                    } else {
+                        y.b[u][j] = __ldg(reinterpret_cast<const uint2*>(b0[j] + (size_t)col * 2));
                     }
                 }
+            }
+        };
+        // `left`: blocks of this four that exist; what stands in the places of the others is zeros, but B may hold anything there.
+        auto multiply = [&](const Four& x, Panel<BT, NT, U>& y, int u0, int left) {
 #pragma unroll
-                for (int u = 0; u < U; u++) {
-                    if (u0 + u >= cnt) break;
-                    const uint32_t got = __shfl_xor_sync(~0u, t < 2 ? w[u] >> 16 : w[u] & 0xffffu, 2);
-                    const uint32_t both = t < 2 ? (w[u] & 0xffffu) | got << 16 : got | (w[u] & 0xffff0000u);
-                    uint32_t h[4];
-                    e2m1x8_to_f16(both, h);
-                    uint32_t am[4] = {h[0], h[2], h[1], h[3]};
+            for (int u = 0; u < U; u++) {
+                const int k = u0 + u;
+                const uint32_t w = k == 0 ? x.w.x : k == 1 ? x.w.y : k == 2 ? x.w.z : x.w.w, sc = (k < 2 ? x.s.x : x.s.y) >> (k % 2 * 16) & 0xffff;
+                uint32_t h[4];
+                e2m1x8_to_f16(w, h);
+                uint32_t am[4] = {h[0], h[2], h[1], h[3]};
+                float s0 = 1.f, s1 = 1.f;
+                if constexpr (FOLD) {
+                    // the pair of scales of rows 2g and 2g + 1, each in both halves of a word
+                    uint32_t s2;
+                    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(s2) : "h"((uint16_t)sc));
+                    if constexpr (BT == SMAT_F16) {
+                        const uint32_t lo2 = __byte_perm(s2, s2, 0x1010), hi2 = __byte_perm(s2, s2, 0x3232);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&am[e]), *reinterpret_cast<const __half2*>(e % 2 ? &hi2 : &lo2));
+                            am[e] = *reinterpret_cast<const uint32_t*>(&v);
+                        }
+                    } else {
+                        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&s2));
+#pragma unroll
+                        for (int e = 0; e < 4; e++) am[e] = f16_code_to_bf16(am[e], e % 2 ? f.y : f.x);
+                    }
+                } else {
                     if constexpr (BT == SMAT_BF16) {
 #pragma unroll
-                        for (int e = 0; e < 4; e++) am[e] = f16_code_to_bf16(am[e]);
+                        for (int e = 0; e < 4; e++) am[e] = f16_code_to_bf16(am[e], 1.f);
                     }
-                    const float s0 = scale_value<FMT>(sc[u] & 0xff), s1 = scale_value<FMT>(sc[u] >> 8);
+                    s0 = scale_value<FMT>(sc & 0xff);
+                    s1 = scale_value<FMT>(sc >> 8);
+                }
 #pragma unroll
-                    for (int j = 0; j < NT; j++) {
+                for (int j = 0; j < NT; j++) {
+                    uint32_t bx = k < left ? y.b[u][j].x : 0, by = k < left ? y.b[u][j].y : 0;
+                    if constexpr (BT == kFp4Rhs) e2m1x4_to_f16((uint16_t)bx, bx, by);
+                    if constexpr (FOLD) {
+                        mma_16816<BT == SMAT_BF16>(acc[j], am, bx, by, acc[j]);
+                    } else {
+                        const float zero[4] = {0.f, 0.f, 0.f, 0.f};
                         float d[4];
+                        mma_16816<BT == SMAT_BF16>(d, am, bx, by, zero);
                         if constexpr (BT == kFp4Rhs) {
-                            uint32_t b0, b1;
-                            e2m1x4_to_f16((uint16_t)b[u][j][0], b0, b1);
-                            mma_16816<false>(d, am, b0, b1);
-                            const float q0 = scale_value<FMT>(bs[u][j][0]), q1 = scale_value<FMT>(bs[u][j][1]);
+                            const float q0 = k < left ? scale_value<FMT>(y.q[u][j][0]) : 0.f, q1 = k < left ? scale_value<FMT>(y.q[u][j][1]) : 0.f;
                             d[0] *= q0; d[1] *= q1; d[2] *= q0; d[3] *= q1;
-                        } else {
-                            mma_16816<BT == SMAT_BF16>(d, am, b[u][j][0], b[u][j][1]);
                         }
                         acc[j][0] = fmaf(s0, d[0], acc[j][0]);
                         acc[j][1] = fmaf(s0, d[1], acc[j][1]);
@@ -130,6 +169,33 @@ __global__ void __launch_bounds__(kWarps * 32) fp4_stream_kernel(const StreamArg
                     }
                 }
             }
+        };
+        if (hi > lo) {
+            // Codes a four ahead (two where the registers hold it), rows of B, which need the columns, a panel ahead.
+            constexpr bool DEEP = NT <= 4;
+            Four x, y, z;
+            load(x);
+            if (lo + 1 < hi) load(y); else y = x;
+            Panel<BT, NT, U> p[2];
+            panel(x, p[0], 0);
+            auto four = [&](int i, int left) {
+                if (DEEP) {
+                    if (i + 2 < hi) load(z); else z = y;
+                }
+#pragma unroll
+                for (int u0 = 0; u0 < 4; u0 += U) {
+                    const int cur = u0 / U % 2;
+                    if (u0 + U < 4) panel(x, p[cur ^ 1], u0 + U);
+                    else panel(y, p[cur ^ 1], 0);
+                    multiply(x, p[cur], u0, left);
+                }
+                if (4 / U % 2) p[0] = p[1];
+                x = y;
+                if (DEEP) y = z;
+                else if (i + 2 < hi) load(y);
+            };
+            for (int i = lo; i < hi - 1; i++) four(i, 4);
+            four(hi - 1, min(4, row.blocks - 4 * (hi - 1)));
         }
     }
 
@@ -188,12 +254,20 @@ cudaError_t launch(const StreamArgs& a, int wr, int cl, cudaStream_t stream) {
     return cudaLaunchKernelEx(&cfg, fp4_stream_kernel<BT, FMT, NT, U>, a, wr);
 }
 
+// Columns in tiles of equal width, 64 at most; as many blocks in a batch as the registers hold.
 template <int BT, int FMT>
 cudaError_t launch_width(const StreamArgs& a, int wr, int cl, cudaStream_t stream) {
-    if (a.N <= 8) return launch<BT, FMT, 1, 8>(a, wr, cl, stream);
-    if (a.N <= 16) return launch<BT, FMT, 2, 4>(a, wr, cl, stream);
-    if (a.N <= 32) return launch<BT, FMT, 4, 2>(a, wr, cl, stream);
-    return launch<BT, FMT, 8, 2>(a, wr, cl, stream);
+    const int tiles = (a.N + 63) / 64, width = (a.N + tiles - 1) / tiles;
+    switch ((width + 7) / 8) {
+        case 1: return launch<BT, FMT, 1, 4>(a, wr, cl, stream);
+        case 2: return launch<BT, FMT, 2, 4>(a, wr, cl, stream);
+        case 3: return launch<BT, FMT, 3, 2>(a, wr, cl, stream);
+        case 4: return launch<BT, FMT, 4, 2>(a, wr, cl, stream);
+        case 5: return launch<BT, FMT, 5, 1>(a, wr, cl, stream);
+        case 6: return launch<BT, FMT, 6, 1>(a, wr, cl, stream);
+        case 7: return launch<BT, FMT, 7, 1>(a, wr, cl, stream);
+        default: return launch<BT, FMT, 8, 1>(a, wr, cl, stream);
+    }
 }
 template <int BT>
 cudaError_t launch_format(int fmt, const StreamArgs& a, int wr, int cl, cudaStream_t stream) {
@@ -206,11 +280,9 @@ int launch_fp4_stream(const Fp4View& A, const Fp4Rhs& B, void* C, int c_dtype, s
     DeviceCtx* ctx = nullptr;
     if (int rc = get_device_ctx(&ctx)) return rc;
     StreamArgs a = {};
-    a.codes = A.codes;
-    a.scales = A.scales;
+    a.fours = A.fours;
+    a.rows = A.rows;
     a.row_scale = A.row_scale ? A.row_scale + A.brow_begin * 16 : nullptr;
-    a.colidx = A.colidx;
-    a.range = A.range;
     a.B = B.data;
     a.b_scales = B.scales;
     a.b_row_scale = B.row_scale;
