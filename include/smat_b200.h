@@ -174,7 +174,7 @@ int smat_selftest_plan_wait_timeout(const smat_plan* plan, const void* B, void* 
  * and a block matrix, beside rowptr and colidx as above,
  *   codes   128 bytes a block (16 rows of 8), scales 16 bytes a block (one for each row), row_scale float[M].
  *   Of SMAT_FP4_MX, the blocks of an aligned pair of block-columns (columns 32 c to 32 c + 31) have equal scales.
- * All arrays 16-byte aligned in device memory; K a multiple of 16. */
+ * All arrays 16-byte aligned in device memory; K a multiple of 16 below 2^30, N below 2^31. */
 enum { SMAT_FP4_NV = 0, SMAT_FP4_MX = 1 };
 /* Element types of values. */
 enum { SMAT_F16 = 0, SMAT_BF16 = 1, SMAT_F32 = 2 };

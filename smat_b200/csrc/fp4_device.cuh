@@ -44,14 +44,21 @@ __device__ __forceinline__ void e2m1x4_to_f16(uint16_t w, uint32_t& h0, uint32_t
     asm("{\n\t.reg .b8 b0, b1;\n\tmov.b16 {b0, b1}, %2;\n\tcvt.rn.f16x2.e2m1x2 %0, b0;\n\tcvt.rn.f16x2.e2m1x2 %1, b1;\n\t}"
         : "=r"(h0), "=r"(h1) : "h"(w));
 }
-// A pair of fp16 that came from e2m1 -> the same pair times `scale` in bf16, exact where the product fits bf16.  The magnitude shifted
-// down by the three bits that the exponent field is wider reads as the value times 2^-112 (0 stays 0, all others are normal); the
-// factor takes that back.  scale * 2^112 has to be finite in bf16.
-__device__ __forceinline__ uint32_t f16_code_to_bf16(uint32_t h2, float scale) {
-    const uint32_t small = (h2 & 0x80008000u) | ((h2 & 0x7fff7fffu) >> 3);
-    const float up = scale * 5192296858534827628530496329220096.f;  // 2^112
-    const __nv_bfloat162 v = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&small), __floats2bfloat162_rn(up, up));
-    return *reinterpret_cast<const uint32_t*>(&v);
+// Product of two pairs.
+template <int DT>
+__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
+    if constexpr (DT == SMAT_F16) {
+        const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+        return *reinterpret_cast<const uint32_t*>(&v);
+    } else {
+        const __nv_bfloat162 v = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+        return *reinterpret_cast<const uint32_t*>(&v);
+    }
+}
+// A pair of fp16 that came from e2m1 -> the same pair in bf16.  The magnitude shifted down by the three bits that the exponent field is
+// wider reads as the value times 2^-112 (0 stays 0, all others are normal); the factor 2^112 (0x7780) takes that back.
+__device__ __forceinline__ uint32_t f16_code_to_bf16(uint32_t h2) {
+    return mul2<SMAT_BF16>((h2 & 0x80008000u) | ((h2 & 0x7fff7fffu) >> 3), 0x77807780u);
 }
 // Eight fp32 -> eight codes, to nearest, ties to even, saturating at 6 (no NaN comes here).
 __device__ __forceinline__ uint32_t f32x8_to_e2m1(const float* v) {
@@ -70,32 +77,58 @@ template <> struct Elem<SMAT_F16> { using T = __half; };
 template <> struct Elem<SMAT_BF16> { using T = __nv_bfloat16; };
 template <> struct Elem<SMAT_F32> { using T = float; };
 
-// 16 consecutive values (16-byte aligned) in fp32.
+// 16 consecutive values (16-byte aligned) as they lie in memory.
 template <int DT>
-__device__ __forceinline__ void load16(const typename Elem<DT>::T* p, float (&v)[16]) {
-    if constexpr (DT == SMAT_F32) {
+struct Raw {
+    uint4 v[DT == SMAT_F32 ? 4 : 2];
+    __device__ __forceinline__ void load(const typename Elem<DT>::T* p) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float4 q = __ldg(reinterpret_cast<const float4*>(p) + i);
-            v[4 * i] = q.x; v[4 * i + 1] = q.y; v[4 * i + 2] = q.z; v[4 * i + 3] = q.w;
-        }
-    } else {
+        for (int i = 0; i < (DT == SMAT_F32 ? 4 : 2); i++) v[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    }
+    __device__ __forceinline__ void zero() {
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const uint4 q = __ldg(reinterpret_cast<const uint4*>(p) + i);
-            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+        for (int i = 0; i < (DT == SMAT_F32 ? 4 : 2); i++) v[i] = make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ void unpack(float (&f)[16]) const {
+#pragma unroll
+        for (int i = 0; i < (DT == SMAT_F32 ? 4 : 2); i++) {
+            const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                if constexpr (DT == SMAT_F16) {
-                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
-                    v[8 * i + 2 * j] = f.x; v[8 * i + 2 * j + 1] = f.y;
+                if constexpr (DT == SMAT_F32) {
+                    f[4 * i + j] = __uint_as_float(w[j]);
+                } else if constexpr (DT == SMAT_F16) {
+                    const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+                    f[8 * i + 2 * j] = t.x; f[8 * i + 2 * j + 1] = t.y;
                 } else {
-                    v[8 * i + 2 * j] = __uint_as_float(w[j] << 16); v[8 * i + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+                    f[8 * i + 2 * j] = __uint_as_float(w[j] << 16); f[8 * i + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
                 }
             }
         }
     }
-}
+    // Largest magnitude among the finite values; bad: there are others.  Magnitudes compare like their bits.
+    __device__ __forceinline__ float amax(bool& bad) const {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < (DT == SMAT_F32 ? 4 : 2); i++) {
+            const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+            for (int j = 0; j < 4; j++) m = DT == SMAT_F32 ? max(m, w[j] & 0x7fffffffu) : __vmaxu2(m, w[j] & 0x7fff7fffu);
+        }
+        if (DT != SMAT_F32) m = max(m & 0xffffu, m >> 16);
+        bad = m >= (DT == SMAT_F32 ? 0x7f800000u : DT == SMAT_F16 ? 0x7c00u : 0x7f80u);
+        if (bad) {
+            float f[16], a = 0.f;
+            unpack(f);
+#pragma unroll
+            for (int i = 0; i < 16; i++) a = fmaxf(a, (__float_as_uint(f[i]) & 0x7f800000u) != 0x7f800000u ? fabsf(f[i]) : 0.f);
+            return a;
+        }
+        if constexpr (DT == SMAT_F32) return __uint_as_float(m);
+        else if constexpr (DT == SMAT_F16) return __half2float(__ushort_as_half((unsigned short)m));
+        else return __uint_as_float(m << 16);
+    }
+};
 template <int DT>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
     if constexpr (DT == SMAT_F16) {

@@ -7,16 +7,18 @@
 // The codes are those of exact arithmetic: quotients that an fp32 division would round onto a tie are moved off it again.
 // A group that holds a NaN or an infinity gets the scale NaN and codes 0; row maxima are taken over finite values.
 //
-// What bounds it: HBM.  The row maximum is taken by the CTA that quantises the row right after it: the second reading comes out of
-// L2 (or L1), so a value crosses HBM once and no launch waits for another.
+// What bounds it: HBM, and eight instructions a value.  A row of a dense matrix stays in the registers of its CTA between the maximum
+// and the codes (up to 128 values a thread; longer ones are read again, from L2); so do not the blocks of a block-row, whose second
+// reading comes out of L2.  Loads are issued several groups at a time.
+#include <algorithm>
+#include <type_traits>
+
 #include "fp4_device.cuh"
 
 namespace smat {
 namespace {
 
 constexpr int kThreads = 256;
-
-__device__ __forceinline__ bool finite_bits(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
 // Least power of two p >= amax / 2688 with exponent >= -100; 1 for 0.  amax = f * 2^e with f in [1, 2); 2688 = 1.3125 * 2^11.
 __device__ __forceinline__ float pow2_of_row(float amax) {
@@ -42,125 +44,149 @@ __device__ __forceinline__ float divide_for_rounding(float x, float d, float y) 
     return q;
 }
 
-// Scale byte of a group with largest magnitude gmax (bad: it holds a NaN or an infinity), and what its values are divided by.
-// The quotients are formed from values times `up`, a power of two that keeps them and the divisor inside the normal numbers.
+// Scale byte of a group with largest magnitude gmax (bad: it holds a NaN or an infinity); values are divided by d, whose correctly
+// rounded reciprocal is y.  p: the row's power of two.
 template <int FMT>
-__device__ __forceinline__ uint32_t group_scale(float gmax, bool bad, float inv_p, float& d, float& up) {
+__device__ __forceinline__ uint32_t group_scale(float gmax, bool bad, float p, float inv_p, float& d, float& y) {
     if constexpr (FMT == SMAT_FP4_NV) {
-        up = inv_p;
         const float g = divide_for_rounding<false>(gmax * inv_p, 6.f, 1.f / 6.f);
         uint16_t c;
         asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(c) : "f"(0.f), "f"(g));
-        d = scale_e4m3(c & 0x7fu);
+        const float s = scale_e4m3(c & 0x7fu);
+        d = s * p;  // exact: four bits, and powers of two that stay inside the normal numbers (2^-9 2^-100 to 2^9 2^117)
+        y = __frcp_rn(s) * inv_p;
         return bad ? 0x7fu : c & 0x7fu;
     } else {
         const int e = max((int)(__float_as_uint(gmax) >> 23) - 127 - 2, -127);  // of a subnormal gmax: the bound
-        up = __uint_as_float((uint32_t)min(127 - e, 254) << 23);  // 2^-e; e <= 125
         d = 1.f;
+        y = __uint_as_float((uint32_t)(127 - e) << 23);  // 2^-e; e is -127 to 125
         return bad ? 0xffu : (uint32_t)(e + 127);
     }
 }
 
 // 16 values with the largest magnitude of their group -> 8 bytes of codes and the scale byte.
 template <int FMT, int DT>
-__device__ __forceinline__ uint2 quantize16(const float (&v)[16], float gmax, bool bad, float inv_p, uint32_t& scale) {
-    float d, up;
-    scale = group_scale<FMT>(gmax, bad, inv_p, d, up);
+__device__ __forceinline__ uint2 quantize16(const Raw<DT>& raw, float gmax, bool bad, float p, float inv_p, uint32_t& scale) {
+    float d, y, q[16];
+    scale = group_scale<FMT>(gmax, bad, p, inv_p, d, y);
     if (bad || d == 0.f) return make_uint2(0, 0);
-    float q[16];
-    if constexpr (FMT == SMAT_FP4_NV) {
-        const float y = __frcp_rn(d);
+    raw.unpack(q);
 #pragma unroll
-        for (int i = 0; i < 16; i++) q[i] = divide_for_rounding<DT != SMAT_F32>(v[i] * up, d, y);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; i++) q[i] = v[i] * up;
-    }
+    for (int i = 0; i < 16; i++) q[i] = FMT == SMAT_FP4_NV ? divide_for_rounding<DT != SMAT_F32>(q[i], d, y) : q[i] * y;
     return make_uint2(f32x8_to_e2m1(q), f32x8_to_e2m1(q + 8));
 }
-
-// Largest magnitude among the finite values; bad: there are others.
-__device__ __forceinline__ float amax16(const float (&v)[16], bool& bad) {
-    float m = 0.f;
-    bad = false;
+template <int DT>
+__device__ __forceinline__ void dequantize16(uint2 c, float s, typename Elem<DT>::T* to) {
+    uint32_t h[2][4];
+    e2m1x8_to_f16(c.x, h[0]);
+    e2m1x8_to_f16(c.y, h[1]);
+    float v[16];
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
-        const bool f = finite_bits(v[i]);
-        bad |= !f;
-        m = fmaxf(m, f ? fabsf(v[i]) : 0.f);
+    for (int i = 0; i < 8; i++) {
+        const float2 f = __half22float2(*reinterpret_cast<__half2*>(&h[i / 4][i % 4]));
+        v[2 * i] = f.x * s; v[2 * i + 1] = f.y * s;
     }
-    return m;
+    store16<DT>(to, v);
 }
 
 // ---- dense ----------------------------------------------------------------------------------------------------------------------
+// Codes and scale of group j of row r; lanes j & 3 of a warp hold the groups of 64 columns and write their scales together.
 template <int FMT, int DT>
-__global__ void __launch_bounds__(kThreads) fp4_quantize_kernel(const typename Elem<DT>::T* __restrict__ X, size_t N, size_t K, size_t ldx,
+__device__ __forceinline__ void quantize_group(const Raw<DT>& raw, size_t r, int j, bool in, int quads, float p, float inv_p, uint8_t* codes, uint8_t* scales) {
+    bool bad;
+    float g = raw.amax(bad);
+    if constexpr (FMT == SMAT_FP4_MX) {
+        g = fmaxf(g, __shfl_xor_sync(~0u, g, 1));
+        bad = __shfl_xor_sync(~0u, bad ? 1 : 0, 1) || bad;
+    }
+    uint32_t s;
+    const uint2 c = quantize16<FMT, DT>(raw, g, bad, p, inv_p, s);
+    if (!in) s = 0;
+    uint32_t word = FMT == SMAT_FP4_NV ? s << (j & 3) * 8 : j & 1 ? 0 : s << (j & 3) * 4;
+    word |= __shfl_xor_sync(~0u, word, 1);
+    word |= __shfl_xor_sync(~0u, word, 2);
+    if (j >= quads * 4) return;
+    *reinterpret_cast<uint2*>(codes + r * quads * 32 + (size_t)j * 8) = c;
+    if ((j & 3) == 0) *reinterpret_cast<uint32_t*>(scales + dense_scale_at<SMAT_FP4_NV>(r, (size_t)j * 16, quads)) = word;
+}
+
+// A CTA a row; G groups of 16 a thread in registers, or 0: the row is read twice.
+template <int FMT, int DT, int G>
+__global__ void __launch_bounds__(kThreads) fp4_quantize_kernel(const typename Elem<DT>::T* __restrict__ X, int K, size_t ldx,
                                                                 uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
                                                                 float* __restrict__ row_scale) {
-    const size_t r = blockIdx.x, quads = (K + 63) / 64;
+    const size_t r = blockIdx.x;
+    const int quads = (K + 63) / 64, threads = blockDim.x;
     const auto* x = X + r * ldx;
-    float v[16];
-    bool bad;
-    __shared__ float s_max[kThreads / 32];
-    float inv_p = 1.f;
+    Raw<DT> raw[G ? G : 1];
+    float p = 1.f, inv_p = 1.f;
+    if constexpr (G > 0) {
+#pragma unroll
+        for (int i = 0; i < G; i++) {
+            const int j = (int)threadIdx.x + i * threads;
+            if (j * 16 < K) raw[i].load(x + (size_t)j * 16);
+            else raw[i].zero();
+        }
+    }
     if constexpr (FMT == SMAT_FP4_NV) {
+        __shared__ float s_max[kThreads / 32];
         float m = 0.f;
-        for (size_t j = threadIdx.x; j * 16 < K; j += kThreads) {
-            load16<DT>(x + j * 16, v);
-            m = fmaxf(m, amax16(v, bad));
+        bool bad;
+        if constexpr (G > 0) {
+#pragma unroll
+            for (int i = 0; i < G; i++) m = fmaxf(m, raw[i].amax(bad));
+        } else {
+            for (int j = threadIdx.x; j * 16 < K; j += threads) {
+                raw[0].load(x + (size_t)j * 16);
+                m = fmaxf(m, raw[0].amax(bad));
+            }
         }
         for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
         if (threadIdx.x % 32 == 0) s_max[threadIdx.x / 32] = m;
         __syncthreads();
         m = s_max[0];
-        for (int w = 1; w < kThreads / 32; w++) m = fmaxf(m, s_max[w]);
-        const float p = pow2_of_row(m);
+        for (int w = 1; w < threads / 32; w++) m = fmaxf(m, s_max[w]);
+        p = pow2_of_row(m);
         inv_p = 1.f / p;
         if (threadIdx.x == 0) row_scale[r] = p;
     }
-    const size_t groups = quads * 4, up = (groups + kThreads - 1) / kThreads * kThreads;  // whole warps: lanes exchange below
-    for (size_t j = threadIdx.x; j < up; j += kThreads) {
-        const bool in = j * 16 < K;
-        if (in) {
-            load16<DT>(x + j * 16, v);
-        } else {
+    if constexpr (G > 0) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) v[i] = 0.f;
+        for (int i = 0; i < G; i++) {
+            const int j = (int)threadIdx.x + i * threads;
+            quantize_group<FMT, DT>(raw[i], r, j, j * 16 < K, quads, p, inv_p, codes, scales);
         }
-        float g = amax16(v, bad);
-        if constexpr (FMT == SMAT_FP4_MX) {
-            g = fmaxf(g, __shfl_xor_sync(~0u, g, 1));
-            bad = __shfl_xor_sync(~0u, bad ? 1 : 0, 1) || bad;
+    } else {
+        for (int j = threadIdx.x; j - (int)threadIdx.x < quads * 4; j += threads) {  // whole warps: lanes exchange
+            if (j * 16 < K) raw[0].load(x + (size_t)j * 16);
+            else raw[0].zero();
+            quantize_group<FMT, DT>(raw[0], r, j, j * 16 < K, quads, p, inv_p, codes, scales);
         }
-        if (j >= groups) continue;
-        uint32_t s;
-        const uint2 c = quantize16<FMT, DT>(v, g, bad, inv_p, s);
-        *reinterpret_cast<uint2*>(codes + r * quads * 32 + j * 8) = c;
-        const size_t at = dense_scale_at<SMAT_FP4_NV>(r, j * 16, quads);
-        if constexpr (FMT == SMAT_FP4_NV) scales[at] = in ? s : 0;
-        else scales[at - (j & 3) + ((j & 1) ? 2 : 0) + ((j & 3) >> 1)] = (j & 1) || !in ? 0 : s;
     }
 }
 
 template <int FMT, int DT>
 __global__ void __launch_bounds__(kThreads) fp4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
-                                                                  const float* __restrict__ row_scale, size_t K,
+                                                                  const float* __restrict__ row_scale, int K,
                                                                   typename Elem<DT>::T* __restrict__ Y, size_t ldy) {
-    const size_t r = blockIdx.x, quads = (K + 63) / 64;
+    constexpr int U = 4;
+    const size_t r = blockIdx.x;
+    const int quads = (K + 63) / 64, groups = K / 16, threads = blockDim.x;
     const float p = row_scale ? __ldg(row_scale + r) : 1.f;
-    for (size_t j = threadIdx.x; j * 16 < K; j += kThreads) {
-        const uint2 c = __ldg(reinterpret_cast<const uint2*>(codes + r * quads * 32) + j);
-        const float s = scale_value<FMT>(__ldg(scales + dense_scale_at<FMT>(r, j * 16, quads))) * p;
-        uint32_t h[2][4];
-        e2m1x8_to_f16(c.x, h[0]);
-        e2m1x8_to_f16(c.y, h[1]);
-        float v[16];
+    for (int j0 = threadIdx.x; j0 < groups; j0 += U * threads) {
+        uint2 c[U];
+        uint32_t s[U];
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float2 f = __half22float2(*reinterpret_cast<__half2*>(&h[i / 4][i % 4]));
-            v[2 * i] = f.x * s; v[2 * i + 1] = f.y * s;
+        for (int u = 0; u < U; u++) {
+            const int j = min(j0 + u * threads, groups - 1);
+            c[u] = __ldg(reinterpret_cast<const uint2*>(codes + r * quads * 32) + j);
+            s[u] = __ldg(scales + dense_scale_at<FMT>(r, (size_t)j * 16, quads));
         }
-        store16<DT>(Y + r * ldy + j * 16, v);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int j = j0 + u * threads;
+            if (j < groups) dequantize16<DT>(c[u], scale_value<FMT>(s[u]) * p, Y + r * ldy + (size_t)j * 16);
+        }
     }
 }
 
@@ -182,45 +208,57 @@ __global__ void __launch_bounds__(kThreads) fp4_quantize_blocks_kernel(const typ
                                                                        size_t nnzb, uint8_t* __restrict__ codes,
                                                                        uint8_t* __restrict__ scales, float* __restrict__ row_scale,
                                                                        int* status) {
+    constexpr int U = DT == SMAT_F32 ? 2 : 4, STEP = kThreads / 16;  // blocks a thread has on their way, blocks of the CTA at a time
     const int2 range = blocks_of_row(rowptr, blockIdx.x, nnzb, status);
     const int i = threadIdx.x % 16;
-    float v[16];
+    Raw<DT> raw[U];
     bool bad;
-    float inv_p = 1.f;
+    float p = 1.f, inv_p = 1.f;
     if constexpr (FMT == SMAT_FP4_NV) {
         __shared__ unsigned s_max[16];  // magnitudes of floats compare like their bits
         if (threadIdx.x < 16) s_max[threadIdx.x] = 0;
         __syncthreads();
         float m = 0.f;
-        for (int b = range.x + threadIdx.x / 16; b < range.y; b += kThreads / 16) {
-            load16<DT>(vals + (size_t)b * 256 + i * 16, v);
-            m = fmaxf(m, amax16(v, bad));
+        for (int b0 = range.x + threadIdx.x / 16; b0 < range.y; b0 += U * STEP) {
+#pragma unroll
+            for (int u = 0; u < U; u++) raw[u].load(vals + (size_t)min(b0 + u * STEP, range.y - 1) * 256 + i * 16);
+#pragma unroll
+            for (int u = 0; u < U; u++) m = fmaxf(m, raw[u].amax(bad));
         }
         m = fmaxf(m, __shfl_xor_sync(~0u, m, 16));
         if (threadIdx.x % 32 < 16) atomicMax(&s_max[i], __float_as_uint(m));
         __syncthreads();
-        const float p = pow2_of_row(__uint_as_float(s_max[i]));
+        p = pow2_of_row(__uint_as_float(s_max[i]));
         inv_p = 1.f / p;
         if (threadIdx.x < 16) row_scale[(size_t)blockIdx.x * 16 + i] = p;
     }
-    for (int b = range.x + threadIdx.x / 16; b < range.y; b += kThreads / 16) {
-        load16<DT>(vals + (size_t)b * 256 + i * 16, v);
-        float g = amax16(v, bad);
-        if constexpr (FMT == SMAT_FP4_MX) {
-            const int col = __ldg(colidx + b);
-            const int other = col & 16 ? b - 1 : b + 1;  // where the other block of the pair would be
-            if (other >= range.x && other < range.y && __ldg(colidx + other) == (col ^ 16)) {
-                float w[16];
-                bool bad2;
-                load16<DT>(vals + (size_t)other * 256 + i * 16, w);
-                g = fmaxf(g, amax16(w, bad2));
-                bad |= bad2;
+    for (int b0 = range.x + threadIdx.x / 16; b0 < range.y; b0 += U * STEP) {
+        Raw<DT> pair[FMT == SMAT_FP4_MX ? U : 1];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int b = min(b0 + u * STEP, range.y - 1);
+            raw[u].load(vals + (size_t)b * 256 + i * 16);
+            if constexpr (FMT == SMAT_FP4_MX) {
+                const int col = __ldg(colidx + b), other = col & 16 ? b - 1 : b + 1;  // where the other block of the pair would be
+                if (other >= range.x && other < range.y && __ldg(colidx + other) == (col ^ 16)) pair[u].load(vals + (size_t)other * 256 + i * 16);
+                else pair[u].zero();
             }
         }
-        uint32_t s;
-        const uint2 c = quantize16<FMT, DT>(v, g, bad, inv_p, s);
-        *reinterpret_cast<uint2*>(codes + (size_t)b * 128 + i * 8) = c;
-        scales[(size_t)b * 16 + i] = s;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int b = b0 + u * STEP;
+            if (b >= range.y) break;
+            float g = raw[u].amax(bad);
+            if constexpr (FMT == SMAT_FP4_MX) {
+                bool bad2;
+                g = fmaxf(g, pair[u].amax(bad2));
+                bad |= bad2;
+            }
+            uint32_t s;
+            const uint2 c = quantize16<FMT, DT>(raw[u], g, bad, p, inv_p, s);
+            *reinterpret_cast<uint2*>(codes + (size_t)b * 128 + i * 8) = c;
+            scales[(size_t)b * 16 + i] = s;
+        }
     }
 }
 
@@ -230,20 +268,22 @@ __global__ void __launch_bounds__(kThreads) fp4_dequantize_blocks_kernel(const u
                                                                          size_t nnzb, typename Elem<DT>::T* __restrict__ vals, int* status) {
     const int2 range = blocks_of_row(rowptr, blockIdx.x, nnzb, status);
     const int i = threadIdx.x % 16;
+    constexpr int U = 4, STEP = kThreads / 16;
     const float p = row_scale ? __ldg(row_scale + (size_t)blockIdx.x * 16 + i) : 1.f;
-    for (int b = range.x + threadIdx.x / 16; b < range.y; b += kThreads / 16) {
-        const uint2 c = __ldg(reinterpret_cast<const uint2*>(codes + (size_t)b * 128) + i);
-        const float s = scale_value<FMT>(__ldg(scales + (size_t)b * 16 + i)) * p;
-        uint32_t h[2][4];
-        e2m1x8_to_f16(c.x, h[0]);
-        e2m1x8_to_f16(c.y, h[1]);
-        float v[16];
+    for (int b0 = range.x + threadIdx.x / 16; b0 < range.y; b0 += U * STEP) {
+        uint2 c[U];
+        uint32_t s[U];
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const float2 f = __half22float2(*reinterpret_cast<__half2*>(&h[j / 4][j % 4]));
-            v[2 * j] = f.x * s; v[2 * j + 1] = f.y * s;
+        for (int u = 0; u < U; u++) {
+            const int b = min(b0 + u * STEP, range.y - 1);
+            c[u] = __ldg(reinterpret_cast<const uint2*>(codes + (size_t)b * 128) + i);
+            s[u] = __ldg(scales + (size_t)b * 16 + i);
         }
-        store16<DT>(vals + (size_t)b * 256 + i * 16, v);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int b = b0 + u * STEP;
+            if (b < range.y) dequantize16<DT>(c[u], scale_value<FMT>(s[u]) * p, vals + (size_t)b * 256 + i * 16);
+        }
     }
 }
 
@@ -268,7 +308,7 @@ size_t size_of(int dtype) { return dtype == SMAT_F32 ? 4 : 2; }
 int check_dense(const void* X, int dtype, size_t N, size_t K, size_t ld, int fmt, const void* codes, const void* scales) {
     if (int rc = check_types(fmt, dtype)) return rc;
     if (K % 16) return fail(SMAT_ERR_BAD_ARG, "K (%zu) must be a multiple of 16", K);
-    if (N >= ((size_t)1 << 31) || K >= ((size_t)1 << 31)) return fail(SMAT_ERR_RANGE, "dimension beyond 2^31");
+    if (N >= ((size_t)1 << 31) || K >= ((size_t)1 << 30)) return fail(SMAT_ERR_RANGE, "N beyond 2^31 - 1 or K beyond 2^30 - 1");
     if (N && K && (!X || !codes || !scales)) return fail(SMAT_ERR_BAD_ARG, "NULL argument");
     if (ld < K || ld * size_of(dtype) % 16) return fail(SMAT_ERR_BAD_ARG, "rows must be at least K elements and a multiple of 16 bytes apart");
     if (((uintptr_t)X | (uintptr_t)codes | (uintptr_t)scales) & 15) return fail(SMAT_ERR_BAD_ARG, "arrays must be 16-byte aligned");
@@ -303,8 +343,16 @@ int smat_fp4_quantize(const void* X, int dtype, size_t N, size_t K, size_t ldx, 
     if (!N || (!K && fmt == SMAT_FP4_MX)) return SMAT_OK;
     SMAT_CUDA_TRY(with_types(fmt, dtype, [&](auto f, auto d) {
         constexpr int F = decltype(f)::value, D = decltype(d)::value;
-        fp4_quantize_kernel<F, D><<<(unsigned)N, kThreads, 0, (cudaStream_t)stream>>>(
-            static_cast<const typename Elem<D>::T*>(X), N, K, ldx, static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), row_scale);
+        const int groups = (int)fp4_quads(K) * 4, threads = std::max(32, std::min(kThreads, (groups + 31) / 32 * 32));
+        const auto* x = static_cast<const typename Elem<D>::T*>(X);
+        auto *c = static_cast<uint8_t*>(codes), *s = static_cast<uint8_t*>(scales);
+        auto launch = [&](auto kernel) { kernel<<<(unsigned)N, threads, 0, (cudaStream_t)stream>>>(x, (int)K, ldx, c, s, row_scale); };
+        const int per = (groups + threads - 1) / threads;
+        if (per <= 1) launch(fp4_quantize_kernel<F, D, 1>);
+        else if (per <= 2) launch(fp4_quantize_kernel<F, D, 2>);
+        else if (per <= 4) launch(fp4_quantize_kernel<F, D, 4>);
+        else if (per <= 8 && D != SMAT_F32) launch(fp4_quantize_kernel<F, D, D == SMAT_F32 ? 4 : 8>);
+        else launch(fp4_quantize_kernel<F, D, 0>);
         return cudaGetLastError();
     }));
     count_launch();
@@ -320,8 +368,9 @@ int smat_fp4_dequantize(const void* codes, const void* scales, const float* row_
     if (!N || !K) return SMAT_OK;
     SMAT_CUDA_TRY(with_types(fmt, dtype, [&](auto f, auto d) {
         constexpr int F = decltype(f)::value, D = decltype(d)::value;
-        fp4_dequantize_kernel<F, D><<<(unsigned)N, kThreads, 0, (cudaStream_t)stream>>>(
-            static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), row_scale, K, static_cast<typename Elem<D>::T*>(Y), ldy);
+        const int threads = std::max(32, std::min(kThreads, ((int)K / 16 + 31) / 32 * 32));
+        fp4_dequantize_kernel<F, D><<<(unsigned)N, threads, 0, (cudaStream_t)stream>>>(
+            static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), row_scale, (int)K, static_cast<typename Elem<D>::T*>(Y), ldy);
         return cudaGetLastError();
     }));
     count_launch();
@@ -339,8 +388,7 @@ int smat_fp4_quantize_blocks(const void* vals, int dtype, const int* rowptr, con
     if (!M) return SMAT_OK;
     SMAT_CUDA_TRY(with_types(fmt, dtype, [&](auto f, auto d) {
         constexpr int F = decltype(f)::value, D = decltype(d)::value;
-        fp4_quantize_blocks_kernel<F, D><<<(unsigned)(M / 16), kThreads, 0, (cudaStream_t)stream>>>(
-            static_cast<const typename Elem<D>::T*>(vals), rowptr, colidx, nnzb, static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales),
+        fp4_quantize_blocks_kernel<F, D><<<(unsigned)(M / 16), kThreads, 0, (cudaStream_t)stream>>>(static_cast<const typename Elem<D>::T*>(vals), rowptr, colidx, nnzb, static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales),
             row_scale, ctx->d_status);
         return cudaGetLastError();
     }));
@@ -357,8 +405,7 @@ int smat_fp4_dequantize_blocks(const void* codes, const void* scales, const floa
     if (!M) return SMAT_OK;
     SMAT_CUDA_TRY(with_types(fmt, dtype, [&](auto f, auto d) {
         constexpr int F = decltype(f)::value, D = decltype(d)::value;
-        fp4_dequantize_blocks_kernel<F, D><<<(unsigned)(M / 16), kThreads, 0, (cudaStream_t)stream>>>(
-            static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), row_scale, rowptr, nnzb,
+        fp4_dequantize_blocks_kernel<F, D><<<(unsigned)(M / 16), kThreads, 0, (cudaStream_t)stream>>>(static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), row_scale, rowptr, nnzb,
             static_cast<typename Elem<D>::T*>(vals), ctx->d_status);
         return cudaGetLastError();
     }));

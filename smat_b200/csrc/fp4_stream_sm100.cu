@@ -1,9 +1,9 @@
 // C = A x B with A in 4-bit blocks and few columns of B: warps walk the blocks of a block-row.
 //
 // Mathematics.  A block is 16 x 16 and a scale covers a whole row of it.  e2m1 times e4m3 has at most six significant bits and fits
-// fp16 and bf16, so with SMAT_FP4_NV the scaled values go into m16n8k16 MMAs that accumulate in fp32, nothing rounded on the way in.
-// Powers of two beyond the range of 16 bits (SMAT_FP4_MX) and scales of B in 4 bits are applied to a block's product instead, one
-// fp32 FMA per element.
+// fp16 and bf16, and e2m1 times 2^e fits bf16, so the scaled values go into m16n8k16 MMAs that accumulate in fp32, nothing rounded on
+// the way in.  Powers of two beyond the range of fp16 (SMAT_FP4_MX and fp16) and scales of B in 4 bits are applied to a block's product
+// instead, one fp32 FMA per element.
 //
 // Layout.  Plans keep the blocks in fours in the order in which a warp's lanes take them (fp4_format.h): read as they are stored, a
 // word a lane and block, they cost twice the instructions.  MMA rows g and g + 8 stand for rows 2g and 2g + 1 of the block, the k
@@ -62,7 +62,7 @@ struct Panel {
 // BT: SMAT_F16, SMAT_BF16 or kFp4Rhs.  NT: 8-column tiles of C per warp.  WR warps of a CTA (times the CTAs of a cluster) share a
 // block-row; a CTA holds kWarps / WR block-rows.
 template <int BT, int FMT, int NT, int U>
-__global__ void __launch_bounds__(kWarps * 32, NT <= 2 ? 3 : 2) fp4_stream_kernel(const StreamArgs a, int wr) {
+__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) fp4_stream_kernel(const StreamArgs a, int wr) {
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
     const int cl = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT <= 2 ? 3 : 2) fp4_stream_kerne
     const int r0 = (int)(blockIdx.x / cl % row_ctas) * rows_per_cta, r = r0 + warp / wr;
     const int n0 = (int)(blockIdx.x / cl / row_ctas) * NT * 8;
     const size_t quads = (a.K + 63) / 64;
-    constexpr bool FOLD = FMT == SMAT_FP4_NV && BT != kFp4Rhs;  // scales go into the values of A
+    constexpr bool FOLD = BT == SMAT_BF16 || (BT == SMAT_F16 && FMT == SMAT_FP4_NV);  // scales go into the values of A
 
     float acc[NT][4];
 #pragma unroll
@@ -127,24 +127,17 @@ __global__ void __launch_bounds__(kWarps * 32, NT <= 2 ? 3 : 2) fp4_stream_kerne
                 if constexpr (FOLD) {
                     // the pair of scales of rows 2g and 2g + 1, each in both halves of a word
                     uint32_t s2;
-                    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(s2) : "h"((uint16_t)sc));
-                    if constexpr (BT == SMAT_F16) {
-                        const uint32_t lo2 = __byte_perm(s2, s2, 0x1010), hi2 = __byte_perm(s2, s2, 0x3232);
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&am[e]), *reinterpret_cast<const __half2*>(e % 2 ? &hi2 : &lo2));
-                            am[e] = *reinterpret_cast<const uint32_t*>(&v);
-                        }
-                    } else {
+                    if constexpr (FMT == SMAT_FP4_NV) asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(s2) : "h"((uint16_t)sc));
+                    else asm("cvt.rn.bf16x2.ue8m0x2 %0, %1;" : "=r"(s2) : "h"((uint16_t)sc));
+                    uint32_t both[2] = {__byte_perm(s2, s2, 0x1010), __byte_perm(s2, s2, 0x3232)};
+                    if constexpr (FMT == SMAT_FP4_NV && BT == SMAT_BF16) {
                         const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&s2));
-#pragma unroll
-                        for (int e = 0; e < 4; e++) am[e] = f16_code_to_bf16(am[e], e % 2 ? f.y : f.x);
+                        both[0] = pack2<SMAT_BF16>(f.x, f.x);
+                        both[1] = pack2<SMAT_BF16>(f.y, f.y);
                     }
+#pragma unroll
+                    for (int e = 0; e < 4; e++) am[e] = BT == SMAT_F16 ? mul2<SMAT_F16>(am[e], both[e % 2]) : mul2<SMAT_BF16>(f16_code_to_bf16(am[e]), both[e % 2]);
                 } else {
-                    if constexpr (BT == SMAT_BF16) {
-#pragma unroll
-                        for (int e = 0; e < 4; e++) am[e] = f16_code_to_bf16(am[e], 1.f);
-                    }
                     s0 = scale_value<FMT>(sc & 0xff);
                     s1 = scale_value<FMT>(sc >> 8);
                 }

@@ -71,7 +71,7 @@ def test_c_refusals_of_quantize():
         return call(a["X"], a["dtype"], a["N"], a["K"], a["ldx"], a["fmt"], a["codes"], a["scales"], a["row"], None)
     for kw, code in [(dict(K=24, ldx=24), BAD), (dict(dtype=3), BAD), (dict(fmt=2), BAD), (dict(fmt=-1), BAD), (dict(X=None), BAD), (dict(codes=None), BAD),
                      (dict(scales=None), BAD), (dict(row=None), BAD), (dict(X=P + 8), BAD), (dict(codes=P + 4), BAD), (dict(scales=P + 1), BAD),
-                     (dict(ldx=48), BAD), (dict(ldx=68), BAD), (dict(dtype=2, ldx=66), BAD), (dict(N=1 << 31), RANGE)]:
+                     (dict(ldx=48), BAD), (dict(ldx=68), BAD), (dict(dtype=2, ldx=66), BAD), (dict(N=1 << 31), RANGE), (dict(K=1 << 30, ldx=1 << 30), RANGE)]:
         assert rc(**kw) == code, kw
     assert L.smat_fp4_dequantize(P, P, None, 0, 4, 64, P, 5, 64, None) == BAD
     assert L.smat_fp4_dequantize(P, P, None, 0, 4, 64, P, 0, 32, None) == BAD

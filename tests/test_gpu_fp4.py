@@ -38,7 +38,7 @@ def _same_values(t, want):
 
 @pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
 @pytest.mark.parametrize("dt", list(DTYPES))
-@pytest.mark.parametrize("N,K", [(1, 16), (1, 32), (5, 48), (33, 64), (129, 80), (3, 1040), (2, 4112), (300, 256), (1, 28672)])
+@pytest.mark.parametrize("N,K", [(1, 16), (1, 32), (5, 48), (33, 64), (129, 80), (3, 1040), (2, 4112), (300, 256), (1, 28672), (2, 8192), (3, 16384), (2, 36880), (2, 65536)])
 def test_quantize(fmt, dt, N, K):
     g = torch.Generator("cuda").manual_seed(N + K)
     X = (torch.randn((N, K), generator=g, device="cuda") * torch.exp(torch.randn((N, 1), generator=g, device="cuda"))).to(DTYPES[dt])

@@ -148,6 +148,39 @@ def test_scale_nan_of_a_row_makes_nan(four):
     assert bad[5] and bad.sum() == 1 and not bool(torch.isnan(C[:5]).any())
 
 
+@pytest.mark.parametrize("kind", ["f16", "bf16", "4bit", "4bit, no tiles"])
+def test_scales_from_end_to_end(kind):
+    """mxfp4 scales over the whole of their range: each row of A has its own, activations bring the products back to ordinary size."""
+    rng = np.random.default_rng(12)
+    n = 40  # blocks of each of two block-rows, side by side
+    bytes_of_row = np.array([0, 1, 2, 3, 10, 20, 40, 60, 80, 100, 127, 150, 180, 220, 240, 250])
+    rowptr, colidx = np.array([0, n, 2 * n], np.int32), np.tile(np.arange(n, dtype=np.int32) * 16, 2)
+    codes = rng.integers(0, 16, (2 * n, 16, 16)).astype(np.uint8)
+    scales = np.tile(bytes_of_row.astype(np.uint8), (2 * n, 1))
+    A = S.Fp4SparseMatrix.from_codes(32, n * 16, rowptr, colidx, F.pack(codes), scales, "mxfp4")
+    vals = F.block_values(codes, scales, None, rowptr, "mxfp4")
+    dtype = torch.float16 if kind == "f16" else torch.bfloat16
+    tokens = np.arange(-100, 101, 50) if kind != "f16" else np.arange(-12, 13, 6)  # token t is of size 2^t
+    if kind[0] == "4":
+        bc = rng.integers(0, 16, (len(tokens), n * 16)).astype(np.uint8)
+        bs = np.repeat((tokens + 127).astype(np.uint8)[:, None], n // 2, 1)
+        B = S.Fp4Matrix.from_codes(torch.from_numpy(F.pack(bc)), torch.from_numpy(bs), n * 16, "mxfp4")
+        b = F.dense_values(bc, bs, None, "mxfp4")
+    else:
+        B = torch.from_numpy(rng.standard_normal((len(tokens), n * 16)) * 2.0 ** tokens[:, None]).to(dtype).cuda()
+        b = B.double().cpu().numpy()
+    C = torch.empty((32, len(tokens)), dtype=dtype, device="cuda")
+    S.Fp4Plan(A, tiles=kind != "4bit, no tiles").spmm(B, C, check=True)
+    ref, mag = F.multiply(vals, rowptr, colidx, b)
+    # what fp32 and the type of C hold: neither overflows nor loses digits below the normal numbers
+    top = 2.0 ** 14 if kind == "f16" else 2.0 ** 120
+    fine = (mag < top) & (mag > (2.0 ** -10 if kind == "f16" else 2.0 ** -100))
+    assert fine.sum() >= (6 if kind == "f16" else 60)  # f16: scale 127 with tokens -12, -6, 0, scale 100 with token 12
+    got = C.double().cpu().numpy()
+    tol = (n + 32) * 2.0 ** -22 * mag + HALF[dtype] * np.abs(ref) * (1 + 1e-3) + LEAST[dtype]
+    assert np.all(np.abs(got - ref)[fine] <= tol[fine]), np.max((np.abs(got - ref) / tol)[fine])
+
+
 @pytest.mark.parametrize("four", [False, True])
 def test_values_change(four):
     c = Case(8, [5, 9, 2], 11, "nvfp4")
