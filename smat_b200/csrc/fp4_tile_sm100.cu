@@ -17,6 +17,7 @@
 // 140 in a pair); one thread issues the MMAs; eight warps store finished tiles of C through shared memory, whole 128-byte lines at a
 // time.  Of a pair, the second CTA issues no MMAs.  All waits are bounded.
 #include <algorithm>
+#include <type_traits>
 
 #include "fp4_device.cuh"
 #include "ptx_sm100.cuh"
@@ -419,23 +420,28 @@ fp4_tile_kernel(const __grid_constant__ CUtensorMap mapB, const __grid_constant_
         const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21), out = base + G::OFF_OUT + (uint32_t)(warp - 4) * 4096;
         const uint32_t col = base + G::OFF_COL + (uint32_t)(warp - 4) * 256;
         const int row0 = (warp & 3) * 32, c0 = (warp - 4) / 4 * 64;  // rows and first columns of this warp
-        for (uint32_t n = 0; walk.next(s); n++) {
-            const uint32_t buf = n % G::ACC;
-            const int m0 = s.g * 256 + half_of(s.t) * 128 + row0, n0 = column_of(s.t) * NT, cols = min(NT, a.N - n0);
-            const float rs = a.row_scale && m0 + lane < a.rows ? __ldg(a.row_scale + m0 + lane) : 1.f;
-            float cs[(NT + 127) / 128][2];
+        // What the next unit needs is looked up before this one is stored.
+        Piece f = {};
+        float rs, cs[NT == 256 ? 2 : 1][2];
+        auto look_up = [&]() {
+            const int m = f.g * 256 + half_of(f.t) * 128 + row0 + lane, n = column_of(f.t) * NT + c0 + lane;
+            rs = a.row_scale && m < a.rows ? __ldg(a.row_scale + m) : 1.f;
 #pragma unroll
-            for (int j = 0; j < (NT + 127) / 128; j++)
+            for (int j = 0; j < (NT == 256 ? 2 : 1); j++)
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const int c = n0 + c0 + j * 128 + lane + e * 32;
-                    cs[j][e] = a.b_row_scale && c < a.N ? __ldg(a.b_row_scale + c) : 1.f;
-                }
+                for (int e = 0; e < 2; e++) cs[j][e] = a.b_row_scale && n + j * 128 + e * 32 < a.N ? __ldg(a.b_row_scale + n + j * 128 + e * 32) : 1.f;
             // of a pair, only the one step of an empty group has no MMA
-            bool none = CG == 2 && s.ns == 1 && (__ldg(a.steps + s.gs) & 0xff) == 0;
+            f.k0 = CG == 2 && f.ns == 1 && (__ldg(a.steps + f.gs) & 0xff) == 0;
+        };
+        bool more = walk.next(f);
+        if (more) look_up();
+        for (uint32_t n = 0; more; n++) {
+            const uint32_t buf = n % G::ACC;
+            s = f;
+            const int m0 = s.g * 256 + half_of(s.t) * 128 + row0, n0 = column_of(s.t) * NT, cols = min(NT, a.N - n0);
             if (!__all_sync(~0u, wait_bar(acc_full(buf), (n / G::ACC) & 1, abort_addr, a.status, 69))) break;
             tc_fence_after();
-            if (CG == 1) none = ld_shared_u32(any_addr + 4 * buf) == 0;
+            const bool none = CG == 1 ? ld_shared_u32(any_addr + 4 * buf) == 0 : s.k0 != 0;  // no MMA wrote the accumulators
             auto release = [&]() {  // all of this warp's accumulators are read
                 tc_fence_before();
                 __syncwarp();
@@ -455,36 +461,44 @@ fp4_tile_kernel(const __grid_constant__ CUtensorMap mapB, const __grid_constant_
                         for (int j = 0; j < 16; j++) to[(size_t)(j0 + j) * (128 * CG)] = none ? 0.f : __uint_as_float(u[j]);
                     }
                 release();
+                more = walk.next(f);
+                if (more) look_up();
                 continue;
             }
             // 64 columns at a time: scaled, rounded, through shared memory and out.  Of 256 columns (one accumulator) the second half
             // is taken into registers before the first is stored, so that the next unit's MMAs need not wait for that.
-            auto take = [&](int jc, uint32_t (&w)[NT < 64 ? NT / 2 : 32]) {
-                const int c = c0 + jc * 128;
+            constexpr int W = NT < 64 ? NT : 64;
+            auto take = [&](int jc, auto type, auto&& sink) {  // sink(j, words): columns j to j + 31 of the 64
                 st_shared_u32(col + lane * 4, __float_as_uint(cs[jc][0]));
                 st_shared_u32(col + lane * 4 + 128, __float_as_uint(cs[jc][1]));
                 __syncwarp();
 #pragma unroll
-                for (int j0 = 0; j0 < (NT < 64 ? NT : 64); j0 += 16) {
-                    uint32_t u[16];
-                    tmem_ld_x16(lanes + buf * NT + c + j0, u);
+                for (int j0 = 0; j0 < W; j0 += 32) {
+                    uint32_t u[2][16], w[16];
+                    tmem_ld_x16(lanes + buf * NT + c0 + jc * 128 + j0, u[0]);
+                    tmem_ld_x16(lanes + buf * NT + c0 + jc * 128 + j0 + 16, u[1]);
                     tmem_ld_wait();
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const uint4 f = ld_shared_v4(col + (j0 + 4 * j) * 4);
-                        const float v0 = __uint_as_float(u[4 * j]) * rs * __uint_as_float(f.x), v1 = __uint_as_float(u[4 * j + 1]) * rs * __uint_as_float(f.y);
-                        const float v2 = __uint_as_float(u[4 * j + 2]) * rs * __uint_as_float(f.z), v3 = __uint_as_float(u[4 * j + 3]) * rs * __uint_as_float(f.w);
-                        w[j0 / 2 + 2 * j] = none ? 0 : a.c_dtype == SMAT_F16 ? pack2<SMAT_F16>(v0, v1) : pack2<SMAT_BF16>(v0, v1);
-                        w[j0 / 2 + 2 * j + 1] = none ? 0 : a.c_dtype == SMAT_F16 ? pack2<SMAT_F16>(v2, v3) : pack2<SMAT_BF16>(v2, v3);
+                    for (int j = 0; j < 8; j++) {
+                        const uint32_t* q = u[j / 4] + 4 * (j % 4);
+                        const uint4 by = ld_shared_v4(col + (j0 + 4 * j) * 4);
+                        w[2 * j] = pack2<decltype(type)::value>(__uint_as_float(q[0]) * rs * __uint_as_float(by.x), __uint_as_float(q[1]) * rs * __uint_as_float(by.y));
+                        w[2 * j + 1] = pack2<decltype(type)::value>(__uint_as_float(q[2]) * rs * __uint_as_float(by.z), __uint_as_float(q[3]) * rs * __uint_as_float(by.w));
                     }
+                    if (none) {
+#pragma unroll
+                        for (int j = 0; j < 16; j++) w[j] = 0;
+                    }
+                    sink(j0, w);
                 }
                 __syncwarp();
             };
-            auto store = [&](int jc, const uint32_t (&w)[NT < 64 ? NT / 2 : 32]) {
-                const int c = c0 + jc * 128;
+            auto put = [&](int j0, const uint32_t* w) {
 #pragma unroll
-                for (int j = 0; j < (NT < 64 ? NT / 8 : 8); j++)
-                    st_shared_v4(out + lane * 128 + ((j ^ (lane & 7)) << 4), w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+                for (int j = 0; j < 4; j++) st_shared_v4(out + lane * 128 + (((j0 / 8 + j) ^ (lane & 7)) << 4), w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+            };
+            auto store = [&](int jc) {
+                const int c = c0 + jc * 128;
                 __syncwarp();
                 const int width = min(64, cols - c);
                 uint16_t* const to = static_cast<uint16_t*>(a.C) + (size_t)m0 * a.N + n0 + c;
@@ -501,14 +515,26 @@ fp4_tile_kernel(const __grid_constant__ CUtensorMap mapB, const __grid_constant_
                 }
                 __syncwarp();
             };
-            uint32_t w[(NT + 127) / 128][NT < 64 ? NT / 2 : 32];
+            uint32_t second[NT == 256 ? 32 : 1];
+            auto take_all = [&](auto type) {
+                if (NT == 256 && c0 + 128 < cols)
+                    take(1, type, [&](int j0, const uint32_t* w) {
 #pragma unroll
-            for (int jc = 0; jc < (NT + 127) / 128; jc++)
-                if (c0 + jc * 128 < cols) take(jc, w[jc]);
+                        for (int j = 0; j < 16; j++) second[(j0 / 2 + j) % (NT == 256 ? 32 : 1)] = w[j];
+                    });
+                if (c0 < cols) take(0, type, put);
+            };
+            if (a.c_dtype == SMAT_F16) take_all(std::integral_constant<int, SMAT_F16>());
+            else take_all(std::integral_constant<int, SMAT_BF16>());
             release();
+            more = walk.next(f);
+            if (more) look_up();
+            if (c0 < cols) store(0);
+            if (NT == 256 && c0 + 128 < cols) {
 #pragma unroll
-            for (int jc = 0; jc < (NT + 127) / 128; jc++)
-                if (c0 + jc * 128 < cols) store(jc, w[jc]);
+                for (int j0 = 0; j0 < 64; j0 += 32) put(j0, second + j0 / 2 % (NT == 256 ? 32 : 1));
+                store(1);
+            }
         }
     }
 
@@ -525,30 +551,41 @@ fp4_tile_kernel(const __grid_constant__ CUtensorMap mapB, const __grid_constant_
     }
 }
 
-// Adds up the parts of the units that a start falls into, in the order of the parts.  CTA (c - 1, j): if start c is the first inside
-// a unit, 32 columns of it from 32 j on.
+// Units that a start falls into, and the scratch slots of their parts in order.  Listed on the host: found on the device, from dozens of
+// dependent reads of the schedule, they took the joining kernel 15 of its 19 us.
+struct Joins {
+    Start unit[kMaxParts];
+    short first[kMaxParts + 1], slot[3 * kMaxParts];
+    int n;
+};
+void list_joins(const Schedule& s, Joins& j) {
+    j.n = 0;
+    int used = 0;
+    for (int c = 1; c < s.parts; c++) {
+        const Start b = s.at[c], before = s.at[c - 1];
+        const bool same = before.g == b.g && before.t == b.t;
+        if (b.k == 0 || (same && before.k != 0)) continue;  // no cut, or not the first in this unit
+        j.unit[j.n] = b;
+        j.first[j.n++] = (short)used;
+        j.slot[used++] = (short)(2 * (c - 1) + (same ? 0 : 1));
+        int k = c;
+        do {
+            const Start from = s.at[k], to = s.at[k + 1];
+            if (from.k != to.k || from.g != to.g || from.t != to.t) j.slot[used++] = (short)(2 * k);  // not an empty range
+        } while (++k < s.parts && s.at[k].g == b.g && s.at[k].t == b.t);
+    }
+    j.first[j.n] = (short)used;
+}
+
+// Adds up the parts of cut units in the order of the ranges.  CTA (i, j): 32 columns of the i-th from 32 j on.
 template <int NT>
-__global__ void __launch_bounds__(256) fp4_join_kernel(const __grid_constant__ TileArgs a, const __grid_constant__ Schedule plan) {
+__global__ void __launch_bounds__(256) fp4_join_kernel(const __grid_constant__ TileArgs a, const __grid_constant__ Joins joins) {
     constexpr int CG = Cfg<NT>::CG, ROWS = 128 * CG;
-    const int c = (int)blockIdx.x + 1;
-    const Start b = plan.at[c], before = plan.at[c - 1];
-    const bool same = before.g == b.g && before.t == b.t;
-    if (b.k == 0 || (same && before.k != 0)) return;
+    const Start b = joins.unit[blockIdx.x];
+    const int k0 = joins.first[blockIdx.x], k1 = joins.first[blockIdx.x + 1];
     const int n0 = (CG == 2 ? b.t : b.t % a.col_tiles) * NT + (int)blockIdx.y * 32;
     const int m0 = b.g * 256 + (CG == 2 ? 0 : b.t / a.col_tiles * 128);
     __shared__ float tile[32][ROWS + 1];
-    __shared__ int slots[kMaxParts + 1], n_slots;
-    if (threadIdx.x == 0) {
-        int n = 0;
-        slots[n++] = 2 * (c - 1) + (same ? 0 : 1);
-        int k = c;
-        do {
-            const Start from = plan.at[k], to = plan.at[k + 1];
-            if (from.k != to.k || from.g != to.g || from.t != to.t) slots[n++] = 2 * k;  // not an empty range
-        } while (++k < plan.parts && plan.at[k].g == b.g && plan.at[k].t == b.t);
-        n_slots = n;
-    }
-    __syncthreads();
     // 16 independent sums a thread: one after the other, each a chain of loads, they took 48 us
     const int row = threadIdx.x % ROWS, cols = min(32, a.N - n0);
     for (int c0 = threadIdx.x / ROWS * 16; c0 < 32; c0 += 256 / ROWS * 16) {
@@ -556,8 +593,8 @@ __global__ void __launch_bounds__(256) fp4_join_kernel(const __grid_constant__ T
 #pragma unroll
         for (int j = 0; j < 16; j++) v[j] = 0.f;
         const float* src = a.scratch + ((size_t)blockIdx.y * 32 + c0) * ROWS + row;
-        for (int k = 0; k < n_slots; k++) {
-            const float* p = src + (size_t)slots[k] * (ROWS * NT);
+        for (int k = k0; k < k1; k++) {
+            const float* p = src + (size_t)joins.slot[k] * (ROWS * NT);
 #pragma unroll
             for (int j = 0; j < 16; j++)
                 if (c0 + j < cols) v[j] += __ldg(p + j * ROWS);
@@ -579,31 +616,48 @@ __global__ void __launch_bounds__(256) fp4_join_kernel(const __grid_constant__ T
 // Returns whether any unit is cut.
 bool make_schedule(const int* gsp, int groups, int units, int sms, Schedule& s) {
     constexpr long long kLeast = 8;  // steps of a range: below, joining costs more than the time saved
+    constexpr long long kUnit = 6;   // what a unit takes beside its steps, in steps
     const long long total = (long long)gsp[groups] * units, all = (long long)groups * units;
     s.parts = (int)std::max<long long>(std::min<long long>(std::min(sms, kMaxParts), std::max(total / kLeast, all)), 1);
     s.units = units;
     s.rounds = (int)(all / s.parts);
     long long load[kMaxParts];
-    auto steps_of = [&](long long unit) { return (long long)(gsp[unit / units + 1] - gsp[unit / units]); };
+    auto cost_of = [&](long long unit) { return (long long)(gsp[unit / units + 1] - gsp[unit / units]) + kUnit; };
+    const long long cost = total + kUnit * all;
     auto deal = [&]() {
         long long most = 0;
         for (int c = 0; c < s.parts; c++) load[c] = 0;
         for (int r = 0; r < s.rounds; r++)
-            for (int c = 0; c < s.parts; c++) load[c] += steps_of((long long)r * s.parts + c);
+            for (int c = 0; c < s.parts; c++) load[c] += cost_of((long long)r * s.parts + c);
         for (int c = 0; c < s.parts; c++) most = std::max(most, load[c]);
         return most;
     };
     // Units of very different lengths: everything in ranges.
-    if (deal() * s.parts > total + total / 4) { s.rounds = 0; deal(); }
+    if (deal() * s.parts > cost + cost / 4) { s.rounds = 0; deal(); }
     const long long first = (long long)s.rounds * s.parts;  // the first unit of the ranges
     int g = (int)(first / units);
     const long long begin = (long long)gsp[g] * units + (first - (long long)g * units) * (g < groups ? gsp[g + 1] - gsp[g] : 0);
     const long long rest = total - begin;
-    // A part gets of the rest what it is short of an equal share; ranges of long units may cut them, others hold whole ones.
     const bool may_cut = rest >= 2 * kLeast * (all - first);
     long long want[kMaxParts], sum = 0, given = 0;
+    if (s.rounds && !may_cut) {
+        // Short units: one more for each of the parts with the least to do.
+        int order[kMaxParts];
+        for (int c = 0; c < s.parts; c++) order[c] = c;
+        std::sort(order, order + s.parts, [&](int x, int y) { return load[x] != load[y] ? load[x] < load[y] : x < y; });
+        bool one[kMaxParts] = {};
+        for (long long j = 0; j < all - first; j++) one[order[j]] = true;
+        long long unit = first;
+        for (int c = 0; c < s.parts; c++) {
+            s.at[c] = {(int)(unit / units), (int)(unit % units), 0};
+            unit += one[c];
+        }
+        s.at[s.parts] = {groups, 0, 0};
+        return false;
+    }
+    // A part gets of the rest what it is short of an equal share; ranges of long units may cut them, others hold whole ones.
     for (int c = 0; c < s.parts; c++) {
-        want[c] = std::max<long long>(total / s.parts + 1 - load[c], 0);
+        want[c] = std::max<long long>(cost / s.parts + 1 - load[c], 0);
         if (want[c] < kLeast && may_cut) want[c] = 0;
         sum += want[c];
     }
@@ -658,7 +712,9 @@ int launch_tile(const TileArgs& args, const CUtensorMap& map, const int* gsp, in
     cudaError_t e = cudaLaunchKernelEx(&cfg, fp4_tile_kernel<NT, FMT>, map, a, s);
     count_launch();
     if (e == cudaSuccess && cut) {
-        fp4_join_kernel<NT><<<dim3(s.parts - 1, NT / 32), 256, 0, stream>>>(a, s);
+        Joins joins;
+        list_joins(s, joins);
+        fp4_join_kernel<NT><<<dim3(joins.n, NT / 32), 256, 0, stream>>>(a, joins);
         e = cudaGetLastError();
         count_launch();
     }
