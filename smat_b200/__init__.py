@@ -43,5 +43,6 @@ _FP4 = ("Fp4Matrix", "Fp4Plan", "Fp4SparseMatrix")  # need torch, which is impor
 def __getattr__(name):
     if name in _FP4:
         from . import fp4
-        return getattr(fp4, name)
+        globals().update({n: getattr(fp4, n) for n in _FP4})
+        return globals()[name]
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -14,7 +14,8 @@ import ctypes as C
 
 import torch
 
-from .api import Matrix, SmatError, SparseMatrix, _check, _stream, lib
+from . import api
+from .api import Matrix, SmatError, SparseMatrix, _check, lib
 
 _FORMATS = {"nvfp4": 0, "mxfp4": 1}
 _GROUP = {"nvfp4": 16, "mxfp4": 32}
@@ -100,14 +101,15 @@ class Fp4Matrix:
     [N, groups]), ``row_scale`` float32 [N] or None."""
 
     def __init__(self, N, K, fmt="nvfp4", device="cuda"):
-        _format(fmt)
+        if fmt not in _FORMATS:
+            _format(fmt)
         if K % 16:
             _refuse(f"K ({K}) must be a multiple of 16")
-        self.N, self.K, self.fmt = int(N), int(K), fmt
-        self.quads = -(-self.K // 64)
-        self.codes = torch.empty((self.N, self.quads * 32), dtype=torch.uint8, device=device)
-        self.scales = torch.empty(-(-self.N // 128) * self.quads * 512, dtype=torch.uint8, device=device)
-        self.row_scale = torch.empty(self.N, dtype=torch.float32, device=device) if fmt == "nvfp4" else None
+        self.N, self.K, self.fmt = N, K, fmt
+        self.quads = quads = (K + 63) // 64
+        self.codes = torch.empty((N, quads * 32), dtype=torch.uint8, device=device)
+        self.scales = torch.empty((N + 127) // 128 * quads * 512, dtype=torch.uint8, device=device)
+        self.row_scale = torch.empty(N, dtype=torch.float32, device=device) if fmt == "nvfp4" else None
 
     @classmethod
     def quantize(cls, X, fmt="nvfp4", out=None):
@@ -127,7 +129,7 @@ class Fp4Matrix:
         elif f == 0 and out.row_scale is None:
             _refuse("out has no row scales")
         ld = x.stride(0) if N > 1 else K
-        rc = _lib().smat_fp4_quantize(x.data_ptr(), d, N, K, ld, f, out.codes.data_ptr(), out.scales.data_ptr(), _ptr(out.row_scale), _stream())
+        rc = _lib().smat_fp4_quantize(x.data_ptr(), d, N, K, ld, f, out.codes.data_ptr(), out.scales.data_ptr(), _ptr(out.row_scale), api._stream())
         if rc:
             _check(rc)
         return out
@@ -167,7 +169,7 @@ class Fp4Matrix:
             _refuse("out has another size, strided columns or another device")
         ld = out.stride(0) if self.N > 1 else self.K
         rc = _lib().smat_fp4_dequantize(self.codes.data_ptr(), self.scales.data_ptr(), _ptr(self.row_scale), _FORMATS[self.fmt], self.N,
-                                        self.K, out.data_ptr(), d, ld, _stream())
+                                        self.K, out.data_ptr(), d, ld, api._stream())
         if rc:
             _check(rc)
         return out
@@ -198,11 +200,11 @@ class Fp4SparseMatrix:
         self.bcsrRowPtr, self.bcsrColIdx = A.bcsrRowPtr, A.bcsrColIdx
         self._allocate()
         rc = _lib().smat_fp4_quantize_blocks(A.bcsrVal.data_ptr(), _dtype(A.bcsrVal.dtype), A.bcsrRowPtr.data_ptr(), A.bcsrColIdx.data_ptr(),
-                                             A.M, A.nnzb, f, self.codes.data_ptr(), self.scales.data_ptr(), _ptr(self.row_scale), _stream())
+                                             A.M, A.nnzb, f, self.codes.data_ptr(), self.scales.data_ptr(), _ptr(self.row_scale), api._stream())
         if rc:
             _check(rc)
         if check:
-            _check(lib().smat_device_status(_stream()))
+            _check(lib().smat_device_status(api._stream()))
         return self
 
     @classmethod
@@ -231,11 +233,11 @@ class Fp4SparseMatrix:
         A.bcsrRowPtr, A.bcsrColIdx = self.bcsrRowPtr, self.bcsrColIdx
         A.bcsrVal = torch.empty(max(self.nnzb, 1) * 256, dtype=torch.float16, device=self.codes.device)
         rc = _lib().smat_fp4_dequantize_blocks(self.codes.data_ptr(), self.scales.data_ptr(), _ptr(self.row_scale), _FORMATS[self.fmt],
-                                               A.bcsrRowPtr.data_ptr(), A.M, A.nnzb, A.bcsrVal.data_ptr(), 0, _stream())
+                                               A.bcsrRowPtr.data_ptr(), A.M, A.nnzb, A.bcsrVal.data_ptr(), 0, api._stream())
         if rc:
             _check(rc)
         if check:
-            _check(lib().smat_device_status(_stream()))
+            _check(lib().smat_device_status(api._stream()))
         return A
 
 
@@ -254,7 +256,7 @@ class Fp4Plan:
         L = _lib()
         _check(L.smat_fp4_plan_create(C.byref(h), A.codes.data_ptr(), A.scales.data_ptr(), _ptr(A.row_scale), _FORMATS[A.fmt],
                                       A.bcsrRowPtr.data_ptr(), A.bcsrColIdx.data_ptr(), A.M, A.K, A.nnzb, self.brow_begin,
-                                      self.brow_end, int(tiles), _stream()))
+                                      self.brow_end, int(tiles), api._stream()))
         self._h = h
         self._rows = (self.brow_end - self.brow_begin) * 16
         self._device = A.bcsrRowPtr.device
@@ -263,7 +265,7 @@ class Fp4Plan:
         """After A's codes or scales changed (same structure)."""
         if self._h is None:
             _refuse("the plan is closed")
-        _check(_LIB.smat_fp4_plan_set_values(self._h, _stream()))
+        _check(_LIB.smat_fp4_plan_set_values(self._h, api._stream()))
 
     def spmm(self, B, Cout, check=False):
         """C = A x B.  B: Matrix / tensor [N, K] in fp16 or bf16 with C of the same type, or an Fp4Matrix of A's format with C in
@@ -289,13 +291,13 @@ class Fp4Plan:
             if B.fmt != self.A.fmt:
                 _refuse(f"B is in {B.fmt}, A in {self.A.fmt}")
             rc = _LIB.smat_fp4_plan_spmm_fp4(self._h, Bt.data_ptr(), B.scales.data_ptr(), _ptr(B.row_scale), _FORMATS[B.fmt], Ct.data_ptr(),
-                                             d, N, _stream())
+                                             d, N, api._stream())
         else:
-            rc = _LIB.smat_fp4_plan_spmm(self._h, Bt.data_ptr(), d, Ct.data_ptr(), N, _stream())
+            rc = _LIB.smat_fp4_plan_spmm(self._h, Bt.data_ptr(), d, Ct.data_ptr(), N, api._stream())
         if rc:
             _check(rc)
         if check:
-            _check(lib().smat_device_status(_stream()))
+            _check(lib().smat_device_status(api._stream()))
 
     def close(self):
         if self._h is not None:
