@@ -23,8 +23,13 @@ namespace smat {
 namespace {
 
 constexpr int kThreads = 256;
-// Tiles are made where a step holds so many blocks (of 256) on average.
-constexpr size_t kFp4TileFill = 8;
+// Tiles are made where a step of 256 x 256 holds so many blocks (of 256) on average; they take 36 KB a step.  They are faster at any
+// fill (8192 x 8192, N = 512, tiles against warp-level MMAs: 31 and 55 us with 2 blocks a step, 33 and 77 with 4, 33 and 211 with 16),
+// so this bounds the memory: 9 KB a block, 64 times what is stored.
+constexpr size_t kFp4TileFill = 4;
+// With so few columns and blocks the warp-level kernel is faster all the same (8192 x 8192, N = 8: 5 and 11 us for 2000 blocks, 9 and 13
+// for 33000; it takes 0.15 us more for every 1000).
+constexpr size_t kFp4NarrowColumns = 8, kFp4NarrowBlocks = 50000;
 
 // Looks a block-row's pointers and columns over (a CTA a block-row): they have to lie in the arrays and the matrix, the columns in
 // ascending order.  An inconsistent block-row is left out (empty) and reported.  totals: blocks, longest block-row.
@@ -350,7 +355,8 @@ int smat_fp4_plan_spmm_fp4(const smat_fp4_plan* plan, const void* codes, const v
     rhs.scales = static_cast<const uint8_t*>(scales);
     rhs.row_scale = row_scale;
     rhs.dtype = kFp4Rhs;
-    return (plan->v.tiles ? launch_fp4_tile : launch_fp4_stream)(plan->v, rhs, C, c_dtype, N, (cudaStream_t)stream);
+    const bool narrow = N <= kFp4NarrowColumns && plan->v.blocks <= kFp4NarrowBlocks;
+    return (plan->v.tiles && !narrow ? launch_fp4_tile : launch_fp4_stream)(plan->v, rhs, C, c_dtype, N, (cudaStream_t)stream);
 }
 
 int smat_fp4_plan_destroy(smat_fp4_plan* plan) {

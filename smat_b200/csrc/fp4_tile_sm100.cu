@@ -641,13 +641,25 @@ bool make_schedule(const int* gsp, int groups, int units, int sms, Schedule& s) 
     s.units = units;
     s.rounds = (int)(all / s.parts);
     long long load[kMaxParts];
-    auto cost_of = [&](long long unit) { return (long long)(gsp[unit / units + 1] - gsp[unit / units]) + kUnit; };
+    int shortest = gsp[1], longest = 0;
+    for (int g = 0; g < groups; g++) {
+        shortest = std::min(shortest, gsp[g + 1] - gsp[g]);
+        longest = std::max(longest, gsp[g + 1] - gsp[g]);
+    }
     const long long cost = total + kUnit * all;
     auto deal = [&]() {
         long long most = 0;
-        for (int c = 0; c < s.parts; c++) load[c] = 0;
-        for (int r = 0; r < s.rounds; r++)
-            for (int c = 0; c < s.parts; c++) load[c] += cost_of((long long)r * s.parts + c);
+        for (int c = 0; c < s.parts; c++) load[c] = shortest == longest ? s.rounds * (longest + kUnit) : 0;
+        if (shortest != longest) {
+            const long long dealt = (long long)s.rounds * s.parts;
+            int c = 0;
+            long long unit = 0;
+            for (int g = 0; g < groups && unit < dealt; g++)
+                for (int t = 0; t < units && unit < dealt; t++, unit++) {
+                    load[c] += gsp[g + 1] - gsp[g] + kUnit;
+                    if (++c == s.parts) c = 0;
+                }
+        }
         for (int c = 0; c < s.parts; c++) most = std::max(most, load[c]);
         return most;
     };
