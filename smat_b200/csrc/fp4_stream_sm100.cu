@@ -247,20 +247,27 @@ cudaError_t launch(const StreamArgs& a, int wr, int cl, cudaStream_t stream) {
     return cudaLaunchKernelEx(&cfg, fp4_stream_kernel<BT, FMT, NT, U>, a, wr);
 }
 
-// Columns in tiles of equal width, 64 at most; as many blocks in a batch as the registers hold.
+// Columns in tiles of equal width: 64 at most, 32 of B in 4 bits, whose scales take registers too; as many blocks in a panel as the
+// registers hold.
 template <int BT, int FMT>
 cudaError_t launch_width(const StreamArgs& a, int wr, int cl, cudaStream_t stream) {
-    const int tiles = (a.N + 63) / 64, width = (a.N + tiles - 1) / tiles;
+    constexpr int most = BT == kFp4Rhs ? 32 : 64;
+    const int tiles = (int)(((long long)a.N + most - 1) / most), width = (int)(((long long)a.N + tiles - 1) / tiles);
     switch ((width + 7) / 8) {
         case 1: return launch<BT, FMT, 1, 4>(a, wr, cl, stream);
         case 2: return launch<BT, FMT, 2, 4>(a, wr, cl, stream);
         case 3: return launch<BT, FMT, 3, 2>(a, wr, cl, stream);
         case 4: return launch<BT, FMT, 4, 2>(a, wr, cl, stream);
-        case 5: return launch<BT, FMT, 5, 1>(a, wr, cl, stream);
-        case 6: return launch<BT, FMT, 6, 1>(a, wr, cl, stream);
-        case 7: return launch<BT, FMT, 7, 1>(a, wr, cl, stream);
-        default: return launch<BT, FMT, 8, 1>(a, wr, cl, stream);
     }
+    if constexpr (BT != kFp4Rhs) {
+        switch ((width + 7) / 8) {
+            case 5: return launch<BT, FMT, 5, 1>(a, wr, cl, stream);
+            case 6: return launch<BT, FMT, 6, 1>(a, wr, cl, stream);
+            case 7: return launch<BT, FMT, 7, 1>(a, wr, cl, stream);
+            default: return launch<BT, FMT, 8, 1>(a, wr, cl, stream);
+        }
+    }
+    return cudaErrorInvalidValue;  // not reached
 }
 template <int BT>
 cudaError_t launch_format(int fmt, const StreamArgs& a, int wr, int cl, cudaStream_t stream) {
