@@ -107,9 +107,42 @@ class Fp4Matrix:
             _refuse(f"K ({K}) must be a multiple of 16")
         self.N, self.K, self.fmt = N, K, fmt
         self.quads = quads = (K + 63) // 64
-        self.codes = torch.empty((N, quads * 32), dtype=torch.uint8, device=device)
-        self.scales = torch.empty((N + 127) // 128 * quads * 512, dtype=torch.uint8, device=device)
-        self.row_scale = torch.empty(N, dtype=torch.float32, device=device) if fmt == "nvfp4" else None
+        # One piece of memory; the tensors in it are made when they are asked for (a microsecond each).
+        self._scales_at = at = (N * quads * 32 + 15) // 16 * 16
+        self._row_at = end = at + (N + 127) // 128 * quads * 512
+        self._memory = m = torch.empty(end + (4 * N if fmt == "nvfp4" else 0), dtype=torch.uint8, device=device)
+        self._codes = self._scales = self._row = None
+        self._own = True  # the addresses below are those of the memory
+        p = m.data_ptr()
+        self._at = (p, p + at, p + end if fmt == "nvfp4" else None)
+
+    @property
+    def device(self):
+        return self._memory.device
+
+    @property
+    def codes(self):
+        if self._codes is None:
+            self._codes = self._memory[:self.N * self.quads * 32].view(self.N, self.quads * 32)
+        return self._codes
+
+    @property
+    def scales(self):
+        if self._scales is None:
+            self._scales = self._memory[self._scales_at:self._row_at]
+        return self._scales
+
+    @property
+    def row_scale(self):
+        if self._row is None and self._at[2] is not None and self._own:
+            self._row = self._memory[self._row_at:].view(torch.float32)
+        return self._row
+
+    @row_scale.setter
+    def row_scale(self, value):
+        self._row = _row_scales(value, self.fmt, self.N, self.device)
+        self._own = False
+        self._at = (self._at[0], self._at[1], _ptr(self._row))
 
     @classmethod
     def quantize(cls, X, fmt="nvfp4", out=None):
@@ -124,12 +157,12 @@ class Fp4Matrix:
         N, K = x.shape
         if out is None:
             out = cls(N, K, fmt, x.device)
-        elif (out.N, out.K, out.fmt, out.codes.device) != (N, K, fmt, x.device):
+        elif (out.N, out.K, out.fmt, out.device) != (N, K, fmt, x.device):
             _refuse("out has another size, format or device")
-        elif f == 0 and out.row_scale is None:
+        elif f == 0 and out._at[2] is None:
             _refuse("out has no row scales")
-        ld = x.stride(0) if N > 1 else K
-        rc = _lib().smat_fp4_quantize(x.data_ptr(), d, N, K, ld, f, out.codes.data_ptr(), out.scales.data_ptr(), _ptr(out.row_scale), api._stream())
+        codes, scales, row = out._at
+        rc = (_LIB or _lib()).smat_fp4_quantize(x.data_ptr(), d, N, K, x.stride(0) if N > 1 else K, f, codes, scales, row, api._stream())
         if rc:
             _check(rc)
         return out
@@ -140,7 +173,7 @@ class Fp4Matrix:
         scales 8-bit [N, ceil(K / 16 or 32)] (e4m3, or e8m0 bytes), row_scale one number or [N]."""
         N = codes.shape[0]
         self = cls(N, K, fmt, device)
-        dev = self.codes.device
+        dev = self.device
         self.codes.zero_()
         self.codes[:, :K // 2] = _bytes_like(codes, (N, K // 2), "codes", dev)
         groups, per = -(-K // _GROUP[fmt]), 64 // _GROUP[fmt]
@@ -149,8 +182,8 @@ class Fp4Matrix:
         flat = torch.zeros((N, self.quads * per), dtype=torch.uint8, device=dev)
         flat[:, :groups] = s
         full[:N, :, :per] = flat.view(N, self.quads, per)
-        self.scales = full.view(-1, 4, 32, self.quads, 4).permute(0, 3, 2, 1, 4).reshape(-1).contiguous()
-        self.row_scale = _row_scales(row_scale, fmt, N, dev)
+        self.scales.copy_(full.view(-1, 4, 32, self.quads, 4).permute(0, 3, 2, 1, 4).reshape(-1))
+        self.row_scale = row_scale
         return self
 
     def group_scales(self):
@@ -162,14 +195,15 @@ class Fp4Matrix:
     def dequantize(self, dtype=torch.float16, out=None):
         """The values as a tensor [N, K] in fp16, bf16 or fp32, rounded once; ``out``: a tensor to write to."""
         d = _dtype(dtype if out is None else out.dtype)
-        _on_current_device(self.codes)
+        _on_current_device(self._memory)
         if out is None:
-            out = torch.empty((self.N, self.K), dtype=dtype, device=self.codes.device)
-        elif tuple(out.shape) != (self.N, self.K) or (self.K > 1 and out.stride(1) != 1) or out.device != self.codes.device:
-            _refuse("out has another size, strided columns or another device")
-        ld = out.stride(0) if self.N > 1 else self.K
-        rc = _lib().smat_fp4_dequantize(self.codes.data_ptr(), self.scales.data_ptr(), _ptr(self.row_scale), _FORMATS[self.fmt], self.N,
-                                        self.K, out.data_ptr(), d, ld, api._stream())
+            out, ld = torch.empty((self.N, self.K), dtype=dtype, device=self.device), self.K
+        else:
+            if tuple(out.shape) != (self.N, self.K) or (self.K > 1 and out.stride(1) != 1) or out.device != self.device:
+                _refuse("out has another size, strided columns or another device")
+            ld = out.stride(0) if self.N > 1 else self.K
+        codes, scales, row = self._at
+        rc = _lib().smat_fp4_dequantize(codes, scales, row, _FORMATS[self.fmt], self.N, self.K, out.data_ptr(), d, ld, api._stream())
         if rc:
             _check(rc)
         return out
@@ -273,25 +307,29 @@ class Fp4Plan:
         if self._h is None:
             _refuse("the plan is closed")
         Ct = Cout.data if isinstance(Cout, Matrix) else Cout
-        if isinstance(B, Fp4Matrix):
-            N, K, Bt = B.N, B.K, B.codes
+        four = isinstance(B, Fp4Matrix)
+        if four:
+            N, K, device = B.N, B.K, B.device
         else:
             Bt = B.data if isinstance(B, Matrix) else B
             N, K = Bt.shape
+            device = Bt.device
             if Bt.dtype != Ct.dtype:
                 _refuse(f"B is {Bt.dtype}, C is {Ct.dtype}: the same type is expected")
+            if not Bt.is_contiguous():
+                _refuse("B has to be contiguous")
         if K != self.A.K or tuple(Ct.shape) != (self._rows, N):
             _refuse(f"B [N, {self.A.K}] and C [{self._rows}, N] are expected, not [{N}, {K}] and {list(Ct.shape)}")
-        if not (Bt.is_contiguous() and Ct.is_contiguous()):
-            _refuse("B and C have to be contiguous")
-        if Bt.device != self._device or Ct.device != self._device:
+        if not Ct.is_contiguous():
+            _refuse("C has to be contiguous")
+        if device != self._device or Ct.device != self._device:
             _refuse(f"B and C have to be on {self._device}, like A")
         d = _dtype(Ct.dtype, most=1)
-        if isinstance(B, Fp4Matrix):
+        if four:
             if B.fmt != self.A.fmt:
                 _refuse(f"B is in {B.fmt}, A in {self.A.fmt}")
-            rc = _LIB.smat_fp4_plan_spmm_fp4(self._h, Bt.data_ptr(), B.scales.data_ptr(), _ptr(B.row_scale), _FORMATS[B.fmt], Ct.data_ptr(),
-                                             d, N, api._stream())
+            codes, scales, row = B._at
+            rc = _LIB.smat_fp4_plan_spmm_fp4(self._h, codes, scales, row, _FORMATS[B.fmt], Ct.data_ptr(), d, N, api._stream())
         else:
             rc = _LIB.smat_fp4_plan_spmm(self._h, Bt.data_ptr(), d, Ct.data_ptr(), N, api._stream())
         if rc:
