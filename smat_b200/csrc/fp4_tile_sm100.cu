@@ -636,6 +636,7 @@ __global__ void __launch_bounds__(256) fp4_join_kernel(const __grid_constant__ T
 bool make_schedule(const int* gsp, int groups, int units, int sms, Schedule& s) {
     constexpr long long kLeast = 8;  // steps of a range: below, joining costs more than the time saved
     constexpr long long kUnit = 6;   // what a unit takes beside its steps, in steps
+    constexpr long long kJoin = 24;  // what storing parts and joining them takes, in steps (8 to 10 us)
     const long long total = (long long)gsp[groups] * units, all = (long long)groups * units;
     s.parts = (int)std::max<long long>(std::min<long long>(std::min(sms, kMaxParts), std::max(total / kLeast, all)), 1);
     s.units = units;
@@ -664,20 +665,33 @@ bool make_schedule(const int* gsp, int groups, int units, int sms, Schedule& s) 
         return most;
     };
     // Units of very different lengths: everything in ranges.
-    if (deal() * s.parts > cost + cost / 4) { s.rounds = 0; deal(); }
+    const bool uneven = s.rounds && deal() * s.parts > cost + cost / 4;
+    if (uneven) s.rounds = 0;
+    long long most = deal();
     const long long first = (long long)s.rounds * s.parts;  // the first unit of the ranges
     int g = (int)(first / units);
     const long long begin = (long long)gsp[g] * units + (first - (long long)g * units) * (g < groups ? gsp[g + 1] - gsp[g] : 0);
     const long long rest = total - begin;
-    const bool may_cut = rest >= 2 * kLeast * (all - first);
-    long long want[kMaxParts], sum = 0, given = 0;
-    if (s.rounds && !may_cut) {
-        // Short units: one more for each of the parts with the least to do.
-        int order[kMaxParts];
+    const long long left = all - first;  // units: fewer than parts, unless they are uneven
+    bool may_cut = rest >= 2 * kLeast * left;
+    int order[kMaxParts];
+    if (!uneven) {
+        // Whole units, one more for each of the parts with the least to do, or cut to equal shares?
         for (int c = 0; c < s.parts; c++) order[c] = c;
         std::sort(order, order + s.parts, [&](int x, int y) { return load[x] != load[y] ? load[x] < load[y] : x < y; });
+        if (left) most = std::max(most, load[order[left - 1]] + longest + kUnit);
+        if (most <= cost / s.parts + kJoin) may_cut = false;
+        if (!may_cut && !s.rounds) {
+            s.parts = (int)all;
+            s.rounds = 1;
+            for (int c = 0; c <= s.parts; c++) s.at[c] = {groups, 0, 0};
+            return false;
+        }
+    }
+    long long want[kMaxParts], sum = 0, given = 0;
+    if (!uneven && !may_cut) {
         bool one[kMaxParts] = {};
-        for (long long j = 0; j < all - first; j++) one[order[j]] = true;
+        for (long long j = 0; j < left; j++) one[order[j]] = true;
         long long unit = first;
         for (int c = 0; c < s.parts; c++) {
             s.at[c] = {(int)(unit / units), (int)(unit % units), 0};
