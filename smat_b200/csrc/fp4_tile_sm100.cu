@@ -96,6 +96,13 @@ __device__ __forceinline__ void arrive_at_first(uint32_t bar) {
 __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
+// Stores under a predicate, without a branch.
+__device__ __forceinline__ void store_if(bool on, uint16_t* p, uint32_t v) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %2, 0;\n\t@q st.global.u32 [%0], %1;\n\t}" ::"l"(p), "r"(v), "r"((uint32_t)on) : "memory");
+}
+__device__ __forceinline__ void store_if(bool on, uint16_t* p, uint16_t v) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %2, 0;\n\t@q st.global.u16 [%0], %1;\n\t}" ::"l"(p), "h"(v), "r"((uint32_t)on) : "memory");
+}
 // Writes 16 consecutive columns of the calling thread's lane.
 __device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint4* v) {
     asm volatile(
@@ -103,11 +110,6 @@ __device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint4* v) {
         "r"(v[0].x), "r"(v[0].y), "r"(v[0].z), "r"(v[0].w), "r"(v[1].x), "r"(v[1].y), "r"(v[1].z), "r"(v[1].w), "r"(v[2].x), "r"(v[2].y),
         "r"(v[2].z), "r"(v[2].w), "r"(v[3].x), "r"(v[3].y), "r"(v[3].z), "r"(v[3].w)
         : "memory");
-}
-__device__ __forceinline__ uint16_t ld_shared_u16(uint32_t addr) {
-    uint16_t v;
-    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr) : "memory");
-    return v;
 }
 
 // ---- schedule -------------------------------------------------------------------------------------------------------------------
@@ -510,8 +512,23 @@ fp4_tile_kernel(const __grid_constant__ CUtensorMap mapB, const __grid_constant_
                         if (m0 + r < a.rows && j * 8 < width) *reinterpret_cast<uint4*>(to + (size_t)r * a.N + j * 8) = v;
                     }
                 } else {
-                    for (int r = 0; r < 32 && m0 + r < a.rows; r++)
-                        for (int j = lane; j < width; j += 32) to[(size_t)r * a.N + j] = ld_shared_u16(out + r * 128 + (((j >> 3) ^ (r & 7)) << 4) + (j & 7) * 2);
+                    // Rows begin anywhere: a warp a row, two columns a lane from the first even address on.  (One column at a time took
+                    // 20000 cycles a tile.)
+                    for (int r0 = 0; r0 < 32; r0 += 8) {
+                        uint32_t w[8];
+#pragma unroll
+                        for (int i = 0; i < 8; i++) w[i] = ld_shared_u32(out + (r0 + i) * 128 + (((lane >> 2) ^ i) << 4) + (lane & 3) * 4);
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            uint16_t* const row = to + (size_t)(r0 + i) * a.N;
+                            const int odd = (int)((uintptr_t)row >> 1 & 1), j = 2 * lane + odd;
+                            const uint32_t after = __shfl_down_sync(~0u, w[i], 1), v = odd ? w[i] >> 16 | after << 16 : w[i];
+                            const bool in = m0 + r0 + i < a.rows;
+                            store_if(in && j + 1 < width, row + j, v);
+                            store_if(in && j + 1 == width, row + j, (uint16_t)v);
+                            store_if(in && odd && lane == 0, row, (uint16_t)w[i]);
+                        }
+                    }
                 }
                 __syncwarp();
             };

@@ -87,7 +87,7 @@ def test_16bit(fmt, dtype, counts, Kb, N):
 @pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("counts,Kb", SHAPES + [([100] * 40, 130), ([16] * 3 + [0] * 40 + [13] * 10 + [0] * 30, 16), ([0] * 9 + [12], 12), ([5] * 300, 48)])
-@pytest.mark.parametrize("N", [1, 8, 9, 31, 64, 128, 129, 300])
+@pytest.mark.parametrize("N", [1, 8, 9, 31, 64, 106, 128, 129, 191, 300])
 def test_4bit(fmt, dtype, counts, Kb, N):
     c = Case(N + Kb, counts, Kb, fmt)
     B, b = c.acts4(N)
