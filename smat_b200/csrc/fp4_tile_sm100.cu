@@ -100,6 +100,11 @@ __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t
 __device__ __forceinline__ void store_if(bool on, uint16_t* p, uint32_t v) {
     asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %2, 0;\n\t@q st.global.u32 [%0], %1;\n\t}" ::"l"(p), "r"(v), "r"((uint32_t)on) : "memory");
 }
+__device__ __forceinline__ void store_if(bool on, uint16_t* p, uint4 v) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %5, 0;\n\t@q st.global.v4.u32 [%0], {%1, %2, %3, %4};\n\t}" ::"l"(p), "r"(v.x),
+                 "r"(v.y), "r"(v.z), "r"(v.w), "r"((uint32_t)on)
+                 : "memory");
+}
 __device__ __forceinline__ void store_if(bool on, uint16_t* p, uint16_t v) {
     asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %2, 0;\n\t@q st.global.u16 [%0], %1;\n\t}" ::"l"(p), "h"(v), "r"((uint32_t)on) : "memory");
 }
@@ -509,7 +514,7 @@ fp4_tile_kernel(const __grid_constant__ CUtensorMap mapB, const __grid_constant_
                     for (int r0 = 0; r0 < 32; r0 += 4) {
                         const int r = r0 + lane / 8, j = lane % 8;
                         const uint4 v = ld_shared_v4(out + r * 128 + ((j ^ (r & 7)) << 4));
-                        if (m0 + r < a.rows && j * 8 < width) *reinterpret_cast<uint4*>(to + (size_t)r * a.N + j * 8) = v;
+                        store_if(m0 + r < a.rows && j * 8 < width, to + (size_t)r * a.N + j * 8, v);
                     }
                 } else {
                     // Rows begin anywhere: a warp a row, two columns a lane from the first even address on.  (One column at a time took
