@@ -139,18 +139,6 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
         return *reinterpret_cast<const uint32_t*>(&h);
     }
 }
-template <int DT>
-__device__ __forceinline__ void store16(typename Elem<DT>::T* p, const float (&v)[16]) {
-    if constexpr (DT == SMAT_F32) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) reinterpret_cast<float4*>(p)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-            reinterpret_cast<uint4*>(p)[i] = make_uint4(pack2<DT>(v[8 * i], v[8 * i + 1]), pack2<DT>(v[8 * i + 2], v[8 * i + 3]),
-                                                        pack2<DT>(v[8 * i + 4], v[8 * i + 5]), pack2<DT>(v[8 * i + 6], v[8 * i + 7]));
-    }
-}
 __device__ __forceinline__ void store_c(void* C, int dtype, size_t at, float v) {
     if (dtype == SMAT_F16) static_cast<__half*>(C)[at] = __float2half_rn(v);
     else static_cast<__nv_bfloat16*>(C)[at] = __float2bfloat16_rn(v);

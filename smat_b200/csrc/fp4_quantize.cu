@@ -75,18 +75,24 @@ __device__ __forceinline__ uint2 quantize16(const Raw<DT>& raw, float gmax, bool
     for (int i = 0; i < 16; i++) q[i] = FMT == SMAT_FP4_NV ? divide_for_rounding<DT != SMAT_F32>(q[i], d, y) : q[i] * y;
     return make_uint2(f32x8_to_e2m1(q), f32x8_to_e2m1(q + 8));
 }
+// Eight codes to values: half a group a lane, so that a warp's 16-byte stores lie side by side (a group a lane, each store filled half
+// of 32 sectors: 72 us instead of 57 for 4096 x 28672 bf16).
 template <int DT>
-__device__ __forceinline__ void dequantize16(uint2 c, float s, typename Elem<DT>::T* to) {
-    uint32_t h[2][4];
-    e2m1x8_to_f16(c.x, h[0]);
-    e2m1x8_to_f16(c.y, h[1]);
-    float v[16];
+__device__ __forceinline__ void dequantize8(uint32_t c, float s, typename Elem<DT>::T* to) {
+    uint32_t h[4];
+    e2m1x8_to_f16(c, h);
+    float v[8];
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const float2 f = __half22float2(*reinterpret_cast<__half2*>(&h[i / 4][i % 4]));
+    for (int i = 0; i < 4; i++) {
+        const float2 f = __half22float2(*reinterpret_cast<__half2*>(&h[i]));
         v[2 * i] = f.x * s; v[2 * i + 1] = f.y * s;
     }
-    store16<DT>(to, v);
+    if constexpr (DT == SMAT_F32) {
+        reinterpret_cast<float4*>(to)[0] = make_float4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<float4*>(to)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+        *reinterpret_cast<uint4*>(to) = make_uint4(pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3]), pack2<DT>(v[4], v[5]), pack2<DT>(v[6], v[7]));
+    }
 }
 
 // ---- dense ----------------------------------------------------------------------------------------------------------------------
@@ -169,23 +175,22 @@ template <int FMT, int DT>
 __global__ void __launch_bounds__(kThreads) fp4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                                                                   const float* __restrict__ row_scale, int K,
                                                                   typename Elem<DT>::T* __restrict__ Y, size_t ldy) {
-    constexpr int U = 4;
+    constexpr int U = 8;
     const size_t r = blockIdx.x;
-    const int quads = (K + 63) / 64, groups = K / 16, threads = blockDim.x;
+    const int quads = (K + 63) / 64, halves = K / 8, threads = blockDim.x;
     const float p = row_scale ? __ldg(row_scale + r) : 1.f;
-    for (int j0 = threadIdx.x; j0 < groups; j0 += U * threads) {
-        uint2 c[U];
-        uint32_t s[U];
+    for (int j0 = threadIdx.x; j0 < halves; j0 += U * threads) {
+        uint32_t c[U], s[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const int j = min(j0 + u * threads, groups - 1);
-            c[u] = __ldg(reinterpret_cast<const uint2*>(codes + r * quads * 32) + j);
-            s[u] = __ldg(scales + dense_scale_at<FMT>(r, (size_t)j * 16, quads));
+            const int j = min(j0 + u * threads, halves - 1);
+            c[u] = __ldg(reinterpret_cast<const uint32_t*>(codes + r * quads * 32) + j);
+            s[u] = __ldg(scales + dense_scale_at<FMT>(r, (size_t)j * 8, quads));
         }
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int j = j0 + u * threads;
-            if (j < groups) dequantize16<DT>(c[u], scale_value<FMT>(s[u]) * p, Y + r * ldy + (size_t)j * 16);
+            if (j < halves) dequantize8<DT>(c[u], scale_value<FMT>(s[u]) * p, Y + r * ldy + (size_t)j * 8);
         }
     }
 }
@@ -266,23 +271,23 @@ template <int FMT, int DT>
 __global__ void __launch_bounds__(kThreads) fp4_dequantize_blocks_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                                                                          const float* __restrict__ row_scale, const int* __restrict__ rowptr,
                                                                          size_t nnzb, typename Elem<DT>::T* __restrict__ vals, int* status) {
+    // A warp a block, half a row of it a lane.
+    constexpr int U = 8, STEP = kThreads / 32;
     const int2 range = blocks_of_row(rowptr, blockIdx.x, nnzb, status);
-    const int i = threadIdx.x % 16;
-    constexpr int U = 4, STEP = kThreads / 16;
-    const float p = row_scale ? __ldg(row_scale + (size_t)blockIdx.x * 16 + i) : 1.f;
-    for (int b0 = range.x + threadIdx.x / 16; b0 < range.y; b0 += U * STEP) {
-        uint2 c[U];
-        uint32_t s[U];
+    const int lane = threadIdx.x % 32;
+    const float p = row_scale ? __ldg(row_scale + (size_t)blockIdx.x * 16 + lane / 2) : 1.f;
+    for (int b0 = range.x + threadIdx.x / 32; b0 < range.y; b0 += U * STEP) {
+        uint32_t c[U], s[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int b = min(b0 + u * STEP, range.y - 1);
-            c[u] = __ldg(reinterpret_cast<const uint2*>(codes + (size_t)b * 128) + i);
-            s[u] = __ldg(scales + (size_t)b * 16 + i);
+            c[u] = __ldg(reinterpret_cast<const uint32_t*>(codes + (size_t)b * 128) + lane);
+            s[u] = __ldg(scales + (size_t)b * 16 + lane / 2);
         }
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int b = b0 + u * STEP;
-            if (b < range.y) dequantize16<DT>(c[u], scale_value<FMT>(s[u]) * p, vals + (size_t)b * 256 + i * 16);
+            if (b < range.y) dequantize8<DT>(c[u], scale_value<FMT>(s[u]) * p, vals + (size_t)b * 256 + lane * 8);
         }
     }
 }
@@ -368,7 +373,7 @@ int smat_fp4_dequantize(const void* codes, const void* scales, const float* row_
     if (!N || !K) return SMAT_OK;
     SMAT_CUDA_TRY(with_types(fmt, dtype, [&](auto f, auto d) {
         constexpr int F = decltype(f)::value, D = decltype(d)::value;
-        const int threads = std::max(32, std::min(kThreads, ((int)K / 16 + 31) / 32 * 32));
+        const int threads = std::max(32, std::min(kThreads, ((int)K / 8 + 31) / 32 * 32));
         fp4_dequantize_kernel<F, D><<<(unsigned)N, threads, 0, (cudaStream_t)stream>>>(
             static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), row_scale, (int)K, static_cast<typename Elem<D>::T*>(Y), ldy);
         return cudaGetLastError();
