@@ -28,10 +28,10 @@ __device__ __forceinline__ float pow2_of_row(float amax) {
     return __uint_as_float((uint32_t)(max(e, -100) + 127) << 23);
 }
 
-// x / d for a later rounding to a few bits.  q = RN(x / d) by a reciprocal and one corrective step (Markstein 1990: with the
-// correctly rounded reciprocal, q1 = RN(q0 + (x - q0 d) y) is the correctly rounded quotient).  That q may be a tie of the coarse
-// rounding although x / d is not: then it is moved to the neighbour on the side of x / d.  EXACT16: x has at most 11 significant
-// bits and d four, so a quotient that is no tie is at least 2^-13 away from one and q is already on its side.
+// x / d for a later rounding to a few bits, y = RN(1 / d).  One corrective step makes the quotient the correctly rounded one (Markstein
+// 1990: q1 = RN(q0 + (x - q0 d) y)).  That may be a tie of the coarse rounding although x / d is not: then it is moved to the neighbour
+// on the side of x / d.  EXACT16: x has at most 11 significant bits, and d and the ties so few that a quotient that is no tie is at
+// least 2^-13 of itself away from one; the correctly rounded one is on its side then.
 template <bool EXACT16>
 __device__ __forceinline__ float divide_for_rounding(float x, float d, float y) {
     float q = x * y;
@@ -43,13 +43,16 @@ __device__ __forceinline__ float divide_for_rounding(float x, float d, float y) 
     }
     return q;
 }
+// The same for a code of a value with at most 11 significant bits, in two instructions: the quotient, at most 6.5 in size, rounded to a
+// multiple of 2^-16.  x y is within 2^-21 of it; ties are multiples of 1/4, and what is no tie is at least 2^-13 away from one.
+__device__ __forceinline__ float divide_for_code(float x, float y) { return fmaf(x, y, 192.f) - 192.f; }
 
 // Scale byte of a group with largest magnitude gmax (bad: it holds a NaN or an infinity); values are divided by d, whose correctly
 // rounded reciprocal is y.  p: the row's power of two.
-template <int FMT>
+template <int FMT, bool EXACT16>
 __device__ __forceinline__ uint32_t group_scale(float gmax, bool bad, float p, float inv_p, float& d, float& y) {
     if constexpr (FMT == SMAT_FP4_NV) {
-        const float g = divide_for_rounding<false>(gmax * inv_p, 6.f, 1.f / 6.f);
+        const float g = divide_for_rounding<EXACT16>(gmax * inv_p, 6.f, 1.f / 6.f);
         uint16_t c;
         asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(c) : "f"(0.f), "f"(g));
         const float s = scale_e4m3(c & 0x7fu);
@@ -68,11 +71,12 @@ __device__ __forceinline__ uint32_t group_scale(float gmax, bool bad, float p, f
 template <int FMT, int DT>
 __device__ __forceinline__ uint2 quantize16(const Raw<DT>& raw, float gmax, bool bad, float p, float inv_p, uint32_t& scale) {
     float d, y, q[16];
-    scale = group_scale<FMT>(gmax, bad, p, inv_p, d, y);
+    scale = group_scale<FMT, DT != SMAT_F32>(gmax, bad, p, inv_p, d, y);
     if (bad || d == 0.f) return make_uint2(0, 0);
     raw.unpack(q);
 #pragma unroll
-    for (int i = 0; i < 16; i++) q[i] = FMT == SMAT_FP4_NV ? divide_for_rounding<DT != SMAT_F32>(q[i], d, y) : q[i] * y;
+    for (int i = 0; i < 16; i++)
+        q[i] = FMT == SMAT_FP4_MX ? q[i] * y : DT == SMAT_F32 ? divide_for_rounding<false>(q[i], d, y) : divide_for_code(q[i], y);
     return make_uint2(f32x8_to_e2m1(q), f32x8_to_e2m1(q + 8));
 }
 // Eight codes to values: half a group a lane, so that a warp's 16-byte stores lie side by side (a group a lane, each store filled half
