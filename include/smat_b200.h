@@ -196,10 +196,11 @@ int smat_fp4_dequantize_blocks(const void* codes, const void* scales, const floa
 
 /* Plan for products of block-rows [brow_begin, brow_end) of a block matrix in 4 bits.  It looks the arrays over (block columns in
  * strictly ascending order, multiples of 16 inside the matrix; inconsistent block-rows count as empty and are reported by
- * smat_device_status) and keeps the pointers it was given.  with_tiles: it also holds the blocks laid out for products with B in 4
- * bits, 36 KB for every 256 rows x 256 columns that hold a block, unless they hold fewer than 4 on average; without, such products work
- * but are slow.  After codes or scales changed (same structure) call smat_fp4_plan_set_values.  Nothing in a plan is written by a
- * product, so any number of streams may use it at a time.  Creation synchronises `stream`; K below 2^26. */
+ * smat_device_status), keeps the pointers it was given and holds the blocks in the order of the kernel for few columns (148 bytes
+ * each).  with_tiles: it also holds them laid out for products with B in 4 bits, 36 KB for every 256 rows x 256 columns that hold a
+ * block, unless they hold fewer than 4 on average; without, such products work but are slow.  After codes or scales changed (same
+ * structure) call smat_fp4_plan_set_values.  Nothing in a plan is written by a product, so any number of streams may use it at a
+ * time.  Creation synchronises `stream`; K below 2^26. */
 typedef struct smat_fp4_plan smat_fp4_plan;
 int smat_fp4_plan_create(smat_fp4_plan** plan, const void* codes, const void* scales, const float* row_scale, int fmt, const int* rowptr,
                          const int* colidx, size_t M, size_t K, size_t nonzeroBlocks, size_t brow_begin, size_t brow_end, int with_tiles, void* stream);

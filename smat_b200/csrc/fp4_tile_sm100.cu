@@ -15,7 +15,10 @@
 // Roles.  One thread fetches tiles of A (bulk copies), B (tiled TMA copies with 128-byte swizzle) and its scales; four warps move the
 // scales to tensor memory through registers (tcgen05.cp, 12 of them a step, took their issuer 24 cycles each in a CTA of its own and
 // 140 in a pair); one thread issues the MMAs; eight warps store finished tiles of C through shared memory, whole 128-byte lines at a
-// time.  Of a pair, the second CTA issues no MMAs.  All waits are bounded.
+// time.  Of a pair, the second CTA issues no MMAs.
+//
+// Measured: layer 8192 x 28672 at 20 %, N = 4096, 335 us, steps of 630 cycles (512 of MMAs) at 1.6 GHz, the power limit; that is 5.7
+// PFLOP/s with the zeros, 1.15 without.  All waits are bounded.
 #include <algorithm>
 #include <type_traits>
 

@@ -220,8 +220,8 @@ class Fp4SparseMatrix:
 
     def _allocate(self):
         dev = self.bcsrRowPtr.device
-        self.codes = torch.empty((max(self.nnzb, 1), 16, 8), dtype=torch.uint8, device=dev)[:self.nnzb]
-        self.scales = torch.empty((max(self.nnzb, 1), 16), dtype=torch.uint8, device=dev)[:self.nnzb]
+        self.codes = torch.empty((self.nnzb, 16, 8), dtype=torch.uint8, device=dev)
+        self.scales = torch.empty((self.nnzb, 16), dtype=torch.uint8, device=dev)
         self.row_scale = torch.empty(self.M, dtype=torch.float32, device=dev) if self.fmt == "nvfp4" else None
 
     @classmethod
@@ -277,7 +277,7 @@ class Fp4SparseMatrix:
 
 class Fp4Plan:
     """Plan for products of block-rows [brow_begin, brow_end) of an Fp4SparseMatrix (smat_fp4_plan_*).  ``tiles=False``: only for
-    products with 16-bit B (decoding); those with B in 4 bits work but are slow, and the plan takes next to no memory.  Products do
+    products with 16-bit B (decoding), 148 bytes a block; those with B in 4 bits work but are slow.  Products do
     not change the plan and may run on several streams at a time."""
 
     def __init__(self, A, brow_begin=0, brow_end=None, tiles=True):

@@ -264,6 +264,43 @@ def test_inconsistent_arrays_are_reported_and_left_out():
             _close(C[lo:lo + 16], ref[lo:lo + 16], mag[lo:lo + 16], 4)
 
 
+@pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
+def test_nothing_stored(fmt):
+    """A matrix without blocks goes all the way; its products are zeros, whatever B holds."""
+    A = S.SparseMatrix.from_bcsr(64, 96, np.zeros(5, np.int32), np.zeros(0, np.int32), np.zeros(0, np.float16))
+    A4 = S.Fp4SparseMatrix.quantize(A, fmt, check=True)
+    assert A4.dequantize(check=True).nnzb == 0
+    plan = S.Fp4Plan(A4)
+    plan.set_values()
+    x = torch.full((5, 96), float("nan"), dtype=torch.float16, device="cuda")
+    for B in (x, S.Fp4Matrix.quantize(x, fmt)):
+        C = torch.full((64, 5), float("nan"), dtype=torch.float16, device="cuda")
+        plan.spmm(B, C, check=True)
+        assert bool((C == 0).all())
+    plan.spmm(x[:0], torch.empty((64, 0), dtype=torch.float16, device="cuda"), check=True)
+    assert S.Fp4Matrix.quantize(x[:0], fmt).dequantize().shape == (0, 96)
+
+
+@pytest.mark.parametrize("N", [40, 300])
+def test_long_and_short_groups(N):
+    """Groups of block-rows of very different lengths: their tiles of C are dealt out in ranges, and cut."""
+    rng = np.random.default_rng(13)
+    Kb, rows = 1600, 16 * 90
+    cols = [np.sort(rng.choice(Kb, 500, replace=False)) if r // 16 in (3, 40) else np.arange(r % 7, r % 7 + 16) for r in range(rows)]
+    rowptr = np.zeros(rows + 1, np.int32)
+    rowptr[1:] = np.cumsum([len(c) for c in cols])
+    colidx = np.concatenate(cols).astype(np.int32) * 16
+    n = int(rowptr[-1])
+    codes, scales = rng.integers(0, 16, (n, 16, 16)).astype(np.uint8), rng.integers(30, 60, (n, 16)).astype(np.uint8)
+    A = S.Fp4SparseMatrix.from_codes(rows * 16, Kb * 16, rowptr, colidx, F.pack(codes), scales)
+    vals = F.block_values(codes, scales, None, rowptr, "nvfp4")
+    x = torch.from_numpy(rng.standard_normal((N, Kb * 16))).half().cuda()
+    B = S.Fp4Matrix.quantize(x)
+    C = torch.empty((rows * 16, N), dtype=torch.bfloat16, device="cuda")
+    S.Fp4Plan(A).spmm(B, C, check=True)
+    _close(C, *F.multiply(vals, rowptr, colidx, B.dequantize(torch.float32).double().cpu().numpy()), 500)
+
+
 def test_as_a_program_runs_them():
     """A layer in fp16 goes to 4 bits, decodes with 16-bit activations and prefills with 4-bit ones; both agree with the matrix that
     the codes stand for, multiplied by the framework's fp16 product."""
