@@ -140,9 +140,11 @@ class Fp4Matrix:
 
     @row_scale.setter
     def row_scale(self, value):
-        self._row = _row_scales(value, self.fmt, self.N, self.device)
-        self._own = False
-        self._at = (self._at[0], self._at[1], _ptr(self._row))
+        t = _row_scales(value, self.fmt, self.N, self.device)
+        self._row, self._own = None, t is not None
+        if self._own:  # a copy: quantize(out=...) writes to it later
+            self._memory[self._row_at:].view(torch.float32).copy_(t)
+        self._at = (self._at[0], self._at[1], self._memory.data_ptr() + self._row_at if self._own else None)
 
     @classmethod
     def quantize(cls, X, fmt="nvfp4", out=None):
@@ -292,13 +294,20 @@ class Fp4Plan:
                                       A.bcsrRowPtr.data_ptr(), A.bcsrColIdx.data_ptr(), A.M, A.K, A.nnzb, self.brow_begin,
                                       self.brow_end, int(tiles), api._stream()))
         self._h = h
+        self._arrays = self._arrays_of(A)  # the plan has their addresses
         self._rows = (self.brow_end - self.brow_begin) * 16
         self._device = A.bcsrRowPtr.device
 
+    @staticmethod
+    def _arrays_of(A):
+        return (A.codes, A.scales, A.row_scale, A.bcsrRowPtr, A.bcsrColIdx)
+
     def set_values(self):
-        """After A's codes or scales changed (same structure)."""
+        """After A's codes or scales changed in place (same structure)."""
         if self._h is None:
             _refuse("the plan is closed")
+        if any(a is not b for a, b in zip(self._arrays, self._arrays_of(self.A))):
+            _refuse("A has other arrays than when the plan was made: change them in place, or make a new plan")
         _check(_LIB.smat_fp4_plan_set_values(self._h, api._stream()))
 
     def spmm(self, B, Cout, check=False):
@@ -341,6 +350,7 @@ class Fp4Plan:
         if self._h is not None:
             _lib().smat_fp4_plan_destroy(self._h)
             self._h = None
+            self._arrays = None
 
     def __del__(self):
         try:

@@ -301,6 +301,41 @@ def test_long_and_short_groups(N):
     _close(C, *F.multiply(vals, rowptr, colidx, B.dequantize(torch.float32).double().cpu().numpy()), 500)
 
 
+def test_arrays_that_were_replaced():
+    """A plan keeps the arrays that it was made of: those that replace them in A are not its own, and the old ones stay alive."""
+    A = S.SparseMatrix.from_bcsr(32, 64, np.array([0, 2, 4], np.int32), np.array([0, 32, 16, 48], np.int32),
+                                 np.random.default_rng(3).standard_normal(1024).astype(np.float16))
+    A4 = S.Fp4SparseMatrix.quantize(A)
+    plan = S.Fp4Plan(A4)
+    x = torch.randn((4, 64), dtype=torch.float16, device="cuda")
+    before, after = (torch.empty((32, 4), dtype=torch.float16, device="cuda") for _ in range(2))
+    plan.spmm(x, before)
+    A4.row_scale = torch.zeros_like(A4.row_scale)
+    junk = [torch.zeros(32, dtype=torch.float32, device="cuda") for _ in range(64)]  # would take a freed array's place
+    plan.spmm(x, after)
+    assert torch.equal(before, after) and bool((before != 0).any())
+    with pytest.raises(S.SmatError, match="other arrays"):
+        plan.set_values()
+    del junk
+
+
+def test_row_scales_given_are_copied():
+    """Quantising into a matrix leaves the caller's row scales as they were."""
+    x = torch.randn((5, 64), dtype=torch.float16, device="cuda") * 100
+    given = torch.full((5,), 0.75, dtype=torch.float32, device="cuda")
+    B = S.Fp4Matrix.quantize(x)
+    codes, scales, own = B.codes[:, :32].clone(), B.group_scales(), B.row_scale.clone()
+    B.row_scale = given
+    assert torch.equal(B.row_scale, given)
+    assert torch.equal(B.dequantize(torch.float32), S.Fp4Matrix.from_codes(codes, scales, 64, row_scale=given).dequantize(torch.float32))
+    S.Fp4Matrix.quantize(x, out=B)
+    assert bool((given == 0.75).all()) and torch.equal(B.row_scale, own)
+    B.row_scale = None
+    assert B.row_scale is None
+    with pytest.raises(S.SmatError, match="no row scales"):
+        S.Fp4Matrix.quantize(x, out=B)
+
+
 def test_as_a_program_runs_them():
     """A layer in fp16 goes to 4 bits, decodes with 16-bit activations and prefills with 4-bit ones; both agree with the matrix that
     the codes stand for, multiplied by the framework's fp16 product."""
