@@ -124,8 +124,8 @@ int encode_tensor_map_2d_f16(CUtensorMap* map, const void* base, uint64_t inner,
                                 swizzle_bytes, l2_promo_bytes);
 }
 int encode_tensor_map_2d_u8(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint64_t row_pitch_bytes, uint32_t box_inner,
-                            uint32_t box_outer) {
-    return encode_tensor_map_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, inner, outer, row_pitch_bytes, box_inner, box_outer, 128, 128);
+                            uint32_t box_outer, int swizzle_bytes) {
+    return encode_tensor_map_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, inner, outer, row_pitch_bytes, box_inner, box_outer, swizzle_bytes, 128);
 }
 
 int check_spmm_args(const void* vals, const int* rowptr, const int* colidx, const void* B, const void* C, size_t M,

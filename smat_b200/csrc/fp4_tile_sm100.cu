@@ -12,13 +12,13 @@
 // Beyond 128 columns of C two CTAs share a tile of 256 x 256 (cta_group::2): each holds 128 rows of A and 128 columns of B, so an SM
 // fetches 38 KB a step of 512 cycles of MMAs instead of 54; L2 delivers about 70 bytes a cycle and SM.
 //
-// Roles.  One thread fetches tiles of A (bulk copies), B (tiled TMA copies with 128-byte swizzle) and its scales; four warps move the
+// Roles.  One thread fetches tiles of A (bulk copies, of a pair tiled ones), B (tiled TMA copies with 128-byte swizzle) and its scales; four warps move the
 // scales to tensor memory through registers (tcgen05.cp, 12 of them a step, took their issuer 24 cycles each in a CTA of its own and
 // 140 in a pair); one thread issues the MMAs; eight warps store finished tiles of C through shared memory, whole 128-byte lines at a
 // time.  Of a pair, the second CTA issues no MMAs.
 //
-// Measured: layer 8192 x 28672 at 20 %, N = 4096, 335 us, steps of 630 cycles (512 of MMAs) at 1.6 GHz, the power limit; that is 5.7
-// PFLOP/s with the zeros, 1.15 without.  All waits are bounded.
+// Measured: layer 8192 x 28672 at 20 %, N = 4096, 342 us, steps of 640 cycles (512 of MMAs) at 1.6 GHz, the power limit; that is 5.6
+// PFLOP/s with the zeros, 1.12 without.  All waits are bounded.
 #include <algorithm>
 #include <type_traits>
 
@@ -88,8 +88,9 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
-// Arrives on the barrier at the same place of the first CTA's shared memory.  What it announces is tensor memory (ordered by the
-// tcgen05 fences around it), so it needs no release at cluster scope, which takes 700 to 900 cycles.
+// Arrives on the barrier at the same place of the first CTA's shared memory.  Only for what lies in tensor memory, which is ordered by the
+// tcgen05 fences around arrival and wait and needs no release at cluster scope (700 to 900 cycles).  Shared memory of the second CTA is
+// announced by the copies that fill it: they complete on the first CTA's barrier.
 __device__ __forceinline__ void arrive_at_first(uint32_t bar) {
     asm volatile(
         "{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %0, 0;\n\t"
@@ -226,7 +227,7 @@ struct Cfg {
     static constexpr uint32_t OFF_OUT = OFF_SF + Q * SF_STAGE;      // 32 rows x 64 columns for each storing warp
     static constexpr uint32_t OFF_COL = OFF_OUT + 8 * 4096;         // and the scales of these columns
     static constexpr uint32_t OFF_BAR = OFF_COL + 8 * 256;
-    static constexpr uint32_t OFF_MISC = OFF_BAR + 8 * (3 * S + 2 * Q + 4);
+    static constexpr uint32_t OFF_MISC = OFF_BAR + 8 * (2 * S + 2 * Q + 4);
     static constexpr uint32_t SMEM = OFF_MISC + 16 + 1024;
     static_assert(STAGE % 1024 == 0 && Q % 2 == 0 && SMEM <= 232448, "shared memory");
     static_assert(ACC * NT <= 256 && 256 + S * SF_COLUMNS <= 512, "tensor memory");
@@ -235,35 +236,38 @@ constexpr int kTileThreads = 20 * 32;
 
 template <int NT, int FMT>
 __global__ void __launch_bounds__(kTileThreads, 1)
-fp4_tile_kernel(const __grid_constant__ CUtensorMap mapB, const __grid_constant__ TileArgs a, const __grid_constant__ Schedule plan) {
+fp4_tile_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB, const __grid_constant__ TileArgs a,
+                const __grid_constant__ Schedule plan) {
     using G = Cfg<NT>;
     constexpr uint32_t S = G::S;
     constexpr int CG = G::CG;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t bar = base + G::OFF_BAR;
-    // A step's codes have arrived and its scales are in tensor memory, of both CTAs: one barrier, since each wait takes the MMAs' thread
-    // 130 cycles.  `full` counts the second CTA's codes.
+    // A step's codes have arrived and its scales are in tensor memory, of both CTAs: one barrier, the first CTA's, since each wait takes
+    // the MMAs' thread 130 cycles.  The second CTA's codes complete on it as well, which releases them at cluster scope; the MMAs' warp
+    // acquires there.  (Layer 8192 x 28672 at 20 %, N = 4096: 342 us.  With a warp of the second CTA that waits for its codes and announces
+    // them with a releasing arrival: 797.)
     auto ready = [&](uint32_t s) { return bar + 8 * s; };
-    auto full = [&](uint32_t s) { return bar + 8 * (S + s); };
-    auto empty = [&](uint32_t s) { return bar + 8 * (2 * S + s); };  // ... and have been used
+    auto empty = [&](uint32_t s) { return bar + 8 * (S + s); };  // ... and have been used
     // Scales in shared memory.  Two sets of warps wait for them in turn, and each must see every phase of a barrier that it waits for
     // by parity, so the stages are an even number.
-    auto arrived = [&](uint32_t s) { return bar + 8 * (3 * S + s); };
-    auto taken = [&](uint32_t s) { return bar + 8 * (3 * S + G::Q + s); };
-    auto acc_full = [&](uint32_t b) { return bar + 8 * (3 * S + 2 * G::Q + b); };
-    auto acc_empty = [&](uint32_t b) { return bar + 8 * (3 * S + 2 * G::Q + 2 + b); };
+    auto arrived = [&](uint32_t s) { return bar + 8 * (2 * S + s); };
+    auto taken = [&](uint32_t s) { return bar + 8 * (2 * S + G::Q + s); };
+    auto acc_full = [&](uint32_t b) { return bar + 8 * (2 * S + 2 * G::Q + b); };
+    auto acc_empty = [&](uint32_t b) { return bar + 8 * (2 * S + 2 * G::Q + 2 + b); };
     const uint32_t tmem_slot = base + G::OFF_MISC, abort_addr = tmem_slot + 4, any_addr = tmem_slot + 8;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = CG == 2 ? uniform(cluster_rank()) : 0;
 
     if (threadIdx.x == 0) {
-        for (uint32_t s = 0; s < S; s++) { mbar_init(ready(s), 1 + 4 * CG + (CG - 1)); mbar_init(full(s), 1); mbar_init(empty(s), 1); }
+        for (uint32_t s = 0; s < S; s++) { mbar_init(ready(s), 1 + 4 * CG); mbar_init(empty(s), 1); }
         for (uint32_t s = 0; s < G::Q; s++) { mbar_init(arrived(s), 1); mbar_init(taken(s), 4); }
         for (uint32_t b = 0; b < 2; b++) { mbar_init(acc_full(b), CG == 1 ? 2 : 1); mbar_init(acc_empty(b), 8 * CG); }
         st_shared_u32(abort_addr, 0);
         fence_barrier_init();
         fence_proxy_async();
+        if (CG == 2) prefetch_tensormap(&mapA);
         prefetch_tensormap(&mapB);
     }
     if (warp == 1) alloc_all<CG>(tmem_slot);
@@ -296,16 +300,22 @@ fp4_tile_kernel(const __grid_constant__ CUtensorMap mapB, const __grid_constant_
             const int row = (int)uniform(column_of(s.t)) * NT + (CG == 2 ? (int)(rank * G::NB) : 0);
             const uint8_t* tile = a.tiles + ((size_t)(gs + (int)uniform(s.k0)) * 2 + half) * kFp4TileBytes;
             for (int k = (int)uniform(s.k0); k < k1; k++, tile += 2 * kFp4TileBytes) {
-                const uint32_t rec = records.get(gs + k), stage = base + st * G::STAGE, arrives = rank == 0 ? ready(st) : full(st);
+                const uint32_t rec = records.get(gs + k), stage = base + st * G::STAGE;
                 ok = __all_sync(~0u, wait_bar(empty(st), phase, abort_addr, a.status, 60));
                 if (!ok) break;
                 if (elect_one()) {
-                    if (quads_of(rec, half) == 0) {  // no blocks here
-                        mbar_arrive(arrives);
+                    if (quads_of(rec, half) == 0) {  // no blocks here, of a pair in neither half
+                        if (rank == 0) mbar_arrive(ready(st));
+                    } else if constexpr (CG == 1) {
+                        mbar_arrive_expect_tx(ready(st), G::STAGE);
+                        bulk_load(stage, tile, kFp4TileCodes, ready(st));
+                        tma_load_2d(stage + G::OFF_B, &mapB, (int)(rec >> 8) * 128, row, ready(st));
                     } else {
-                        mbar_arrive_expect_tx(arrives, G::STAGE);
-                        bulk_load(stage, tile, kFp4TileCodes, arrives);
-                        tma_load_2d(stage + G::OFF_B, &mapB, (int)(rec >> 8) * 128, row, arrives);
+                        // Copies of the second CTA may complete before the first expects them: the phase ends with the first one's arrival.
+                        const uint32_t first = pair_bar(ready(st), 0);
+                        if (rank == 0) mbar_arrive_expect_tx(ready(st), 2 * G::STAGE);
+                        tma_load_2d_pair(stage, &mapA, 0, ((gs + k) * 2 + half) * (int)(kFp4TileBytes / 128), first);
+                        tma_load_2d_pair(stage + G::OFF_B, &mapB, (int)(rec >> 8) * 128, row, first);
                     }
                 }
                 __syncwarp();
@@ -359,7 +369,7 @@ fp4_tile_kernel(const __grid_constant__ CUtensorMap mapB, const __grid_constant_
                 const uint32_t mask = quads_of(records.get(gs + k), half);
                 const uint32_t sf = tmem + 256 + st * G::SF_COLUMNS;
                 const uint32_t da = (uint32_t)da0 + st * (G::STAGE >> 4), db = (uint32_t)db0 + st * (G::STAGE >> 4);
-                ok = __all_sync(~0u, wait_bar(ready(st), phase, abort_addr, a.status, 63));
+                ok = __all_sync(~0u, wait_bar<CG == 2>(ready(st), phase, abort_addr, a.status, 63));
                 if (!ok) break;
                 tc_fence_after();
                 if (elect_one()) {
@@ -382,18 +392,6 @@ fp4_tile_kernel(const __grid_constant__ CUtensorMap mapB, const __grid_constant_
                 if (CG == 1) mbar_arrive(acc_full(buf));
             }
             __syncwarp();
-        }
-    } else if (warp == 3 && rank == 1) {
-        // Tells the first CTA what has arrived here.
-        bool ok = true;
-        uint32_t st = 0, phase = 0;
-        while (ok && walk.next(s)) {
-            for (int k = s.k0; k < s.k1; k++) {
-                ok = __all_sync(~0u, wait_bar(full(st), phase, abort_addr, a.status, 66));
-                if (!ok) break;
-                if (lane == 0) arrive_at_first(ready(st));
-                if (++st == S) { st = 0; phase ^= 1; }
-            }
         }
     } else if (warp >= 12) {
         // Scales to tensor memory, as soon as the MMAs have used what is there: four words a lane and scale tile, the same in all lane
@@ -756,7 +754,7 @@ bool make_schedule(const int* gsp, int groups, int units, int sms, Schedule& s) 
 }
 
 template <int NT, int FMT>
-int launch_tile(const TileArgs& args, const CUtensorMap& map, const int* gsp, int groups, const DeviceCtx* ctx, cudaStream_t stream) {
+int launch_tile(const TileArgs& args, const CUtensorMap& mapA, const CUtensorMap& map, const int* gsp, int groups, const DeviceCtx* ctx, cudaStream_t stream) {
     using G = Cfg<NT>;
     TileArgs a = args;
     SMAT_CUDA_TRY(cudaFuncSetAttribute(fp4_tile_kernel<NT, FMT>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM));
@@ -779,7 +777,7 @@ int launch_tile(const TileArgs& args, const CUtensorMap& map, const int* gsp, in
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, fp4_tile_kernel<NT, FMT>, map, a, s);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, fp4_tile_kernel<NT, FMT>, mapA, map, a, s);
     count_launch();
     if (e == cudaSuccess && cut) {
         Joins joins;
@@ -795,9 +793,9 @@ int launch_tile(const TileArgs& args, const CUtensorMap& map, const int* gsp, in
 }
 
 template <int NT>
-int launch_tile_format(int fmt, const TileArgs& a, const CUtensorMap& map, const int* gsp, int groups, const DeviceCtx* ctx, cudaStream_t stream) {
-    return fmt == SMAT_FP4_NV ? launch_tile<NT, SMAT_FP4_NV>(a, map, gsp, groups, ctx, stream)
-                              : launch_tile<NT, SMAT_FP4_MX>(a, map, gsp, groups, ctx, stream);
+int launch_tile_format(int fmt, const TileArgs& a, const CUtensorMap& mapA, const CUtensorMap& map, const int* gsp, int groups, const DeviceCtx* ctx, cudaStream_t stream) {
+    return fmt == SMAT_FP4_NV ? launch_tile<NT, SMAT_FP4_NV>(a, mapA, map, gsp, groups, ctx, stream)
+                              : launch_tile<NT, SMAT_FP4_MX>(a, mapA, map, gsp, groups, ctx, stream);
 }
 
 }  // namespace
@@ -806,9 +804,13 @@ int launch_fp4_tile(const Fp4View& A, const Fp4Rhs& B, void* C, int c_dtype, siz
     DeviceCtx* ctx = nullptr;
     if (int rc = get_device_ctx(&ctx)) return rc;
     const int nt = N <= 32 ? 32 : N <= 64 ? 64 : N <= 128 ? 128 : 256;
-    CUtensorMap map;
+    CUtensorMap map, mapA = {};
     const size_t pitch = fp4_pitch(A.K);
-    if (int rc = encode_tensor_map_2d_u8(&map, B.data, pitch, N, pitch, 128, (uint32_t)std::min(nt, 128))) return rc;
+    if (int rc = encode_tensor_map_2d_u8(&map, B.data, pitch, N, pitch, 128, (uint32_t)std::min(nt, 128), 128)) return rc;
+    if (nt == 256) {  // pairs: A's tiles as rows of 128 bytes, 128 of codes and 16 of scales each, which lie in the order of shared memory
+        constexpr uint32_t rows = kFp4TileBytes / 128;
+        if (int rc = encode_tensor_map_2d_u8(&mapA, A.tiles, 128, A.total_steps * 2 * rows, 128, 128, kFp4TileCodes / 128, 0)) return rc;
+    }
     TileArgs a = {};
     a.steps = A.steps;
     a.tiles = A.tiles;
@@ -826,10 +828,10 @@ int launch_fp4_tile(const Fp4View& A, const Fp4Rhs& B, void* C, int c_dtype, siz
     a.b_row_tiles = (int)((N + 127) / 128);
     const int groups = (int)((A.block_rows + kFp4GroupRows - 1) / kFp4GroupRows);
     switch (nt) {
-        case 32: return launch_tile_format<32>(A.fmt, a, map, A.h_gsp, groups, ctx, stream);
-        case 64: return launch_tile_format<64>(A.fmt, a, map, A.h_gsp, groups, ctx, stream);
-        case 128: return launch_tile_format<128>(A.fmt, a, map, A.h_gsp, groups, ctx, stream);
-        default: return launch_tile_format<256>(A.fmt, a, map, A.h_gsp, groups, ctx, stream);
+        case 32: return launch_tile_format<32>(A.fmt, a, mapA, map, A.h_gsp, groups, ctx, stream);
+        case 64: return launch_tile_format<64>(A.fmt, a, mapA, map, A.h_gsp, groups, ctx, stream);
+        case 128: return launch_tile_format<128>(A.fmt, a, mapA, map, A.h_gsp, groups, ctx, stream);
+        default: return launch_tile_format<256>(A.fmt, a, mapA, map, A.h_gsp, groups, ctx, stream);
     }
 }
 

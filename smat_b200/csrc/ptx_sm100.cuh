@@ -66,11 +66,37 @@ __device__ __forceinline__ bool mbar_try_wait_suspend(uint32_t bar, uint32_t par
     return ok != 0;
 }
 
+// The same with an acquire at the scope of the cluster: for a phase that another CTA's arrival completes.
+__device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t parity, uint32_t hint_ns) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(hint_ns)
+        : "memory");
+    return ok != 0;
+}
+
 // ---- TMA tiled 2-D load (global -> this CTA's shared memory), completion on an mbarrier -------
 __device__ __forceinline__ void tma_load_2d(uint32_t dst_smem, const CUtensorMap* map, int x, int y, uint32_t bar) {
     asm volatile(
         "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
         ::"r"(dst_smem), "l"(map), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+// The same from a CTA of a pair (cta_group::2), completing on a barrier of either CTA: `bar_cluster` is its address in the shared memory
+// of the cluster (pair_bar), the data lands in this CTA.  What completes the copy releases it at the scope of the cluster.
+__device__ __forceinline__ uint32_t pair_bar(uint32_t bar, uint32_t rank) {
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(bar), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst_smem, const CUtensorMap* map, int x, int y, uint32_t bar_cluster) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+        ::"r"(dst_smem), "l"(map), "r"(x), "r"(y), "r"(bar_cluster)
         : "memory");
 }
 // Tiled 2D bulk store shared -> global of the box the tensor map describes, at element coordinates (x, y); x * element

@@ -80,9 +80,8 @@ constexpr int kOrderWindow = 16384;
 // cuTensorMapEncodeTiled through the runtime's driver entry point lookup (no link against libcuda).
 int encode_tensor_map_2d_f16(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint64_t row_pitch_bytes,
                              uint32_t box_inner, uint32_t box_outer, int swizzle_bytes, int l2_promo_bytes);
-// Bytes with a 128-byte swizzle.
 int encode_tensor_map_2d_u8(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint64_t row_pitch_bytes, uint32_t box_inner,
-                            uint32_t box_outer);
+                            uint32_t box_outer, int swizzle_bytes);
 
 // Most block-rows per work item of the SpMM kernel (one accumulator each).  A plan is built for groups of
 // `rg` <= kPlanRowsPerGroup block-rows: small matrices / shards use smaller groups to fill the SMs.

@@ -37,13 +37,15 @@ static __device__ unsigned long long g_wait_prof[64];
 #endif
 
 // Bounded mbarrier wait; false: given up.  After the first time-out anywhere in the CTA every wait returns at once.
+// CLUSTER: what other CTAs of the cluster wrote to shared memory before their (releasing) arrivals is seen after the wait.
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, uint32_t abort_addr, int* status, int code,
                                          long long limit = kWaitCycles) {
-    if (mbar_try_wait(bar, parity)) return true;
+    if (CLUSTER ? mbar_try_wait_cluster(bar, parity, 0u) : mbar_try_wait(bar, parity)) return true;
     if (ld_shared_u32(abort_addr)) return false;
     const long long t0 = clock64();
     // suspended waits: the warp sleeps in hardware until the phase completes or ~2 us pass
-    while (!mbar_try_wait_suspend(bar, parity, 2000u)) {
+    while (!(CLUSTER ? mbar_try_wait_cluster(bar, parity, 2000u) : mbar_try_wait_suspend(bar, parity, 2000u))) {
         if (ld_shared_u32(abort_addr)) return false;
         if (clock64() - t0 > limit) {
             st_shared_u32(abort_addr, 1);
