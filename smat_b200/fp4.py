@@ -110,11 +110,18 @@ class Fp4Matrix:
         # One piece of memory; the tensors in it are made when they are asked for (a microsecond each).
         self._scales_at = at = (N * quads * 32 + 15) // 16 * 16
         self._row_at = end = at + (N + 127) // 128 * quads * 512
-        self._memory = m = torch.empty(end + (4 * N if fmt == "nvfp4" else 0), dtype=torch.uint8, device=device)
+        self._memory = torch.empty(end + (4 * N if fmt == "nvfp4" else 0), dtype=torch.uint8, device=device)
         self._codes = self._scales = self._row = None
-        self._own = True  # the addresses below are those of the memory
-        p = m.data_ptr()
-        self._at = (p, p + at, p + end if fmt == "nvfp4" else None)
+        self._has_row = fmt == "nvfp4"
+
+    @property
+    def _at(self):
+        """Addresses of codes, scales and row scales (None: there are none)."""
+        p = self._memory.data_ptr()
+        return p, p + self._scales_at, p + self._row_at if self._has_row else None
+
+    def __getstate__(self):  # of a copy: the tensors in its memory are made again, as parts of its own
+        return {**self.__dict__, "_codes": None, "_scales": None, "_row": None}
 
     @property
     def device(self):
@@ -134,17 +141,16 @@ class Fp4Matrix:
 
     @property
     def row_scale(self):
-        if self._row is None and self._at[2] is not None and self._own:
+        if self._row is None and self._has_row:
             self._row = self._memory[self._row_at:].view(torch.float32)
         return self._row
 
     @row_scale.setter
     def row_scale(self, value):
         t = _row_scales(value, self.fmt, self.N, self.device)
-        self._row, self._own = None, t is not None
-        if self._own:  # a copy: quantize(out=...) writes to it later
+        self._row, self._has_row = None, t is not None
+        if self._has_row:  # a copy: quantize(out=...) writes to it later
             self._memory[self._row_at:].view(torch.float32).copy_(t)
-        self._at = (self._at[0], self._at[1], self._memory.data_ptr() + self._row_at if self._own else None)
 
     @classmethod
     def quantize(cls, X, fmt="nvfp4", out=None):
@@ -161,7 +167,7 @@ class Fp4Matrix:
             out = cls(N, K, fmt, x.device)
         elif (out.N, out.K, out.fmt, out.device) != (N, K, fmt, x.device):
             _refuse("out has another size, format or device")
-        elif f == 0 and out._at[2] is None:
+        elif f == 0 and not out._has_row:
             _refuse("out has no row scales")
         codes, scales, row = out._at
         rc = (_LIB or _lib()).smat_fp4_quantize(x.data_ptr(), d, N, K, x.stride(0) if N > 1 else K, f, codes, scales, row, api._stream())

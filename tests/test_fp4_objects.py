@@ -1,0 +1,44 @@
+"""Objects for matrices in 4 bits on the host: copies, what from_codes takes, and arrays that do not fit."""
+import copy
+import io
+import pickle
+
+import numpy as np
+import pytest
+import torch
+
+import fp4_oracle as F
+import smat_b200 as S
+
+
+def _matrix(N=5, K=80, fmt="nvfp4"):
+    rng = np.random.default_rng(N + K)
+    codes = rng.integers(0, 16, (N, K)).astype(np.uint8)
+    s = rng.integers(1, 120, (N, -(-K // F.GROUP[fmt]))).astype(np.uint8)
+    row = rng.random(N).astype(np.float32) if fmt == "nvfp4" else None
+    return S.Fp4Matrix.from_codes(torch.from_numpy(F.pack(codes)), torch.from_numpy(s), K, fmt, row, device="cpu")
+
+
+def _saved(q):
+    f = io.BytesIO()
+    torch.save(q, f)
+    f.seek(0)
+    return torch.load(f, weights_only=False)
+
+
+@pytest.mark.parametrize("how", [copy.deepcopy, lambda q: pickle.loads(pickle.dumps(q)), _saved])
+@pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
+def test_copies_have_their_own_memory(how, fmt):
+    """What a copy hands to the kernels are its own arrays, and they are the ones that it shows."""
+    q = _matrix(fmt=fmt)
+    want = [t.clone() for t in (q.codes, q.scales)] + [None if q.row_scale is None else q.row_scale.clone()]
+    c = how(q)
+    q.codes.zero_()
+    q.scales.zero_()
+    for t, w, at in zip((c.codes, c.scales, c.row_scale), want, c._at):
+        assert (t is None and w is None and at is None) or (torch.equal(t, w) and t.data_ptr() == at)
+    c.codes.fill_(7)
+    assert c._at[0] == c.codes.data_ptr() and int(q.codes.max()) == 0
+    if fmt == "nvfp4":
+        c.row_scale = None
+        assert c._at[2] is None and c.row_scale is None and q._at[2] is not None and how(c).row_scale is None
