@@ -182,7 +182,8 @@ enum { SMAT_F16 = 0, SMAT_BF16 = 1, SMAT_F32 = 2 };
 size_t smat_fp4_codes_bytes(size_t N, size_t K);
 size_t smat_fp4_scales_bytes(size_t N, size_t K);
 /* X [N][K] of fp16, bf16 or fp32, rows `ldx` elements apart (a multiple of 16 bytes), to 4 bits and back; one launch each, asynchronous
- * on `stream`.  Values on the way back are code * scale * row_scale in fp32, rounded once. */
+ * on `stream`.  Values on the way back are code * scale, which is exact, times row_scale, rounded to fp32 and from there to their
+ * type (with a row scale that is a power of two, like those computed here, the first rounding changes nothing that fp32 can hold). */
 int smat_fp4_quantize(const void* X, int dtype, size_t N, size_t K, size_t ldx, int fmt, void* codes, void* scales, float* row_scale,
                       void* stream);
 int smat_fp4_dequantize(const void* codes, const void* scales, const float* row_scale, int fmt, size_t N, size_t K, void* Y, int dtype,

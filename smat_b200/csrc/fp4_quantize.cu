@@ -82,9 +82,10 @@ __device__ __forceinline__ uint2 quantize16(const Raw<DT>& raw, float gmax, bool
     return make_uint2(f32x8_to_e2m1(q), f32x8_to_e2m1(q + 8));
 }
 // Eight codes to values: half a group a lane, so that a warp's 16-byte stores lie side by side (a group a lane, each store filled half
-// of 32 sectors: 72 us instead of 50 for 4096 x 28672 bf16).
-template <int DT>
-__device__ __forceinline__ void dequantize8(uint32_t c, float s, typename Elem<DT>::T* to) {
+// of 32 sectors: 72 us instead of 50 for 4096 x 28672 bf16).  Code times scale is exact; the row scale p, which may be any number, comes
+// last, so that fp32 rounds once and nothing overflows or ends at zero on the way.
+template <int FMT, int DT>
+__device__ __forceinline__ void dequantize8(uint32_t c, float s, float p, typename Elem<DT>::T* to) {
     uint32_t h[4];
     e2m1x8_to_f16(c, h);
     float v[8];
@@ -92,6 +93,7 @@ __device__ __forceinline__ void dequantize8(uint32_t c, float s, typename Elem<D
     for (int i = 0; i < 4; i++) {
         const float2 f = __half22float2(*reinterpret_cast<__half2*>(&h[i]));
         v[2 * i] = f.x * s; v[2 * i + 1] = f.y * s;
+        if constexpr (FMT == SMAT_FP4_NV) { v[2 * i] *= p; v[2 * i + 1] *= p; }
     }
     if constexpr (DT == SMAT_F32) {
         reinterpret_cast<float4*>(to)[0] = make_float4(v[0], v[1], v[2], v[3]);
@@ -196,7 +198,7 @@ __global__ void __launch_bounds__(kThreads) fp4_dequantize_kernel(const uint8_t*
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int j = j0 + u * threads;
-            if (j < halves) dequantize8<DT>(c[u], scale_value<FMT>(s[u]) * p, Y + r * ldy + (size_t)j * 8);
+            if (j < halves) dequantize8<FMT, DT>(c[u], scale_value<FMT>(s[u]), p, Y + r * ldy + (size_t)j * 8);
         }
     }
 }
@@ -293,7 +295,7 @@ __global__ void __launch_bounds__(kThreads) fp4_dequantize_blocks_kernel(const u
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int b = b0 + u * STEP;
-            if (b < range.y) dequantize8<DT>(c[u], scale_value<FMT>(s[u]) * p, vals + (size_t)b * 256 + lane * 8);
+            if (b < range.y) dequantize8<FMT, DT>(c[u], scale_value<FMT>(s[u]), p, vals + (size_t)b * 256 + lane * 8);
         }
     }
 }

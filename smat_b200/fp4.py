@@ -201,7 +201,8 @@ class Fp4Matrix:
         return s.reshape(self.N, -1)[:, :-(-self.K // _GROUP[self.fmt])].contiguous()
 
     def dequantize(self, dtype=torch.float16, out=None):
-        """The values as a tensor [N, K] in fp16, bf16 or fp32, rounded once; ``out``: a tensor to write to."""
+        """The values as a tensor [N, K] in fp16, bf16 or fp32; ``out``: a tensor to write to.  Code * scale is exact; times the row
+        scale it is rounded to fp32 (powers of two change nothing), then to the type."""
         d = _dtype(dtype if out is None else out.dtype)
         _on_current_device(self._memory)
         if out is None:
@@ -268,7 +269,7 @@ class Fp4SparseMatrix:
         return self
 
     def dequantize(self, check=False):
-        """A SparseMatrix of the values in fp16, rounded once; it shares the structure."""
+        """A SparseMatrix of the values in fp16, rounded as by Fp4Matrix.dequantize; it shares the structure."""
         _on_current_device(self.codes)
         A = SparseMatrix()
         A.M, A.K, A.nnzb = self.M, self.K, self.nnzb

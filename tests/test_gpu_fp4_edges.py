@@ -1,0 +1,45 @@
+"""Matrices in 4 bits where ranges, structures and host state end: scales next to both ends, inconsistent arrays, plans made on
+several threads, errors that must not outlive their call."""
+import numpy as np
+import pytest
+import torch
+
+import fp4_oracle as F
+import smat_b200 as S
+from test_gpu_fp4_spmm import HALF, LEAST, Case, _close
+
+pytestmark = pytest.mark.gpu
+
+
+def _case(fmt, counts, Kb, scales, seed=3):
+    """A Case whose scale bytes are `scales` [rows of all block-rows], the same for all blocks of a row."""
+    c = Case(seed, counts, Kb, fmt, row_scale=False)
+    brow = np.repeat(np.arange(len(counts)), counts)
+    c.scales = np.asarray(scales, np.uint8).reshape(-1, 16)[brow]
+    c.A = S.Fp4SparseMatrix.from_codes(c.M, c.K, c.rowptr, c.colidx, F.pack(c.codes), c.scales, fmt)
+    c.vals = F.block_values(c.codes, c.scales, None, c.rowptr, fmt)
+    return c
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+def test_row_scales_of_any_size(dtype):
+    """Values on the way back are code * scale, which is exact, times the row scale, rounded to fp32 and from there to their type:
+    nothing between overflows, loses digits or turns a zero into NaN."""
+    rng = np.random.default_rng(4)
+    N, K = 24, 64
+    codes = rng.integers(0, 16, (N, K)).astype(np.uint8)
+    s = rng.integers(1, 127, (N, K // 16)).astype(np.uint8)
+    s[:, 0] = 126  # 448
+    p = (rng.random(N) + 0.5).astype(np.float32)
+    p[:4] = [3e38, 1e37, 2e-38, 1e-39]
+    q = S.Fp4Matrix.from_codes(torch.from_numpy(F.pack(codes)), torch.from_numpy(s), K, "nvfp4", p)
+    exact = F.dense_values(codes, s, p, "nvfp4")
+    with np.errstate(over="ignore"):
+        want = torch.from_numpy(exact.astype(np.float32)).to(dtype)  # numpy rounds once to fp32, torch once to the type
+    assert torch.equal(q.dequantize(dtype).cpu(), want)
+    rowptr, colidx = np.array([0, 2], np.int32), np.array([0, 32], np.int32)
+    bc, bs = codes[:16].reshape(16, 4, 16)[:, :2].transpose(1, 0, 2), s[:16, :2].T
+    A = S.Fp4SparseMatrix.from_codes(16, 48, rowptr, colidx, F.pack(np.ascontiguousarray(bc)), np.ascontiguousarray(bs), "nvfp4", p[:16])
+    with np.errstate(over="ignore"):
+        want = torch.from_numpy(F.block_values(bc, bs, p[:16], rowptr, "nvfp4").astype(np.float32)).half()
+    assert torch.equal(A.dequantize(check=True).bcsrVal.cpu().view(2, 16, 16), want)
