@@ -56,9 +56,10 @@ __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
     }
 }
 // A pair of fp16 that came from e2m1 -> the same pair in bf16.  The magnitude shifted down by the three bits that the exponent field is
-// wider reads as the value times 2^-112 (0 stays 0, all others are normal); the factor 2^112 (0x7780) takes that back.
-__device__ __forceinline__ uint32_t f16_code_to_bf16(uint32_t h2) {
-    return mul2<SMAT_BF16>((h2 & 0x80008000u) | ((h2 & 0x7fff7fffu) >> 3), 0x77807780u);
+// wider reads as the value times 2^-112 (0 stays 0, all others are normal); the factor 2^112 (0x7780) takes that back, a smaller one
+// gives the pair times a power of two.
+__device__ __forceinline__ uint32_t f16_code_to_bf16(uint32_t h2, uint32_t factor = 0x77807780u) {
+    return mul2<SMAT_BF16>((h2 & 0x80008000u) | ((h2 & 0x7fff7fffu) >> 3), factor);
 }
 // Eight fp32 -> eight codes, to nearest, ties to even, saturating at 6 (no NaN comes here).
 __device__ __forceinline__ uint32_t f32x8_to_e2m1(const float* v) {

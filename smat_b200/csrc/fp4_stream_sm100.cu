@@ -3,7 +3,9 @@
 // Mathematics.  A block is 16 x 16 and a scale covers a whole row of it.  e2m1 times e4m3 has at most six significant bits and fits
 // fp16 and bf16, and e2m1 times 2^e fits bf16, so the scaled values go into m16n8k16 MMAs that accumulate in fp32, nothing rounded on
 // the way in.  Powers of two beyond the range of fp16 (SMAT_FP4_MX and fp16) and scales of B in 4 bits are applied to a block's product
-// instead, one fp32 FMA per element.
+// instead, one fp32 FMA per element.  Of SMAT_FP4_MX, where scales go up to 2^127, all sums are kept times a power of two that lets
+// nothing overflow on the way to a result that fp32 holds: values of A in bf16 are at most 6 * 2^127 (kept times 2^-3), a block's
+// product with a scale of B in 4 bits at most 16 * 36 * 2^127 (kept times 2^-12).  Downwards both stay exact.
 //
 // Layout.  Plans keep the blocks in fours in the order in which a warp's lanes take them (fp4_format.h): read as they are stored, a
 // word a lane and block, they cost twice the instructions.  MMA rows g and g + 8 stand for rows 2g and 2g + 1 of the block, the k
@@ -74,6 +76,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) fp4_stream_kerne
     const int r0 = (int)(blockIdx.x / cl % row_ctas) * rows_per_cta, r = r0 + warp / wr;
     const int n0 = (int)(blockIdx.x / cl / row_ctas) * NT * 8;
     const size_t quads = (a.K + 63) / 64;
+    constexpr bool DOWN = FMT == SMAT_FP4_MX && BT != SMAT_F16;                         // sums are kept times 1 / UP
+    constexpr float UP = !DOWN ? 1.f : BT == SMAT_BF16 ? 8.f : 4096.f;
     constexpr bool FOLD = BT == SMAT_BF16 || (BT == SMAT_F16 && FMT == SMAT_FP4_NV);  // scales go into the values of A
 
     float acc[NT][4];
@@ -138,10 +142,14 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) fp4_stream_kerne
                         both[1] = pack2<SMAT_BF16>(f.y, f.y);
                     }
 #pragma unroll
-                    for (int e = 0; e < 4; e++) am[e] = BT == SMAT_F16 ? mul2<SMAT_F16>(am[e], both[e % 2]) : mul2<SMAT_BF16>(f16_code_to_bf16(am[e]), both[e % 2]);
+                    for (int e = 0; e < 4; e++) am[e] = BT == SMAT_F16 ? mul2<SMAT_F16>(am[e], both[e % 2]) : mul2<SMAT_BF16>(f16_code_to_bf16(am[e], DOWN ? 0x76007600u : 0x77807780u), both[e % 2]);  // 2^109, 2^112
                 } else {
                     s0 = scale_value<FMT>(sc & 0xff);
                     s1 = scale_value<FMT>(sc >> 8);
+                    if constexpr (DOWN) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) am[e] = mul2<SMAT_F16>(am[e], 0x0c000c00u);  // 2^-12
+                    }
                 }
 #pragma unroll
                 for (int j = 0; j < NT; j++) {
@@ -224,6 +232,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) fp4_stream_kerne
                 for (int k = 0; k < wr; k++) v += part_sum[br * wr + k][row * ROW + c];
             }
             const size_t m = (size_t)gr * 16 + row;
+            if constexpr (DOWN) v *= UP;
             if (a.row_scale) v *= __ldg(a.row_scale + m);
             if (a.b_row_scale) v *= __ldg(a.b_row_scale + n0 + c);
             store_c(a.C, a.c_dtype, m * a.N + n0 + c, v);

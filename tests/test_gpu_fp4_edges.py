@@ -21,6 +21,48 @@ def _case(fmt, counts, Kb, scales, seed=3):
     return c
 
 
+@pytest.mark.parametrize("N", [5, 40, 150])
+@pytest.mark.parametrize("tiles", [False, True])
+@pytest.mark.parametrize("swap", [False, True])
+def test_e8m0_from_end_to_end(N, tiles, swap):
+    """mxfp4 scales over their whole range on one side, all of the reverse size on the other: the products are of ordinary size and
+    so are all sums, in every kernel.  swap: the rows of A get one scale, the tokens theirs."""
+    rng = np.random.default_rng(N)
+    Kb = 24
+    byte = np.concatenate([[0, 1, 2, 3, 4, 5, 249, 250, 251, 252, 253, 254], rng.integers(6, 249, 20)])
+    rows, tokens = byte, np.resize(byte, N)
+    for other in (1, 60, 127, 190, 254):
+        a, t = (rows, np.full(N, other)) if not swap else (np.full(32, other), tokens)
+        c = _case("mxfp4", [20, 24], Kb, a)
+        codes = rng.integers(0, 16, (N, c.K)).astype(np.uint8)
+        s = np.repeat(t.astype(np.uint8)[:, None], Kb // 2, 1)
+        B = S.Fp4Matrix.from_codes(torch.from_numpy(F.pack(codes)), torch.from_numpy(s), c.K, "mxfp4")
+        ref, mag = F.multiply(c.vals, c.rowptr, c.colidx, F.dense_values(codes, s, None, "mxfp4"))
+        C = torch.full((c.M, N), float("nan"), dtype=torch.bfloat16, device="cuda")
+        S.Fp4Plan(c.A, tiles=tiles).spmm(B, C, check=True)
+        got = C.double().cpu().numpy()
+        fine = (mag < 2.0 ** 127) & (mag > 2.0 ** -100)  # sums that fp32 holds with all their digits
+        tol = (c.longest + 32) * 2.0 ** -22 * mag + HALF[C.dtype] * np.abs(ref) * (1 + 1e-3) + LEAST[C.dtype]
+        assert np.all(np.abs(got - ref)[fine] <= tol[fine]), (other, np.argwhere(fine & ~(np.abs(got - ref) <= tol))[:5].tolist())
+
+
+@pytest.mark.parametrize("N", [1, 5, 40, 100])
+def test_e8m0_of_weights_with_bf16(N):
+    """The same with activations in bf16."""
+    rng = np.random.default_rng(N)
+    byte = np.concatenate([[0, 1, 2, 3, 4, 5, 249, 250, 251, 252, 253, 254], rng.integers(6, 249, 20)])
+    c = _case("mxfp4", [20, 24], 24, byte)
+    for size in (-120, -60, 0, 60, 120):
+        x = torch.from_numpy(rng.standard_normal((N, c.K)) * 2.0 ** size).bfloat16().cuda()
+        ref, mag = F.multiply(c.vals, c.rowptr, c.colidx, x.double().cpu().numpy())
+        C = torch.full((c.M, N), float("nan"), dtype=torch.bfloat16, device="cuda")
+        S.Fp4Plan(c.A).spmm(x, C, check=True)
+        got = C.double().cpu().numpy()
+        fine = (mag < 2.0 ** 127) & (mag > 2.0 ** -100)
+        tol = (c.longest + 32) * 2.0 ** -22 * mag + HALF[C.dtype] * np.abs(ref) * (1 + 1e-3) + LEAST[C.dtype]
+        assert np.all(np.abs(got - ref)[fine] <= tol[fine]), size
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
 def test_row_scales_of_any_size(dtype):
     """Values on the way back are code * scale, which is exact, times the row scale, rounded to fp32 and from there to their type:
