@@ -133,7 +133,7 @@ int smat_spmm_set_variant(int variant);
  * device recorded a device-side error: a bounded wait that ran out (SMAT_ERR_DEVICE_WAIT), or BCSR
  * arrays found inconsistent while a plan was built or by a product without one -- row pointers of the
  * range that end before they begin, are negative or exceed nonzeroBlocks, a block column outside the
- * matrix, or block columns out of order (SMAT_ERR_RANGE; such input gets an empty or partial plan or
+ * matrix, block columns out of order, or different scales in a pair of mxfp4 blocks (SMAT_ERR_RANGE; such input gets an empty or partial plan or
  * product instead of an out-of-bounds access).  Order is looked at window by window of 16384
  * block-columns: a block must not lie in an earlier window than the one before it in its block-row;
  * inside a window the order does not show in the product and is not reported.  Clears the device status
@@ -173,7 +173,7 @@ int smat_selftest_plan_wait_timeout(const smat_plan* plan, const void* B, void* 
  *   row_scale  float[N] (SMAT_FP4_NV; may be NULL where it is read: ones)
  * and a block matrix, beside rowptr and colidx as above,
  *   codes   128 bytes a block (16 rows of 8), scales 16 bytes a block (one for each row), row_scale float[M].
- *   Of SMAT_FP4_MX, the blocks of an aligned pair of block-columns (columns 32 c to 32 c + 31) have equal scales.
+ *   Of SMAT_FP4_MX, the blocks of an aligned pair of block-columns (columns 32 c to 32 c + 31) have equal scales, if both are stored.
  * All arrays 16-byte aligned in device memory; K a multiple of 16 below 2^30, N below 2^31. */
 enum { SMAT_FP4_NV = 0, SMAT_FP4_MX = 1 };
 /* Element types of values. */
@@ -196,8 +196,8 @@ int smat_fp4_dequantize_blocks(const void* codes, const void* scales, const floa
                                size_t nonzeroBlocks, void* vals, int dtype, void* stream);
 
 /* Plan for products of block-rows [brow_begin, brow_end) of a block matrix in 4 bits.  It looks the arrays over (block columns in
- * strictly ascending order, multiples of 16 inside the matrix; inconsistent block-rows count as empty and are reported by
- * smat_device_status), keeps the pointers it was given and holds the blocks in the order of the kernel for few columns (148 bytes
+ * strictly ascending order, multiples of 16 inside the matrix, equal scales in the blocks of a pair of SMAT_FP4_MX, which
+ * smat_fp4_plan_set_values looks over again; inconsistent block-rows count as empty and are reported by smat_device_status), keeps the pointers it was given and holds the blocks in the order of the kernel for few columns (148 bytes
  * each).  with_tiles: it also holds them laid out for products with B in 4 bits, 36 KB for every 256 rows x 256 columns that hold a
  * block, unless they hold fewer than 4 on average; without, such products work but are slow.  After codes or scales changed (same
  * structure) call smat_fp4_plan_set_values.  Nothing in a plan is written by a product, so any number of streams may use it at a

@@ -250,6 +250,7 @@ int smat_device_status(void* stream) {
     if (st >= 100)
         return fail(SMAT_ERR_RANGE, "the BCSR arrays are inconsistent (device check %d: %s); the output is invalid", st,
                     st == kStatusBadRowptr ? "bcsrRowPtr disagrees with nonzeroBlocks"
+                    : st == kStatusBadScales ? "blocks of an aligned pair of block-columns have different mxfp4 scales"
                                            : "a block column is out of range or a block-row's columns are not ascending");
     if (st != 0) return fail(SMAT_ERR_DEVICE_WAIT, "a kernel gave up a bounded wait (site code %d); its output is invalid", st);
     return SMAT_OK;

@@ -32,6 +32,7 @@ constexpr uint32_t kFp4TileCodes = 16384, kFp4TileBytes = kFp4TileCodes + 2048;
 // A step is one word: bits [8, 32) say that its columns begin at 256 times that number (K below 2^26), bit 4 h + q that half h of the
 // group has blocks in columns 64 q to 64 q + 63 of them.
 struct Fp4Where {         // of what the tiles of a step are made
+    int group;            // whose step it is
     int begin[16];        // first block of each block-row in these columns
     uint16_t blocks[16];  // bit c: the block-row has a block in columns 16 c to 16 c + 15 of these
 };

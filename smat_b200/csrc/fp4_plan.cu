@@ -58,13 +58,28 @@ __global__ void __launch_bounds__(kThreads) fp4_ranges_kernel(const int* __restr
     }
 }
 
-// Fours of a block-row (a CTA a block-row, a warp a four); `first` is scanned.
+// Fours of a block-row (a CTA a block-row, a warp a four); `first` is scanned.  Of SMAT_FP4_MX, a block-row in which the blocks of a
+// pair have different scales is left out (empty) and reported: an MMA takes one scale for both.
+template <int FMT>
 __global__ void __launch_bounds__(kThreads) fp4_fours_kernel(const int2* __restrict__ range, const int* __restrict__ first, const int* __restrict__ colidx,
                                                              const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
-                                                             Fp4Row* __restrict__ rows, uint8_t* __restrict__ fours) {
+                                                             Fp4Row* __restrict__ rows, uint8_t* __restrict__ fours, int* status) {
     const int2 mine = range[blockIdx.x];
     const int f0 = first[blockIdx.x], lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
-    if (threadIdx.x == 0) rows[blockIdx.x] = {f0, mine.y - mine.x};
+    bool wrong = false;
+    if constexpr (FMT == SMAT_FP4_MX) {
+        for (int p = mine.x + (int)threadIdx.x; p + 1 < mine.y; p += kThreads) {
+            const int c = __ldg(colidx + p);
+            if (c & 16 || __ldg(colidx + p + 1) != c + 16) continue;
+            const uint4 x = __ldg(reinterpret_cast<const uint4*>(scales) + p), y = __ldg(reinterpret_cast<const uint4*>(scales) + p + 1);
+            wrong |= x.x != y.x || x.y != y.y || x.z != y.z || x.w != y.w;
+        }
+        wrong = __syncthreads_or(wrong);
+    }
+    if (threadIdx.x == 0) {
+        rows[blockIdx.x] = {f0, wrong ? 0 : mine.y - mine.x};
+        if (wrong) atomicCAS(status, 0, kStatusBadScales);
+    }
     for (int f = threadIdx.x / 32; f * 4 < mine.y - mine.x; f += kThreads / 32) {
         uint8_t* const to = fours + (size_t)(f0 + f) * kFp4FourBytes;
         uint32_t w[4];
@@ -131,19 +146,23 @@ __global__ void __launch_bounds__(kStepThreads) fp4_steps_kernel(const int2* __r
             mask |= 1u << (c >> 6 & 3);
         }
         const int at = first + (int)prefix[k >> 5] + __popc(bitmap[k >> 5] & ((1u << (k & 31)) - 1));
+        where[at].group = blockIdx.x;  // the same from all block-rows
         where[at].begin[e] = p;
         where[at].blocks[e] = (uint16_t)blocks;
         atomicOr(&steps[at], (uint32_t)k << 8 | mask << (e / 8 * 4));
     }
 }
 
-// Lays the blocks of a step out into its two tiles: a warp a block-row, a lane half a row (eight block-columns).
+// Lays the blocks of a step out into its two tiles: a warp a block-row, a lane half a row (eight block-columns).  Block-rows that `rows`
+// says to be empty are.
 template <int FMT>
 __global__ void __launch_bounds__(kStepThreads) fp4_tiles_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
-                                                                 const Fp4Where* __restrict__ where, uint8_t* __restrict__ tiles) {
+                                                                 const Fp4Row* __restrict__ rows, const Fp4Where* __restrict__ where,
+                                                                 uint8_t* __restrict__ tiles) {
     const uint32_t e = threadIdx.x / 32, lane = threadIdx.x % 32, r = lane & 15, h = lane >> 4;
     const Fp4Where& w = where[blockIdx.x];
-    const uint32_t blocks = w.blocks[e], mine = blocks >> (8 * h) & 0xff;
+    const bool left_out = w.blocks[e] && rows[w.group * (int)kFp4GroupRows + (int)e].blocks == 0;
+    const uint32_t blocks = left_out ? 0 : w.blocks[e], mine = blocks >> (8 * h) & 0xff;
     size_t p = (size_t)w.begin[e] + (h ? __popc(blocks & 0xff) : 0);
     uint2 v[8];
     uint32_t s[8];
@@ -171,17 +190,18 @@ __global__ void __launch_bounds__(kStepThreads) fp4_tiles_kernel(const uint8_t* 
 }
 
 // What a plan holds of codes and scales.
-int fill_values(const smat_fp4_plan* p, cudaStream_t stream) {
+int fill_values(const smat_fp4_plan* p, const DeviceCtx* ctx, cudaStream_t stream) {
     const Fp4View& v = p->v;
     if (!v.block_rows) return SMAT_OK;
-    fp4_fours_kernel<<<(unsigned)v.block_rows, kThreads, 0, stream>>>(p->range, p->four_first, v.colidx, v.codes, v.scales, p->rows,
-                                                                      static_cast<uint8_t*>(p->fours));
+    const auto fours = v.fmt == SMAT_FP4_NV ? fp4_fours_kernel<SMAT_FP4_NV> : fp4_fours_kernel<SMAT_FP4_MX>;
+    fours<<<(unsigned)v.block_rows, kThreads, 0, stream>>>(p->range, p->four_first, v.colidx, v.codes, v.scales, p->rows,
+                                                           static_cast<uint8_t*>(p->fours), ctx->d_status);
     count_launch();
     SMAT_CUDA_TRY(cudaGetLastError());
     if (!v.tiles || !v.blocks) return SMAT_OK;
     uint8_t* tiles = static_cast<uint8_t*>(p->tiles);
-    if (v.fmt == SMAT_FP4_NV) fp4_tiles_kernel<SMAT_FP4_NV><<<(unsigned)v.total_steps, kStepThreads, 0, stream>>>(v.codes, v.scales, p->where, tiles);
-    else fp4_tiles_kernel<SMAT_FP4_MX><<<(unsigned)v.total_steps, kStepThreads, 0, stream>>>(v.codes, v.scales, p->where, tiles);
+    const auto lay_out = v.fmt == SMAT_FP4_NV ? fp4_tiles_kernel<SMAT_FP4_NV> : fp4_tiles_kernel<SMAT_FP4_MX>;
+    lay_out<<<(unsigned)v.total_steps, kStepThreads, 0, stream>>>(v.codes, v.scales, p->rows, p->where, tiles);
     count_launch();
     SMAT_CUDA_TRY(cudaGetLastError());
     return SMAT_OK;
@@ -244,7 +264,7 @@ int build_plan(smat_fp4_plan* p, const int* rowptr, const int* colidx, size_t nn
         v.steps = step;
         v.tiles = static_cast<const uint8_t*>(p->tiles);
     }
-    if (int rc = fill_values(p, stream)) return rc;
+    if (int rc = fill_values(p, ctx, stream)) return rc;
     SMAT_CUDA_TRY(cudaStreamSynchronize(stream));
     return SMAT_OK;
 }
@@ -325,7 +345,9 @@ int smat_fp4_plan_set_values(smat_fp4_plan* plan, void* stream) {
     clear_error();
     if (!plan) return fail(SMAT_ERR_BAD_ARG, "plan is NULL");
     if (int rc = check_plan_device(plan)) return rc;
-    return fill_values(plan, (cudaStream_t)stream);
+    DeviceCtx* ctx = nullptr;
+    if (int rc = get_device_ctx(&ctx)) return rc;
+    return fill_values(plan, ctx, (cudaStream_t)stream);
 }
 
 int smat_fp4_plan_spmm(const smat_fp4_plan* plan, const void* B, int dtype, void* C, size_t N, void* stream) {

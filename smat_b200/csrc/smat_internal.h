@@ -68,11 +68,12 @@ int static_status_take(int* out);
 
 // Device status codes (the word kernels set): 1..99 a bounded wait ran out at that wait site; 100.. the input
 // structure is inconsistent (101: row pointers disagree with the number of blocks, 102: a block column is out of range
-// or the columns of a block-row are not ascending, see kOrderWindow).
+// or the columns of a block-row are not ascending, see kOrderWindow; 103: the blocks of a pair of mxfp4 have different scales).
 // Limit of a wait inside a kernel, in clock cycles: about two seconds; of the waits that a self-test lets run out, about 0.2 ms.
 constexpr long long kWaitCycles = 4000000000LL, kSelftestWaitCycles = 400000LL;
 constexpr int kStatusBadRowptr = 101;
 constexpr int kStatusBadColumns = 102;
+constexpr int kStatusBadScales = 103;
 // Most block-columns that the plan kernels look at together.  Inside such a window they sort for themselves, so the order of
 // a block-row's columns shows nowhere; a block in an earlier window than the block before it is refused, by every kernel.
 constexpr int kOrderWindow = 16384;

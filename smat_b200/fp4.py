@@ -253,7 +253,7 @@ class Fp4SparseMatrix:
     @classmethod
     def from_codes(cls, M, K, bcsr_rowptr, bcsr_colidx, codes, scales, fmt="nvfp4", row_scale=None, device="cuda"):
         """From arrays in 4 bits: codes uint8 [nnzb, 16, 8], scales 8-bit [nnzb, 16] (of mxfp4: equal for the two blocks of an
-        aligned pair), row_scale one number or [M]; rowptr and element columns as in SparseMatrix."""
+        aligned pair; products treat block-rows where they are not as empty and report it), row_scale one number or [M]; rowptr and element columns as in SparseMatrix."""
         _format(fmt)
         self = cls()
         self.M, self.K, self.nnzb, self.fmt = int(M), int(K), int(len(bcsr_colidx)), fmt

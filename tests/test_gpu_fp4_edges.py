@@ -85,3 +85,48 @@ def test_row_scales_of_any_size(dtype):
     with np.errstate(over="ignore"):
         want = torch.from_numpy(F.block_values(bc, bs, p[:16], rowptr, "nvfp4").astype(np.float32)).half()
     assert torch.equal(A.dequantize(check=True).bcsrVal.cpu().view(2, 16, 16), want)
+
+
+@pytest.mark.parametrize("N,tiles", [(3, True), (5, False), (40, True), (40, False), (150, True)])
+def test_pairs_with_different_scales_are_reported(N, tiles):
+    """mxfp4: blocks of a pair share their scales; a block-row where they do not counts as empty, in every kernel."""
+    c = Case(21, [16, 16, 16], 16, "mxfp4")
+    x, (B, b) = c.acts(N, torch.float16), c.acts4(N)
+    ref4, mag4 = F.multiply(c.vals, c.rowptr, c.colidx, b)
+    ref16, mag16 = F.multiply(c.vals, c.rowptr, c.colidx, x.double().cpu().numpy())
+    good = c.A.scales.clone()
+    C = torch.empty((c.M, N), dtype=torch.float16, device="cuda")
+    plan = S.Fp4Plan(c.A, tiles=tiles)
+    for made_anew in (True, False):
+        c.A.scales.copy_(good)
+        c.A.scales[16 + 7, 3] ^= 1
+        if made_anew:
+            plan = S.Fp4Plan(c.A, tiles=tiles)
+        else:
+            plan.set_values()
+        with pytest.raises(S.SmatError) as e:
+            plan.spmm(x, C, check=True)
+        assert e.value.code == -6
+        for right, ref, mag in ((x, ref16, mag16), (B, ref4, mag4)):
+            C.fill_(float("nan"))
+            plan.spmm(right, C, check=True)  # reported once
+            assert bool((C[16:32] == 0).all())
+            for lo in (0, 32):
+                _close(C[lo:lo + 16], ref[lo:lo + 16], mag[lo:lo + 16], 16)
+        c.A.scales.copy_(good)
+        plan.set_values()
+        for right, ref, mag in ((x, ref16, mag16), (B, ref4, mag4)):
+            plan.spmm(right, C, check=True)
+            _close(C, ref, mag, 16)
+
+
+def test_pairs_that_are_not_stored_together():
+    """One block of a pair alone, and neighbours of different pairs or block-rows, may have any scales."""
+    rowptr, colidx = np.array([0, 3, 5], np.int32), np.array([16, 32, 80, 64, 112], np.int32)
+    rng = np.random.default_rng(2)
+    codes, scales = rng.integers(0, 16, (5, 16, 16)).astype(np.uint8), np.repeat(np.arange(120, 125, dtype=np.uint8)[:, None], 16, 1)
+    A = S.Fp4SparseMatrix.from_codes(32, 128, rowptr, colidx, F.pack(codes), scales, "mxfp4")
+    x = torch.from_numpy(rng.standard_normal((3, 128))).half().cuda()
+    C = torch.empty((32, 3), dtype=torch.float16, device="cuda")
+    S.Fp4Plan(A).spmm(x, C, check=True)
+    _close(C, *F.multiply(F.block_values(codes, scales, None, rowptr, "mxfp4"), rowptr, colidx, x.double().cpu().numpy()), 3)
