@@ -289,8 +289,9 @@ int check_plan_device(const smat_fp4_plan* plan) {
 }
 
 int check_product(const smat_fp4_plan* plan, const void* B, const void* C, int c_dtype, size_t N) {
+    // The kernels count columns in 32 bits and add offsets of up to two tiles of 256 to the first column of the last tile.
+    if (N >= ((size_t)1 << 31) - 512) return fail(SMAT_ERR_RANGE, "N (%zu) beyond 2^31 - 513", N);
     if (!plan) return fail(SMAT_ERR_BAD_ARG, "plan is NULL");
-    if (N >= ((size_t)1 << 31)) return fail(SMAT_ERR_RANGE, "N beyond 2^31");
     if (c_dtype != SMAT_F16 && c_dtype != SMAT_BF16) return fail(SMAT_ERR_BAD_ARG, "C must be fp16 or bf16");
     if (plan->v.block_rows && N && (!C || (plan->v.K && !B))) return fail(SMAT_ERR_BAD_ARG, "B or C is NULL");
     if (((uintptr_t)B | (uintptr_t)C) & 15) return fail(SMAT_ERR_BAD_ARG, "B and C must be 16-byte aligned");
@@ -315,7 +316,7 @@ int smat_fp4_plan_create(smat_fp4_plan** out, const void* codes, const void* sca
     if (((uintptr_t)codes | (uintptr_t)scales) & 15) return fail(SMAT_ERR_BAD_ARG, "codes and scales must be 16-byte aligned");
     if (brow_begin > brow_end || brow_end > M / 16)
         return fail(SMAT_ERR_BAD_ARG, "block-row range [%zu, %zu) outside [0, %zu]", brow_begin, brow_end, M / 16);
-    if (nnzb * 16 >= ((size_t)1 << 31) || K >= ((size_t)1 << 31) || M / 16 >= ((size_t)1 << 31)) return fail(SMAT_ERR_RANGE, "size beyond 2^31");
+    if (nnzb * 16 >= ((size_t)1 << 31) || M / 16 >= ((size_t)1 << 30)) return fail(SMAT_ERR_RANGE, "nonzeroBlocks beyond 2^27 - 1 or M beyond 2^34 - 16");
     if (K >= ((size_t)1 << 26)) return fail(SMAT_ERR_RANGE, "K (%zu) beyond 2^26 - 1", K);  // a bitmap of steps in shared memory
     DeviceCtx* ctx = nullptr;
     if (int rc = get_device_ctx(&ctx)) return rc;

@@ -1,5 +1,6 @@
 """Objects for matrices in 4 bits on the host: copies, what from_codes takes, and arrays that do not fit."""
 import copy
+import ctypes as C
 import io
 import pickle
 
@@ -42,3 +43,16 @@ def test_copies_have_their_own_memory(how, fmt):
     if fmt == "nvfp4":
         c.row_scale = None
         assert c._at[2] is None and c.row_scale is None and q._at[2] is not None and how(c).row_scale is None
+
+
+def test_sizes_next_to_the_index_range():
+    """Refused before anything is looked up: columns are counted in 32 bits, in tiles of up to 256 with offsets into them."""
+    L = S.fp4._lib()
+    P = 1 << 20  # an aligned address that no refused call touches
+    for N in (1 << 31, (1 << 31) - 1, (1 << 31) - 512):
+        assert L.smat_fp4_plan_spmm(None, P, 0, P, N, None) == -6
+        assert L.smat_fp4_plan_spmm_fp4(None, P, P, None, 0, P, 0, N, None) == -6
+    assert L.smat_fp4_plan_spmm(None, P, 0, P, (1 << 31) - 513, None) == -1  # no plan
+    h = C.c_void_p()
+    for M in (1 << 34, (1 << 35) - 16):
+        assert L.smat_fp4_plan_create(C.byref(h), P, P, None, 0, P, P, M, 64, 3, 0, M // 16, 1, None) == -6 and not h.value
