@@ -197,7 +197,8 @@ int smat_fp4_dequantize_blocks(const void* codes, const void* scales, const floa
 
 /* Plan for products of block-rows [brow_begin, brow_end) of a block matrix in 4 bits.  It looks the arrays over (block columns in
  * strictly ascending order, multiples of 16 inside the matrix, equal scales in the blocks of a pair of SMAT_FP4_MX, which
- * smat_fp4_plan_set_values looks over again; inconsistent block-rows count as empty and are reported by smat_device_status), keeps the pointers it was given and holds the blocks in the order of the kernel for few columns (148 bytes
+ * smat_fp4_plan_set_values looks over again; inconsistent block-rows, or all if some overlap, count as empty and are reported by
+ * smat_device_status), keeps the pointers it was given and holds the blocks in the order of the kernel for few columns (148 bytes
  * each).  with_tiles: it also holds them laid out for products with B in 4 bits, 36 KB for every 256 rows x 256 columns that hold a
  * block, unless they hold fewer than 4 on average; without, such products work but are slow.  After codes or scales changed (same
  * structure) call smat_fp4_plan_set_values.  Nothing in a plan is written by a product, so any number of streams may use it at a

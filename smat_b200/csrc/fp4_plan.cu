@@ -237,6 +237,14 @@ int build_plan(smat_fp4_plan* p, const int* rowptr, const int* colidx, size_t nn
     SMAT_CUDA_TRY(cudaMemcpyAsync(&h_fours, fours + v.block_rows, sizeof(int), cudaMemcpyDeviceToHost, stream));
     SMAT_CUDA_TRY(cudaMemcpyAsync(&h_steps, gsp + groups, sizeof(int), cudaMemcpyDeviceToHost, stream));
     SMAT_CUDA_TRY(cudaStreamSynchronize(stream));
+    if (h_totals[0] > nnzb) {
+        // Block-rows overlap, so row pointers run backwards somewhere, which is reported.  The 32-bit sums may have wrapped (16384 row
+        // pointers in turn 0 and 2^20 are enough), so nothing is laid out by them: all block-rows count as empty.
+        SMAT_CUDA_TRY(cudaMemsetAsync(p->buffer, 0, bytes, stream));
+        h_totals[0] = h_totals[1] = 0;
+        h_steps = h_fours = 0;
+        with_tiles = false;
+    }
     p->range = range;
     p->four_first = fours;
     v.rows = p->rows;

@@ -130,3 +130,22 @@ def test_pairs_that_are_not_stored_together():
     C = torch.empty((32, 3), dtype=torch.float16, device="cuda")
     S.Fp4Plan(A).spmm(x, C, check=True)
     _close(C, *F.multiply(F.block_values(codes, scales, None, rowptr, "mxfp4"), rowptr, colidx, x.double().cpu().numpy()), 3)
+
+
+@pytest.mark.parametrize("rows,n", [(3, 5), (16385, 1 << 20)])
+def test_row_pointers_that_run_to_and_fro(rows, n):
+    """Block-rows over the same blocks again and again: more blocks in all than are stored, up to more than 32 bits count."""
+    K = n * 16
+    rowptr = (torch.arange(rows + 1, device="cuda", dtype=torch.int32) % 2 * n).int()
+    colidx = torch.arange(n, device="cuda", dtype=torch.int32) * 16
+    A = S.Fp4SparseMatrix.from_codes(rows * 16, K, rowptr, colidx, torch.full((n, 16, 8), 0x22, dtype=torch.uint8, device="cuda"),
+                                     torch.full((n, 16), 56, dtype=torch.uint8, device="cuda"))
+    x = torch.ones((3, K), dtype=torch.float16, device="cuda")
+    C = torch.full((rows * 16, 3), float("nan"), dtype=torch.float16, device="cuda")
+    plan = S.Fp4Plan(A)
+    with pytest.raises(S.SmatError) as e:
+        plan.spmm(x, C, check=True)
+    assert e.value.code == -6 and bool((C == 0).all())
+    C.fill_(float("nan"))
+    plan.spmm(S.Fp4Matrix.quantize(x), C, check=True)
+    assert bool((C == 0).all())
