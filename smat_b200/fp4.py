@@ -226,6 +226,32 @@ class Fp4SparseMatrix:
         self.M = self.K = self.nnzb = 0
         self.fmt = "nvfp4"
         self.bcsrRowPtr = self.bcsrColIdx = self.codes = self.scales = self.row_scale = None
+        self._checked = ()
+
+    def _arrays(self):
+        return self.codes, self.scales, self.row_scale, self.bcsrRowPtr, self.bcsrColIdx
+
+    def _check_arrays(self):
+        """Refuses arrays that are not what the kernels take them for.  Those that were looked over before are not again (0.4 instead of
+        4 us)."""
+        arrays, c = self._arrays(), self._checked
+        if c and arrays[0] is c[0] and arrays[1] is c[1] and arrays[2] is c[2] and arrays[3] is c[3] and arrays[4] is c[4]:
+            return
+        device = self.codes.device if isinstance(self.codes, torch.Tensor) else None
+        for name, t, dtype, least, most in (("codes", self.codes, torch.uint8, self.nnzb * 128, self.nnzb * 128),
+                                            ("scales", self.scales, torch.uint8, self.nnzb * 16, self.nnzb * 16),
+                                            ("row_scale", self.row_scale, torch.float32, self.M, self.M),
+                                            ("bcsrRowPtr", self.bcsrRowPtr, torch.int32, self.M // 16 + 1, self.M // 16 + 1),
+                                            ("bcsrColIdx", self.bcsrColIdx, torch.int32, self.nnzb, None)):
+            if name == "row_scale" and t is None:
+                continue
+            if name == "row_scale" and self.fmt != "nvfp4":
+                _refuse("row_scale: row scales go with nvfp4")
+            if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.numel() < least or (most is not None and t.numel() > most):
+                _refuse(f"{name}: {'at least ' if most is None else ''}{least} elements of {dtype} are expected")
+            if not t.is_contiguous() or t.device != device:
+                _refuse(f"{name}: it has to be contiguous and on {device}, like codes")
+        self._checked = arrays
 
     def _allocate(self):
         dev = self.bcsrRowPtr.device
@@ -237,11 +263,15 @@ class Fp4SparseMatrix:
     def quantize(cls, A, fmt="nvfp4", check=False):
         """The blocks of a SparseMatrix in 4 bits; the structure is shared with it."""
         f = _format(fmt)
-        _on_current_device(A.bcsrVal)
+        v, rp = A.bcsrVal, A.bcsrRowPtr
+        _on_current_device(v)
+        if v.numel() < A.nnzb * 256 or not v.is_contiguous() or rp.dtype != torch.int32 or rp.numel() != A.M // 16 + 1 or not rp.is_contiguous():
+            _refuse(f"a SparseMatrix with bcsrVal of {A.nnzb} blocks and int32 bcsrRowPtr of {A.M // 16 + 1}, contiguous, is expected")
         self = cls()
         self.M, self.K, self.nnzb, self.fmt = A.M, A.K, A.nnzb, fmt
         self.bcsrRowPtr, self.bcsrColIdx = A.bcsrRowPtr, A.bcsrColIdx
         self._allocate()
+        self._checked = self._arrays()
         rc = _lib().smat_fp4_quantize_blocks(A.bcsrVal.data_ptr(), _dtype(A.bcsrVal.dtype), A.bcsrRowPtr.data_ptr(), A.bcsrColIdx.data_ptr(),
                                              A.M, A.nnzb, f, self.codes.data_ptr(), self.scales.data_ptr(), _ptr(self.row_scale), api._stream())
         if rc:
@@ -270,6 +300,7 @@ class Fp4SparseMatrix:
 
     def dequantize(self, check=False):
         """A SparseMatrix of the values in fp16, rounded as by Fp4Matrix.dequantize; it shares the structure."""
+        self._check_arrays()
         _on_current_device(self.codes)
         A = SparseMatrix()
         A.M, A.K, A.nnzb = self.M, self.K, self.nnzb
@@ -294,6 +325,7 @@ class Fp4Plan:
         self.brow_begin = brow_begin
         self.brow_end = A.M // 16 if brow_end is None else brow_end
         self._h = None
+        A._check_arrays()
         _on_current_device(A.bcsrRowPtr)
         h = C.c_void_p()
         L = _lib()
@@ -301,19 +333,15 @@ class Fp4Plan:
                                       A.bcsrRowPtr.data_ptr(), A.bcsrColIdx.data_ptr(), A.M, A.K, A.nnzb, self.brow_begin,
                                       self.brow_end, int(tiles), api._stream()))
         self._h = h
-        self._arrays = self._arrays_of(A)  # the plan has their addresses
+        self._arrays = A._arrays()  # the plan has their addresses
         self._rows = (self.brow_end - self.brow_begin) * 16
         self._device = A.bcsrRowPtr.device
-
-    @staticmethod
-    def _arrays_of(A):
-        return (A.codes, A.scales, A.row_scale, A.bcsrRowPtr, A.bcsrColIdx)
 
     def set_values(self):
         """After A's codes or scales changed in place (same structure)."""
         if self._h is None:
             _refuse("the plan is closed")
-        if any(a is not b for a, b in zip(self._arrays, self._arrays_of(self.A))):
+        if any(a is not b for a, b in zip(self._arrays, self.A._arrays())):
             _refuse("A has other arrays than when the plan was made: change them in place, or make a new plan")
         _check(_LIB.smat_fp4_plan_set_values(self._h, api._stream()))
 

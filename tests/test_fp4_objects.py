@@ -56,3 +56,31 @@ def test_sizes_next_to_the_index_range():
     h = C.c_void_p()
     for M in (1 << 34, (1 << 35) - 16):
         assert L.smat_fp4_plan_create(C.byref(h), P, P, None, 0, P, P, M, 64, 3, 0, M // 16, 1, None) == -6 and not h.value
+
+
+def _sparse(fmt="nvfp4"):
+    rowptr, colidx = np.array([0, 2, 3], np.int32), np.array([0, 32, 16], np.int32)
+    return S.Fp4SparseMatrix.from_codes(32, 48, rowptr, colidx, torch.zeros((3, 16, 8), dtype=torch.uint8), torch.zeros((3, 16), dtype=torch.uint8),
+                                        fmt, np.ones(32, np.float32) if fmt == "nvfp4" else None, device="cpu")
+
+
+@pytest.mark.parametrize("use", [S.Fp4Plan, lambda A: A.dequantize()])
+def test_arrays_that_do_not_fit(use):
+    """Arrays put in the place of a matrix's own are looked over before their addresses go to a kernel."""
+    for name, value in (("row_scale", torch.ones(32, dtype=torch.float64)), ("row_scale", torch.ones(1).expand(32)), ("row_scale", torch.ones(16)),
+                        ("row_scale", np.ones(32, np.float32)),
+                        ("codes", torch.zeros((2, 16, 8), dtype=torch.uint8)), ("codes", torch.zeros((3, 16, 16), dtype=torch.uint8)[:, :, ::2]),
+                        ("scales", torch.zeros((3, 16), dtype=torch.int32)), ("scales", torch.zeros((16, 3), dtype=torch.uint8).T),
+                        ("bcsrRowPtr", torch.zeros(2, dtype=torch.int32)), ("bcsrRowPtr", torch.zeros(3, dtype=torch.int64)),
+                        ("bcsrColIdx", torch.zeros(2, dtype=torch.int32)), ("bcsrColIdx", torch.zeros(3, dtype=torch.int32, device="meta"))):
+        A = _sparse()
+        setattr(A, name, value)
+        with pytest.raises(S.SmatError, match=name) as e:
+            use(A)
+        assert e.value.code == -1
+    A = _sparse("mxfp4")
+    A.row_scale = torch.ones(32)
+    with pytest.raises(S.SmatError, match="row_scale"):
+        use(A)
+    with pytest.raises(S.SmatError, match="current CUDA device"):  # the arrays of from_codes are fine
+        use(_sparse())

@@ -149,3 +149,18 @@ def test_row_pointers_that_run_to_and_fro(rows, n):
     C.fill_(float("nan"))
     plan.spmm(S.Fp4Matrix.quantize(x), C, check=True)
     assert bool((C == 0).all())
+
+
+def test_sparse_matrix_whose_arrays_do_not_fit():
+    rowptr, colidx = np.array([0, 2, 3], np.int32), np.array([0, 32, 16], np.int32)
+    for name, spoil in (("bcsrVal", lambda t: t[:512]), ("bcsrVal", lambda t: torch.cat([t, t])[::2]), ("bcsrRowPtr", lambda t: t[:2]),
+                        ("bcsrRowPtr", lambda t: t.long())):
+        A = S.SparseMatrix.from_bcsr(32, 48, rowptr, colidx, np.ones(768, np.float16))
+        setattr(A, name, spoil(getattr(A, name)))
+        with pytest.raises(S.SmatError) as e:
+            S.Fp4SparseMatrix.quantize(A)
+        assert e.value.code == -1
+    A = S.SparseMatrix.from_bcsr(32, 48, rowptr, colidx, np.ones(768, np.float16))
+    A.bcsrVal = A.bcsrVal.bfloat16()  # other types of values are fine
+    # row scale 2^-11 (1 / 2688 lies above 2^-12), group scale 2^11 / 6 = 341.3 -> 352, code 2^11 / 352 = 5.8 -> 6: 6 * 352 * 2^-11
+    assert bool((S.Fp4SparseMatrix.quantize(A, check=True).dequantize().bcsrVal == 1.03125).all())
