@@ -99,6 +99,8 @@ __global__ void __launch_bounds__(kThreads) fp4_fours_kernel(const int2* __restr
 // The steps of a group (a CTA a group, a warp a block-row): a bitmap of the 256-column ranges that hold a block, counted (FILL false)
 // or turned into records.  Shared memory: `words` words of bitmap and, to fill, as many prefix counts.
 constexpr int kStepThreads = 32 * (int)kFp4GroupRows;
+constexpr size_t kFp4MostColumns = (size_t)1 << 26;  // K lies below
+constexpr int kStepWords = (int)(kFp4MostColumns / (32 * kFp4StepColumns));  // words of a bitmap, at most
 template <bool FILL>
 __global__ void __launch_bounds__(kStepThreads) fp4_steps_kernel(const int2* __restrict__ range, const int* __restrict__ colidx, int block_rows,
                                                                  int words, int* __restrict__ gsp, uint32_t* __restrict__ steps,
@@ -259,7 +261,8 @@ int build_plan(smat_fp4_plan* p, const int* rowptr, const int* colidx, size_t nn
         p->where = reinterpret_cast<Fp4Where*>(step + steps);
         SMAT_CUDA_TRY(cudaMalloc(&p->tiles, steps * 2 * kFp4TileBytes));
         SMAT_CUDA_TRY(cudaMemsetAsync(p->steps, 0, steps * (sizeof(uint32_t) + sizeof(Fp4Where)), stream));
-        SMAT_CUDA_TRY(cudaFuncSetAttribute(fp4_steps_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, words * 8));
+        // The limit is the function's on this device, not this launch's: one for all plans, which may be made by several threads.
+        SMAT_CUDA_TRY(cudaFuncSetAttribute(fp4_steps_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStepWords * 8));
         fp4_steps_kernel<true><<<(unsigned)groups, kStepThreads, words * 8, stream>>>(range, colidx, (int)v.block_rows, words, gsp, step, p->where);
         count_launch();
         SMAT_CUDA_TRY(cudaGetLastError());
@@ -325,7 +328,7 @@ int smat_fp4_plan_create(smat_fp4_plan** out, const void* codes, const void* sca
     if (brow_begin > brow_end || brow_end > M / 16)
         return fail(SMAT_ERR_BAD_ARG, "block-row range [%zu, %zu) outside [0, %zu]", brow_begin, brow_end, M / 16);
     if (nnzb * 16 >= ((size_t)1 << 31) || M / 16 >= ((size_t)1 << 30)) return fail(SMAT_ERR_RANGE, "nonzeroBlocks beyond 2^27 - 1 or M beyond 2^34 - 16");
-    if (K >= ((size_t)1 << 26)) return fail(SMAT_ERR_RANGE, "K (%zu) beyond 2^26 - 1", K);  // a bitmap of steps in shared memory
+    if (K >= kFp4MostColumns) return fail(SMAT_ERR_RANGE, "K (%zu) beyond 2^26 - 1", K);  // a bitmap of steps in shared memory
     DeviceCtx* ctx = nullptr;
     if (int rc = get_device_ctx(&ctx)) return rc;
     smat_fp4_plan* p = new (std::nothrow) smat_fp4_plan();

@@ -1,5 +1,7 @@
 """Matrices in 4 bits where ranges, structures and host state end: scales next to both ends, inconsistent arrays, plans made on
 several threads, errors that must not outlive their call."""
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -130,6 +132,30 @@ def test_pairs_that_are_not_stored_together():
     C = torch.empty((32, 3), dtype=torch.float16, device="cuda")
     S.Fp4Plan(A).spmm(x, C, check=True)
     _close(C, *F.multiply(F.block_values(codes, scales, None, rowptr, "mxfp4"), rowptr, colidx, x.double().cpu().numpy()), 3)
+
+
+def test_plans_made_on_several_threads():
+    """Layers of very different K: the shared memory that one creation asks for does not bound another's."""
+    Ks = [16 * 16, 16 * 512 * 64, 16 * 16 * 512 * 256 - 16]
+    made = []
+    for K in Ks:
+        rowptr, colidx = np.array([0, 8], np.int32), np.arange(8, dtype=np.int32) * 16
+        made.append(S.Fp4SparseMatrix.from_codes(16, K, rowptr, colidx, np.full((8, 16, 8), 0x22, np.uint8), np.full((8, 16), 56, np.uint8)))
+    errors = []
+
+    def work(A, stream):
+        try:
+            with torch.cuda.stream(stream):
+                for _ in range(300):
+                    S.Fp4Plan(A).close()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(A, torch.cuda.Stream())) for A in made * 2]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors[0]
 
 
 @pytest.mark.parametrize("rows,n", [(3, 5), (16385, 1 << 20)])
