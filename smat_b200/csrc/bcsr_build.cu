@@ -200,10 +200,13 @@ bcsr_fill_kernel(const int* __restrict__ rowptr, const int* __restrict__ colidx,
     }
 }
 
-int bitmap_words(size_t K, int* words, size_t factor) {
+// Bitmap of a block-row's column blocks, at most; to fill, there are as many prefix counts.  The limits of dynamic shared memory that are
+// set on the kernels are for this most: they belong to the kernel, and another thread's launch may come between setting and launching.
+constexpr int kMostBitmapBytes = 96 * 1024;
+int bitmap_words(size_t K, int* words) {
     const size_t Kb = K / 16;
     const size_t w = (Kb + 31) / 32;
-    if (w * 4 * factor > 192 * 1024) return fail(SMAT_ERR_RANGE, "K = %zu exceeds the builder's limit of 12582912", K);
+    if (w * 4 > kMostBitmapBytes) return fail(SMAT_ERR_RANGE, "K = %zu exceeds the builder's limit of 12582912", K);
     *words = (int)(w ? w : 1);
     return SMAT_OK;
 }
@@ -233,11 +236,11 @@ int smat_bcsr_count(const int* csr_rowptr, const int* csr_colidx, size_t M, size
     DeviceCtx* ctx = nullptr;
     if (int rc = get_device_ctx(&ctx)) return rc;
     int words = 1;
-    if (int rc = bitmap_words(K, &words, 2)) return rc;
+    if (int rc = bitmap_words(K, &words)) return rc;
     const int Mb = (int)(M / 16);
     if (Mb > 0) {
         const size_t smem = (size_t)words * 4;
-        SMAT_CUDA_TRY(cudaFuncSetAttribute(bcsr_count_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        SMAT_CUDA_TRY(cudaFuncSetAttribute(bcsr_count_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostBitmapBytes));
         bcsr_count_kernel<<<Mb, kBuildThreads, smem, stream>>>(csr_rowptr, csr_colidx, words, bcsr_rowptr);
         count_launch();
         SMAT_CUDA_TRY(cudaGetLastError());
@@ -265,10 +268,10 @@ int smat_bcsr_fill(const int* csr_rowptr, const int* csr_colidx, const void* csr
     DeviceCtx* ctx = nullptr;
     if (int rc = get_device_ctx(&ctx)) return rc;
     int words = 1;
-    if (int rc = bitmap_words(K, &words, 2)) return rc;
+    if (int rc = bitmap_words(K, &words)) return rc;
     const int Mb = (int)(M / 16);
     const size_t smem = (size_t)words * 8;
-    SMAT_CUDA_TRY(cudaFuncSetAttribute(bcsr_fill_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    SMAT_CUDA_TRY(cudaFuncSetAttribute(bcsr_fill_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * kMostBitmapBytes));
     bcsr_fill_kernel<<<Mb, kBuildThreads, smem, stream>>>(csr_rowptr, csr_colidx, reinterpret_cast<const __half*>(csr_vals),
                                                             words, bcsr_rowptr, bcsr_colidx,
                                                             reinterpret_cast<__half*>(bcsr_vals));

@@ -158,6 +158,26 @@ def test_plans_made_on_several_threads():
     assert not errors, errors[0]
 
 
+def test_builders_on_several_threads():
+    """The same for the builder of the blocks."""
+    errors = []
+
+    def work(K, stream):
+        try:
+            rowptr, colidx = np.arange(17, dtype=np.int32), np.arange(16, dtype=np.int32) * (K // 16)
+            with torch.cuda.stream(stream):
+                for _ in range(100):
+                    assert S.SparseMatrix.from_csr(16, K, rowptr, colidx, np.ones(16, np.float16)).nnzb > 0
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(K, torch.cuda.Stream())) for K in (256, 16 * 30000, 16 * 700000) * 2]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors[0]
+
+
 @pytest.mark.parametrize("rows,n", [(3, 5), (16385, 1 << 20)])
 def test_row_pointers_that_run_to_and_fro(rows, n):
     """Block-rows over the same blocks again and again: more blocks in all than are stored, up to more than 32 bits count."""
