@@ -40,6 +40,9 @@ int fail(int code, const char* fmt, ...) {
     va_start(ap, fmt);
     vsnprintf(t_error, sizeof(t_error), fmt, ap);
     va_end(ap);
+    // The runtime keeps the error of a call for the thread's next cudaGetLastError(), which stands behind its next launch and would fail
+    // that one too.  (What leaves the context unusable stays.)
+    if (code == SMAT_ERR_CUDA) (void)cudaGetLastError();
     return code;
 }
 void clear_error() { t_error[0] = 0; }

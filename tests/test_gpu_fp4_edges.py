@@ -178,6 +178,31 @@ def test_builders_on_several_threads():
     assert not errors, errors[0]
 
 
+def test_an_error_does_not_outlive_its_call():
+    """A plan whose tiles do not fit the device (193 GB for blocks in scattered ranges of columns) is refused, and what is asked for next
+    on the thread, the same plan without tiles, is made."""
+    torch.cuda.empty_cache()
+    steps, groups = 1 << 18, 20  # ranges of 256 columns, groups of 16 block-rows; four blocks in each
+    K = steps * 256 - 256
+    per_row = (steps - 1) // 4
+    n = groups * 16 * per_row
+    rowptr = torch.arange(groups * 16 + 1, device="cuda", dtype=torch.int32) * per_row
+    row = torch.arange(per_row, device="cuda", dtype=torch.int32)
+    # block-row e of a group has blocks in the ranges e / 4 modulo 4, so that four of them meet in every one
+    colidx = torch.stack([(row * 4 + e // 4) * 256 + e % 4 * 16 for e in range(16)]).reshape(-1).repeat(groups)
+    A = S.Fp4SparseMatrix.from_codes(groups * 256, K, rowptr, colidx, torch.full((n, 16, 8), 0x22, dtype=torch.uint8, device="cuda"),
+                                     torch.full((n, 16), 56, dtype=torch.uint8, device="cuda"))
+    with pytest.raises(S.SmatError) as e:
+        S.Fp4Plan(A)
+    assert e.value.code == -2
+    plan = S.Fp4Plan(A, tiles=False)
+    x = torch.ones((1, K), dtype=torch.float16, device="cuda")
+    C = torch.empty((groups * 256, 1), dtype=torch.float16, device="cuda")
+    x *= 2.0 ** -12
+    plan.spmm(x, C, check=True)
+    assert bool((C == 256).all())  # 16 * 65535 * 2^-12, rounded to fp16
+
+
 @pytest.mark.parametrize("rows,n", [(3, 5), (16385, 1 << 20)])
 def test_row_pointers_that_run_to_and_fro(rows, n):
     """Block-rows over the same blocks again and again: more blocks in all than are stored, up to more than 32 bits count."""
