@@ -103,8 +103,8 @@ class Fp4Matrix:
     def __init__(self, N, K, fmt="nvfp4", device="cuda"):
         if fmt not in _FORMATS:
             _format(fmt)
-        if K % 16:
-            _refuse(f"K ({K}) must be a multiple of 16")
+        if N < 0 or K < 0 or K % 16:
+            _refuse(f"N ({N}) must not be negative, and K ({K}) a multiple of 16")
         self.N, self.K, self.fmt = N, K, fmt
         self.quads = quads = (K + 63) // 64
         # One piece of memory; the tensors in it are made when they are asked for (a microsecond each).
@@ -179,6 +179,9 @@ class Fp4Matrix:
     def from_codes(cls, codes, scales, K, fmt="nvfp4", row_scale=None, device="cuda"):
         """From arrays as checkpoints and other programs have them: codes uint8 [N, K / 2] (the even column in the low half),
         scales 8-bit [N, ceil(K / 16 or 32)] (e4m3, or e8m0 bytes), row_scale one number or [N]."""
+        codes, scales = torch.as_tensor(codes), torch.as_tensor(scales)
+        if codes.dim() != 2:
+            _refuse(f"codes: a matrix [N, {K // 2}] is expected, not shape {tuple(codes.shape)}")
         N = codes.shape[0]
         self = cls(N, K, fmt, device)
         dev = self.device
@@ -356,6 +359,8 @@ class Fp4Plan:
             N, K, device = B.N, B.K, B.device
         else:
             Bt = B.data if isinstance(B, Matrix) else B
+            if Bt.dim() != 2:
+                _refuse(f"B [N, {self.A.K}] is expected, not shape {tuple(Bt.shape)}")
             N, K = Bt.shape
             device = Bt.device
             if Bt.dtype != Ct.dtype:

@@ -84,3 +84,22 @@ def test_arrays_that_do_not_fit(use):
         use(A)
     with pytest.raises(S.SmatError, match="current CUDA device"):  # the arrays of from_codes are fine
         use(_sparse())
+
+
+@pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
+def test_from_codes_takes_arrays_and_tensors(fmt):
+    """numpy arrays, lists and tensors alike; what has no two dimensions is refused like any other wrong shape."""
+    q = _matrix(fmt=fmt)
+    codes, scales = q.codes[:, :40].numpy().copy(), q.group_scales().numpy().copy()
+    row = None if q.row_scale is None else q.row_scale.numpy().copy()
+    for convert in (lambda a: a, torch.from_numpy, lambda a: torch.from_numpy(a).t().contiguous().t()):
+        p = S.Fp4Matrix.from_codes(convert(codes), convert(scales), 80, fmt, row, device="cpu")
+        assert torch.equal(p.codes, q.codes) and torch.equal(p.scales, q.scales)
+        assert p.row_scale is None if row is None else torch.equal(p.row_scale, q.row_scale)
+    for bad in (codes.reshape(-1), codes[0], np.uint8(3), codes[None]):
+        with pytest.raises(S.SmatError, match="codes") as e:
+            S.Fp4Matrix.from_codes(bad, scales, 80, fmt, row, device="cpu")
+        assert e.value.code == -1
+    for N, K in ((-1, 32), (2, -16)):
+        with pytest.raises(S.SmatError):
+            S.Fp4Matrix(N, K, device="cpu")
