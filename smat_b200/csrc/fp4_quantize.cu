@@ -45,8 +45,10 @@ __device__ __forceinline__ float divide_for_rounding(float x, float d, float y) 
     }
     return q;
 }
-// The same for a code of a value with at most 11 significant bits, in two instructions: the quotient, at most 6.5 in size, rounded to a
-// multiple of 2^-16.  x y is within 2^-21 of it; ties are multiples of 1/4, and what is no tie is at least 2^-13 away from one.
+// The same for a code of a value with at most 11 significant bits, in two instructions: the quotient rounded to a multiple of 2^-16.  It
+// is below 9 in size (6 times 1 + 2^-4 where the scale is a normal e4m3, 6 times 1.5 where it is the least subnormal), so that the sum
+// with 192 stays in [128, 256), whose step is 2^-16.  x y is within 2^-20 of it; ties are multiples of 1/4, and what is no tie is at
+// least 2^-13 away from one.
 __device__ __forceinline__ float divide_for_code(float x, float y) { return fmaf(x, y, 192.f) - 192.f; }
 
 // Scale byte of a group with largest magnitude gmax (bad: it holds a NaN or an infinity); values are divided by d, whose correctly

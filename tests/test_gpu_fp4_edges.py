@@ -23,6 +23,26 @@ def _case(fmt, counts, Kb, scales, seed=3):
     return c
 
 
+@pytest.mark.parametrize("N", [40, 150])
+def test_refreshed_tiles(N):
+    """set_values brings changed codes and scales to the tiles too, of one CTA and of pairs."""
+    c = Case(8, [30] * 40, 48, "nvfp4")
+    B, b = c.acts4(N)
+    plan = S.Fp4Plan(c.A)
+    C = torch.empty((c.M, N), dtype=torch.bfloat16, device="cuda")
+    plan.spmm(B, C, check=True)
+    _close(C, *F.multiply(c.vals, c.rowptr, c.colidx, b), c.longest)
+    c.A.codes.copy_(c.A.codes.flip(0))
+    c.A.scales.copy_(c.A.scales.roll(5, 0))
+    plan.set_values()
+    plan.spmm(B, C, check=True)
+    vals = F.block_values(F.unpack(c.A.codes.cpu().numpy()), c.A.scales.cpu().numpy(), c.p, c.rowptr, "nvfp4")
+    _close(C, *F.multiply(vals, c.rowptr, c.colidx, b), c.longest)
+    D = torch.empty_like(C)
+    S.Fp4Plan(c.A).spmm(B, D)
+    assert torch.equal(C, D)
+
+
 @pytest.mark.parametrize("N", [5, 40, 150])
 @pytest.mark.parametrize("tiles", [False, True])
 @pytest.mark.parametrize("swap", [False, True])
@@ -87,6 +107,29 @@ def test_row_scales_of_any_size(dtype):
     with np.errstate(over="ignore"):
         want = torch.from_numpy(F.block_values(bc, bs, p[:16], rowptr, "nvfp4").astype(np.float32)).half()
     assert torch.equal(A.dequantize(check=True).bcsrVal.cpu().view(2, 16, 16), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+def test_first_e4m3_scales(dtype):
+    """Groups whose scale is among the first e4m3 numbers, beside a large value in the row: their quotients reach 9, and lie on and next
+    to the borders between codes."""
+    eighths = np.arange(0, 73) / 8  # multiples of 1/8 up to 9: all borders and what is next to them in 11 bits
+    rows = []
+    for byte in range(1, 9):
+        s = F.E4M3[byte]
+        for gmax in (s * 6 * (1 - 2.0 ** -5), s * 6, s * 6 * (1 + 2.0 ** -5), (s + 2.0 ** -10) * 6 * (1 - 2.0 ** -7)):
+            x = np.minimum(np.resize(eighths * s, 16 * 5), gmax).reshape(5, 16)
+            x[:, 0] = gmax
+            rows.append(np.concatenate([[2688.0], np.zeros(15), x.reshape(-1)]))
+    X = torch.from_numpy(np.array(rows)).to(dtype).cuda()
+    q = S.Fp4Matrix.quantize(X)
+    codes, s, p = F.quantize_dense(X.double().cpu().numpy(), "nvfp4")
+    assert (p == 1).all() and s[:, 1:].min() <= 1 and s[:, 1:].max() <= 9
+    assert np.array_equal(q.group_scales().cpu().numpy(), s)
+    got = F.unpack(q.codes.cpu().numpy())[:, :X.shape[1]]
+    assert np.array_equal(got & 7, codes & 7)
+    d = X.double().cpu().numpy()[:, 16:].reshape(len(rows), 5, 16) / np.maximum(F.E4M3[s[:, 1:]], 2.0 ** -12)[..., None]
+    assert d.max() > 8.5
 
 
 @pytest.mark.parametrize("N,tiles", [(3, True), (5, False), (40, True), (40, False), (150, True)])
