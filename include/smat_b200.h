@@ -216,6 +216,11 @@ int smat_fp4_plan_spmm(const smat_fp4_plan* plan, const void* B, int dtype, void
 int smat_fp4_plan_spmm_fp4(const smat_fp4_plan* plan, const void* codes, const void* scales, const float* row_scale, int fmt, void* C,
                            int c_dtype, size_t N, void* stream);
 int smat_fp4_plan_destroy(smat_fp4_plan* plan);
+/* The self-test of giving up a wait (smat_selftest_plan_wait_timeout) for the kernel with tiles: the product expects more bytes of codes
+ * than are copied, and all waits give up after about 0.2 ms, in both CTAs of a pair.  C is invalid, the next smat_device_status says so
+ * (SMAT_ERR_DEVICE_WAIT), and products after that are as before.  SMAT_ERR_BAD_ARG for plans without tiles. */
+int smat_selftest_fp4_plan_wait_timeout(const smat_fp4_plan* plan, const void* codes, const void* scales, const float* row_scale, int fmt,
+                                        void* C, int c_dtype, size_t N, void* stream);
 
 /* Number of this library's kernels launched so far by the calling process (all devices). */
 long long smat_launch_count(void);

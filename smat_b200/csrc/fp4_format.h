@@ -75,6 +75,7 @@ constexpr int kFp4Rhs = 3;
 
 int launch_fp4_stream(const Fp4View& A, const Fp4Rhs& B, void* C, int c_dtype, size_t N, cudaStream_t stream);
 
-int launch_fp4_tile(const Fp4View& A, const Fp4Rhs& B, void* C, int c_dtype, size_t N, cudaStream_t stream);
+// selftest: waits for codes run out (smat_selftest_fp4_plan_wait_timeout).
+int launch_fp4_tile(const Fp4View& A, const Fp4Rhs& B, void* C, int c_dtype, size_t N, cudaStream_t stream, bool selftest = false);
 
 }  // namespace smat

@@ -362,6 +362,28 @@ int smat_fp4_plan_set_values(smat_fp4_plan* plan, void* stream) {
     return fill_values(plan, ctx, (cudaStream_t)stream);
 }
 
+static int spmm_fp4(const smat_fp4_plan* plan, const void* codes, const void* scales, const float* row_scale, int fmt, void* C, int c_dtype,
+                    size_t N, void* stream, bool selftest) {
+    clear_error();
+    if (int rc = check_product(plan, codes, C, c_dtype, N)) return rc;
+    if (fmt != plan->v.fmt) return fail(SMAT_ERR_BAD_ARG, "B must be in the format of A");
+    if (selftest && (!plan->v.tiles || !plan->v.blocks || !N)) return fail(SMAT_ERR_BAD_ARG, "this product's kernel has no such self-test");
+    if (!plan->v.block_rows || !N) return SMAT_OK;
+    if ((plan->v.K && !scales) || ((uintptr_t)scales & 15)) return fail(SMAT_ERR_BAD_ARG, "scales is NULL or not 16-byte aligned");
+    if (!plan->v.blocks) {
+        SMAT_CUDA_TRY(cudaMemsetAsync(C, 0, plan->v.block_rows * 16 * N * 2, (cudaStream_t)stream));
+        return SMAT_OK;
+    }
+    Fp4Rhs rhs;
+    rhs.data = codes;
+    rhs.scales = static_cast<const uint8_t*>(scales);
+    rhs.row_scale = row_scale;
+    rhs.dtype = kFp4Rhs;
+    const bool narrow = N <= kFp4NarrowColumns && plan->v.blocks <= kFp4NarrowBlocks && !selftest;
+    if (plan->v.tiles && !narrow) return launch_fp4_tile(plan->v, rhs, C, c_dtype, N, (cudaStream_t)stream, selftest);
+    return launch_fp4_stream(plan->v, rhs, C, c_dtype, N, (cudaStream_t)stream);
+}
+
 int smat_fp4_plan_spmm(const smat_fp4_plan* plan, const void* B, int dtype, void* C, size_t N, void* stream) {
     clear_error();
     if (dtype != SMAT_F16 && dtype != SMAT_BF16) return fail(SMAT_ERR_BAD_ARG, "B must be fp16 or bf16");
@@ -375,22 +397,12 @@ int smat_fp4_plan_spmm(const smat_fp4_plan* plan, const void* B, int dtype, void
 
 int smat_fp4_plan_spmm_fp4(const smat_fp4_plan* plan, const void* codes, const void* scales, const float* row_scale, int fmt, void* C,
                            int c_dtype, size_t N, void* stream) {
-    clear_error();
-    if (int rc = check_product(plan, codes, C, c_dtype, N)) return rc;
-    if (fmt != plan->v.fmt) return fail(SMAT_ERR_BAD_ARG, "B must be in the format of A");
-    if (!plan->v.block_rows || !N) return SMAT_OK;
-    if ((plan->v.K && !scales) || ((uintptr_t)scales & 15)) return fail(SMAT_ERR_BAD_ARG, "scales is NULL or not 16-byte aligned");
-    if (!plan->v.blocks) {
-        SMAT_CUDA_TRY(cudaMemsetAsync(C, 0, plan->v.block_rows * 16 * N * 2, (cudaStream_t)stream));
-        return SMAT_OK;
-    }
-    Fp4Rhs rhs;
-    rhs.data = codes;
-    rhs.scales = static_cast<const uint8_t*>(scales);
-    rhs.row_scale = row_scale;
-    rhs.dtype = kFp4Rhs;
-    const bool narrow = N <= kFp4NarrowColumns && plan->v.blocks <= kFp4NarrowBlocks;
-    return (plan->v.tiles && !narrow ? launch_fp4_tile : launch_fp4_stream)(plan->v, rhs, C, c_dtype, N, (cudaStream_t)stream);
+    return spmm_fp4(plan, codes, scales, row_scale, fmt, C, c_dtype, N, stream, false);
+}
+
+int smat_selftest_fp4_plan_wait_timeout(const smat_fp4_plan* plan, const void* codes, const void* scales, const float* row_scale, int fmt,
+                                        void* C, int c_dtype, size_t N, void* stream) {
+    return spmm_fp4(plan, codes, scales, row_scale, fmt, C, c_dtype, N, stream, true);
 }
 
 int smat_fp4_plan_destroy(smat_fp4_plan* plan) {

@@ -210,6 +210,8 @@ struct TileArgs {
     float* scratch;
     int* status;
     int c_dtype, rows, N, quads, b_row_tiles, col_tiles, total_steps;
+    uint32_t lost_bytes;  // expected but not copied, by the self-test of giving up
+    long long wait_cycles;
 };
 
 // NT columns of C per tile; a pair of CTAs (CG 2) for 256.
@@ -301,19 +303,19 @@ fp4_tile_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant_
             const uint8_t* tile = a.tiles + ((size_t)(gs + (int)uniform(s.k0)) * 2 + half) * kFp4TileBytes;
             for (int k = (int)uniform(s.k0); k < k1; k++, tile += 2 * kFp4TileBytes) {
                 const uint32_t rec = records.get(gs + k), stage = base + st * G::STAGE;
-                ok = __all_sync(~0u, wait_bar(empty(st), phase, abort_addr, a.status, 60));
+                ok = __all_sync(~0u, wait_bar(empty(st), phase, abort_addr, a.status, 60, a.wait_cycles));
                 if (!ok) break;
                 if (elect_one()) {
                     if (quads_of(rec, half) == 0) {  // no blocks here, of a pair in neither half
                         if (rank == 0) mbar_arrive(ready(st));
                     } else if constexpr (CG == 1) {
-                        mbar_arrive_expect_tx(ready(st), G::STAGE);
+                        mbar_arrive_expect_tx(ready(st), G::STAGE + a.lost_bytes);
                         bulk_load(stage, tile, kFp4TileCodes, ready(st));
                         tma_load_2d(stage + G::OFF_B, &mapB, (int)(rec >> 8) * 128, row, ready(st));
                     } else {
                         // Copies of the second CTA may complete before the first expects them: the phase ends with the first one's arrival.
                         const uint32_t first = pair_bar(ready(st), 0);
-                        if (rank == 0) mbar_arrive_expect_tx(ready(st), 2 * G::STAGE);
+                        if (rank == 0) mbar_arrive_expect_tx(ready(st), 2 * G::STAGE + a.lost_bytes);
                         tma_load_2d_pair(stage, &mapA, 0, ((gs + k) * 2 + half) * (int)(kFp4TileBytes / 128), first);
                         tma_load_2d_pair(stage + G::OFF_B, &mapB, (int)(rec >> 8) * 128, row, first);
                     }
@@ -335,7 +337,7 @@ fp4_tile_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant_
             for (int k = (int)uniform(s.k0); k < k1; k++, tile += 2 * kFp4TileBytes) {
                 const uint32_t rec = records.get(gs + k), stage = base + G::OFF_SF + st * G::SF_STAGE, quad = (rec >> 8) * 4;
                 const uint32_t bytes = min(4u, (uint32_t)a.quads - quad) * 512;
-                ok = __all_sync(~0u, wait_bar(taken(st), phase, abort_addr, a.status, 61));
+                ok = __all_sync(~0u, wait_bar(taken(st), phase, abort_addr, a.status, 61, a.wait_cycles));
                 if (!ok) break;
                 if (elect_one()) {
                     if (quads_of(rec, half) == 0) {
@@ -362,14 +364,14 @@ fp4_tile_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant_
         for (; ok && walk.next(s); n++) {
             const uint32_t buf = n % G::ACC;
             const int half = (int)uniform(half_of(s.t)), gs = (int)uniform(s.gs), k1 = (int)uniform(s.k1);
-            ok = __all_sync(~0u, wait_bar(acc_empty(buf), ((n / G::ACC) & 1) ^ 1, abort_addr, a.status, 62));
+            ok = __all_sync(~0u, wait_bar(acc_empty(buf), ((n / G::ACC) & 1) ^ 1, abort_addr, a.status, 62, a.wait_cycles));
             tc_fence_after();
             uint32_t acc = 0;
             for (int k = (int)uniform(s.k0); ok && k < k1; k++) {
                 const uint32_t mask = quads_of(records.get(gs + k), half);
                 const uint32_t sf = tmem + 256 + st * G::SF_COLUMNS;
                 const uint32_t da = (uint32_t)da0 + st * (G::STAGE >> 4), db = (uint32_t)db0 + st * (G::STAGE >> 4);
-                ok = __all_sync(~0u, wait_bar<CG == 2>(ready(st), phase, abort_addr, a.status, 63));
+                ok = __all_sync(~0u, wait_bar<CG == 2>(ready(st), phase, abort_addr, a.status, 63, a.wait_cycles));
                 if (!ok) break;
                 tc_fence_after();
                 if (elect_one()) {
@@ -401,8 +403,8 @@ fp4_tile_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant_
         while (walk.next(s)) steps += (uint32_t)(s.k1 - s.k0);
         for (i = (uint32_t)(warp - 12) / 4; i < steps; i += 2) {
             const uint32_t st = i % S, from = base + G::OFF_SF + i % G::Q * G::SF_STAGE + lane * 16;
-            if (!__all_sync(~0u, wait_bar(arrived(i % G::Q), (i / G::Q) & 1, abort_addr, a.status, 67) &&
-                                     wait_bar(empty(st), ((i / S) & 1) ^ 1, abort_addr, a.status, 68)))
+            if (!__all_sync(~0u, wait_bar(arrived(i % G::Q), (i / G::Q) & 1, abort_addr, a.status, 67, a.wait_cycles) &&
+                                     wait_bar(empty(st), ((i / S) & 1) ^ 1, abort_addr, a.status, 68, a.wait_cycles)))
                 break;
             tc_fence_after();
             uint4 v[4 + 4 * G::BT];
@@ -447,7 +449,7 @@ fp4_tile_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant_
             const uint32_t buf = n % G::ACC;
             s = f;
             const int m0 = s.g * 256 + half_of(s.t) * 128 + row0, n0 = column_of(s.t) * NT, cols = min(NT, a.N - n0);
-            if (!__all_sync(~0u, wait_bar(acc_full(buf), (n / G::ACC) & 1, abort_addr, a.status, 69))) break;
+            if (!__all_sync(~0u, wait_bar(acc_full(buf), (n / G::ACC) & 1, abort_addr, a.status, 69, a.wait_cycles))) break;
             tc_fence_after();
             const bool none = CG == 1 ? ld_shared_u32(any_addr + 4 * buf) == 0 : s.k0 != 0;  // no MMA wrote the accumulators
             auto release = [&]() {  // all of this warp's accumulators are read
@@ -800,7 +802,7 @@ int launch_tile_format(int fmt, const TileArgs& a, const CUtensorMap& mapA, cons
 
 }  // namespace
 
-int launch_fp4_tile(const Fp4View& A, const Fp4Rhs& B, void* C, int c_dtype, size_t N, cudaStream_t stream) {
+int launch_fp4_tile(const Fp4View& A, const Fp4Rhs& B, void* C, int c_dtype, size_t N, cudaStream_t stream, bool selftest) {
     DeviceCtx* ctx = nullptr;
     if (int rc = get_device_ctx(&ctx)) return rc;
     const int nt = N <= 32 ? 32 : N <= 64 ? 64 : N <= 128 ? 128 : 256;
@@ -820,6 +822,8 @@ int launch_fp4_tile(const Fp4View& A, const Fp4Rhs& B, void* C, int c_dtype, siz
     a.b_row_scale = B.row_scale;
     a.C = C;
     a.status = ctx->d_status;
+    a.wait_cycles = selftest ? kSelftestWaitCycles : kWaitCycles;
+    a.lost_bytes = selftest ? 16 : 0;
     a.c_dtype = c_dtype;
     a.rows = (int)(A.block_rows * 16);
     a.N = (int)N;

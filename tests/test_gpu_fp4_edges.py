@@ -278,3 +278,25 @@ def test_sparse_matrix_whose_arrays_do_not_fit():
     A.bcsrVal = A.bcsrVal.bfloat16()  # other types of values are fine
     # row scale 2^-11 (1 / 2688 lies above 2^-12), group scale 2^11 / 6 = 341.3 -> 352, code 2^11 / 352 = 5.8 -> 6: 6 * 352 * 2^-11
     assert bool((S.Fp4SparseMatrix.quantize(A, check=True).dequantize().bcsrVal == 1.03125).all())
+
+
+@pytest.mark.parametrize("N", [24, 64, 128, 264])
+@pytest.mark.parametrize("counts", [[100] * 40, [9] * 40])
+def test_waits_that_run_out(N, counts):
+    """Codes that never arrive: the kernel with tiles gives up, alone and in pairs, reports it, and products after that are right."""
+    c = Case(N, counts, 130, "nvfp4")
+    B, b = c.acts4(N)
+    plan, C = S.Fp4Plan(c.A), torch.empty((c.M, N), dtype=torch.float16, device="cuda")
+    L = S.lib()
+    call = L.smat_selftest_fp4_plan_wait_timeout
+    call.argtypes = S.fp4._lib().smat_fp4_plan_spmm_fp4.argtypes
+    codes, scales, row = B._at
+    torch.cuda.synchronize()
+    assert call(plan._h, codes, scales, row, 0, C.data_ptr(), 0, N, None) == 0
+    assert L.smat_device_status(None) == -3 and b"site code 6" in L.smat_last_error_string()
+    for _ in range(3):
+        C.fill_(float("nan"))
+        plan.spmm(B, C, check=True)
+        _close(C, *F.multiply(c.vals, c.rowptr, c.colidx, b), c.longest)
+    none = S.Fp4Plan(c.A, tiles=False)
+    assert call(none._h, codes, scales, row, 0, C.data_ptr(), 0, N, None) == -1
