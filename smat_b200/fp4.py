@@ -58,8 +58,11 @@ def _dtype(dtype, most=2):
     return code
 
 
+_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)  # a tensor on a GPU has initialised CUDA
+
+
 def _on_current_device(t):
-    if not t.is_cuda or t.device.index != torch.cuda.current_device():
+    if not t.is_cuda or t.get_device() != _device():
         _refuse(f"tensor on {t.device}: it has to be on the current CUDA device")
 
 
