@@ -23,12 +23,15 @@ namespace smat {
 namespace {
 
 constexpr int kThreads = 256;
-// Tiles are made where a step of 256 x 256 holds so many blocks (of 256) on average; they take 36 KB a step.  They are faster at any
-// fill (8192 x 8192, N = 512, tiles against warp-level MMAs: 31 and 55 us with 2 blocks a step, 33 and 77 with 4, 33 and 211 with 16),
-// so this bounds the memory: 9 KB a block, 64 times what is stored.
+// Tiles are made where a step of 256 x 256 holds so many blocks (of 256) on average; they take 36 KB a step.  For wide products they are
+// faster at any fill (8192 x 8192, N = 512, tiles against warp-level MMAs: 31 and 55 us with 2 blocks a step, 33 and 77 with 4, 33 and
+// 211 with 16), so this bounds the memory: 9 KB a block, 64 times what is stored.
 constexpr size_t kFp4TileFill = 4;
-// With so few columns and blocks the warp-level kernel is faster all the same (8192 x 8192, N = 8: 5 and 11 us for 2000 blocks, 9 and 13
-// for 33000; it takes 0.15 us more for every 1000).
+// With so few columns and blocks the warp-level kernel is faster all the same.  Measured, us, warp-level and tiles, 8 columns: 8192 x 8192
+// 6.7 and 13.9 with 5 200 blocks, 7.4 and 14.8 with 26 200, 11.3 and 14.8 with 52 400; 28672 x 8192 18.2 and 30.0 with 91 700;
+// 8192 x 28672 16.2 and 31.2 with 91 700, 27.1 and 31.1 with 183 500.  16 columns: 9.4 and 13.9, 10.3 and 14.8, 16.2 and 14.9; 27.1 and
+// 30.0; 23.8 and 31.3, 40.4 and 30.8.  So both bounds are on the tiles' side: with more blocks, or a few more columns of few blocks,
+// the warp-level kernel would still be the faster one.
 constexpr size_t kFp4NarrowColumns = 8, kFp4NarrowBlocks = 50000;
 
 // Looks a block-row's pointers and columns over (a CTA a block-row): they have to lie in the arrays and the matrix, the columns in

@@ -7,8 +7,9 @@
 // The codes are those of exact arithmetic: quotients that an fp32 division would round onto a tie are moved off it again.
 // A group that holds a NaN or an infinity gets the scale NaN and codes 0; row maxima are taken over finite values.
 //
-// What bounds it: HBM, and some seven instructions a value (half a group a lane, which lays loads side by side as the way back does with
-// its stores, has each scale worked out twice: 125 us instead of 75).  Prompt of 4096 x 28672 bf16: 75 us, 0.61 of HBM's rate; back 50,
+// What bounds it: HBM and some seven instructions a value, of which neither is full (issue slots 53 %, HBM 38 % for 2048 x 14336): a row
+// is loaded, waited for, and converted once its maximum is known.  (Half a group a lane, which lays loads side by side as the way back
+// does with its stores, has each scale worked out twice: 125 us instead of 75.)  Prompt of 4096 x 28672 bf16: 75 us, 0.61 of HBM's rate; back 50,
 // 0.92.  Blocks of the layer 8192 x 28672 at 20 %: 30 and 24 us.  A row of a dense matrix stays in the registers of its CTA between the maximum
 // and the codes (up to 128 values a thread; longer ones are read again, from L2); so do not the blocks of a block-row, whose second
 // reading comes out of L2.  Loads are issued several groups at a time.

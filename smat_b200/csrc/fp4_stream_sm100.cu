@@ -302,7 +302,9 @@ int launch_fp4_stream(const Fp4View& A, const Fp4Rhs& B, void* C, int c_dtype, s
     a.block_rows = (int)A.block_rows;
     a.N = (int)N;
     a.K = A.K;
-    // Warps of a block-row: so many that the SMs hold about 32 warps each, but not below 8 blocks a warp.
+    // Warps of a block-row: so many that the SMs hold about 32 warps each, but not below 8 blocks a warp.  Measured with B in 16 bits,
+    // whose tiles are up to 64 columns wide; of B in 4 bits, with tiles of 32, it counts half the tiles from 33 columns on, and was not
+    // measured.
     const size_t tiles = (N + 63) / 64, want = (size_t)ctx->sm_count * 32;
     const size_t per_row = A.blocks / A.block_rows + 1;
     size_t parts = 1;

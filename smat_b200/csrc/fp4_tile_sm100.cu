@@ -661,7 +661,11 @@ __global__ void __launch_bounds__(256) fp4_join_kernel(const __grid_constant__ T
 bool make_schedule(const int* gsp, int groups, int units, int sms, Schedule& s) {
     constexpr long long kLeast = 8;  // steps of a range: below, joining costs more than the time saved
     constexpr long long kUnit = 6;   // what a unit takes beside its steps, in steps
-    constexpr long long kJoin = 24;  // what storing parts and joining them takes, in steps (8 to 10 us)
+    // What storing parts and joining them takes, in steps of tiles of 256 columns (8 to 10 us).  Narrower tiles have shorter steps; the
+    // same rule is right for them or a little late to cut: us, cut and whole, 32, 64, 128 and 256 columns: layer 4096 x 14336 at 20 %
+    // 13.7 and 22.3, 14.1 and 22.5, 15.5 and 23.3, 23.4 and 27.3 (it cuts); 8192 x 8192 at 5 % 13.0 and 14.6, 13.5 and 14.7, 15.4 and
+    // 15.6, 23.1 and 19.2 (it does not).  kUnit between 1 and 12 makes no difference to the first of these.
+    constexpr long long kJoin = 24;
     const long long total = (long long)gsp[groups] * units, all = (long long)groups * units;
     s.parts = (int)std::max<long long>(std::min<long long>(std::min(sms, kMaxParts), std::max(total / kLeast, all)), 1);
     s.units = units;
@@ -805,6 +809,10 @@ int launch_tile_format(int fmt, const TileArgs& a, const CUtensorMap& mapA, cons
 int launch_fp4_tile(const Fp4View& A, const Fp4Rhs& B, void* C, int c_dtype, size_t N, cudaStream_t stream, bool selftest) {
     DeviceCtx* ctx = nullptr;
     if (int rc = get_device_ctx(&ctx)) return rc;
+    // The narrowest tile that holds N, or pairs.  Below 256 a tile has to hold all of N: its first column is looked for in the scales of
+    // B by tiles of 128 rows.  us, tiles of 32, 64, 128 and 256 columns: layer 8192 x 28672 at 20 %, N = 8 30.9, 31.2, 42.0, 36.1; N = 32
+    // 30.7, 30.2, 30.9, 33.9; N = 128 33.8 and 38.4 (the last two); layer 4096 x 14336, N = 8 13.5, 14.8, 16.5, 18.7; N = 32 13.7, 13.5,
+    // 14.0, 18.1; N = 64 14.2, 14.4 and 19.0; N = 128 15.5 and 20.3.
     const int nt = N <= 32 ? 32 : N <= 64 ? 64 : N <= 128 ? 128 : 256;
     CUtensorMap map, mapA = {};
     const size_t pitch = fp4_pitch(A.K);

@@ -323,8 +323,9 @@ class Fp4SparseMatrix:
 
 class Fp4Plan:
     """Plan for products of block-rows [brow_begin, brow_end) of an Fp4SparseMatrix (smat_fp4_plan_*).  ``tiles=False``: only for
-    products with 16-bit B (decoding), 148 bytes a block; those with B in 4 bits work but are slow.  Products do
-    not change the plan and may run on several streams at a time."""
+    products with 16-bit B (decoding), 148 bytes a block beside the matrix's own 144; those with B in 4 bits work but are slow.  With
+    tiles a layer that stores a fifth of its blocks takes 720 bytes a block more.  Products do not change the plan and may run on several
+    streams at a time."""
 
     def __init__(self, A, brow_begin=0, brow_end=None, tiles=True):
         self.A = A
@@ -353,7 +354,8 @@ class Fp4Plan:
 
     def spmm(self, B, Cout, check=False):
         """C = A x B.  B: Matrix / tensor [N, K] in fp16 or bf16 with C of the same type, or an Fp4Matrix of A's format with C in
-        either; C: Matrix / tensor [rows, N], contiguous, fully overwritten."""
+        either; C: Matrix / tensor [rows, N], contiguous, fully overwritten.  16-bit B is meant for few tokens: from about 32 on
+        ``Plan(A4.dequantize())`` is faster (fp16), for a prompt of thousands four times as fast, if the blocks may take 16 bits."""
         if self._h is None:
             _refuse("the plan is closed")
         Ct = Cout.data if isinstance(Cout, Matrix) else Cout
