@@ -391,6 +391,9 @@ class Fp4Plan:
         if check:
             _check(lib().smat_device_status(api._stream()))
 
+    def __reduce__(self):  # by copy, deepcopy and pickle: a copy would free the handle a second time
+        raise TypeError("a plan cannot be copied: make another one of the same Fp4SparseMatrix")
+
     def close(self):
         if self._h is not None:
             _lib().smat_fp4_plan_destroy(self._h)

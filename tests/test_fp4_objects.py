@@ -103,3 +103,12 @@ def test_from_codes_takes_arrays_and_tensors(fmt):
     for N, K in ((-1, 32), (2, -16)):
         with pytest.raises(S.SmatError):
             S.Fp4Matrix(N, K, device="cpu")
+
+
+@pytest.mark.parametrize("how", [copy.copy, copy.deepcopy, pickle.dumps])
+def test_plans_are_not_copied(how):
+    """Two objects with one handle would free it twice."""
+    plan = S.Fp4Plan.__new__(S.Fp4Plan)
+    plan._h = None
+    with pytest.raises(TypeError, match="plan"):
+        how(plan)
