@@ -240,8 +240,8 @@ class Fp4SparseMatrix:
     def _check_arrays(self):
         """Refuses arrays that are not what the kernels take them for.  Those that were looked over before are not again (0.4 instead of
         4 us)."""
-        arrays, c = self._arrays(), self._checked
-        if c and arrays[0] is c[0] and arrays[1] is c[1] and arrays[2] is c[2] and arrays[3] is c[3] and arrays[4] is c[4]:
+        c = self._checked
+        if c and self.codes is c[0] and self.scales is c[1] and self.row_scale is c[2] and self.bcsrRowPtr is c[3] and self.bcsrColIdx is c[4]:
             return
         device = self.codes.device if isinstance(self.codes, torch.Tensor) else None
         for name, t, dtype, least, most in (("codes", self.codes, torch.uint8, self.nnzb * 128, self.nnzb * 128),
@@ -257,29 +257,26 @@ class Fp4SparseMatrix:
                 _refuse(f"{name}: {'at least ' if most is None else ''}{least} elements of {dtype} are expected")
             if not t.is_contiguous() or t.device != device:
                 _refuse(f"{name}: it has to be contiguous and on {device}, like codes")
-        self._checked = arrays
-
-    def _allocate(self):
-        dev = self.bcsrRowPtr.device
-        self.codes = torch.empty((self.nnzb, 16, 8), dtype=torch.uint8, device=dev)
-        self.scales = torch.empty((self.nnzb, 16), dtype=torch.uint8, device=dev)
-        self.row_scale = torch.empty(self.M, dtype=torch.float32, device=dev) if self.fmt == "nvfp4" else None
+        self._checked = self._arrays()
 
     @classmethod
     def quantize(cls, A, fmt="nvfp4", check=False):
         """The blocks of a SparseMatrix in 4 bits; the structure is shared with it."""
         f = _format(fmt)
-        v, rp = A.bcsrVal, A.bcsrRowPtr
+        v, rp, ci = A.bcsrVal, A.bcsrRowPtr, A.bcsrColIdx
         _on_current_device(v)
-        if v.numel() < A.nnzb * 256 or not v.is_contiguous() or rp.dtype != torch.int32 or rp.numel() != A.M // 16 + 1 or not rp.is_contiguous():
-            _refuse(f"a SparseMatrix with bcsrVal of {A.nnzb} blocks and int32 bcsrRowPtr of {A.M // 16 + 1}, contiguous, is expected")
+        if (v.numel() < A.nnzb * 256 or rp.numel() != A.M // 16 + 1 or ci.numel() < A.nnzb or rp.dtype != torch.int32 or ci.dtype != torch.int32
+                or not (v.is_contiguous() and rp.is_contiguous() and ci.is_contiguous()) or not v.get_device() == rp.get_device() == ci.get_device()):
+            _refuse(f"a SparseMatrix of {A.nnzb} blocks with int32 bcsrRowPtr of {A.M // 16 + 1} and bcsrColIdx, contiguous, on one device is expected")
         self = cls()
-        self.M, self.K, self.nnzb, self.fmt = A.M, A.K, A.nnzb, fmt
-        self.bcsrRowPtr, self.bcsrColIdx = A.bcsrRowPtr, A.bcsrColIdx
-        self._allocate()
-        self._checked = self._arrays()
-        rc = _lib().smat_fp4_quantize_blocks(A.bcsrVal.data_ptr(), _dtype(A.bcsrVal.dtype), A.bcsrRowPtr.data_ptr(), A.bcsrColIdx.data_ptr(),
-                                             A.M, A.nnzb, f, self.codes.data_ptr(), self.scales.data_ptr(), _ptr(self.row_scale), api._stream())
+        n, dev = A.nnzb, v.device
+        self.M, self.K, self.nnzb, self.fmt, self.bcsrRowPtr, self.bcsrColIdx = A.M, A.K, n, fmt, rp, ci
+        self.codes = codes = torch.empty((n, 16, 8), dtype=torch.uint8, device=dev)
+        self.scales = scales = torch.empty((n, 16), dtype=torch.uint8, device=dev)
+        self.row_scale = row = torch.empty(A.M, dtype=torch.float32, device=dev) if f == 0 else None
+        self._checked = (codes, scales, row, rp, ci)
+        rc = (_LIB or _lib()).smat_fp4_quantize_blocks(v.data_ptr(), _dtype(v.dtype), rp.data_ptr(), ci.data_ptr(), A.M, n, f, codes.data_ptr(),
+                                                       scales.data_ptr(), _ptr(row), api._stream())
         if rc:
             _check(rc)
         if check:

@@ -268,7 +268,7 @@ def test_row_pointers_that_run_to_and_fro(rows, n):
 def test_sparse_matrix_whose_arrays_do_not_fit():
     rowptr, colidx = np.array([0, 2, 3], np.int32), np.array([0, 32, 16], np.int32)
     for name, spoil in (("bcsrVal", lambda t: t[:512]), ("bcsrVal", lambda t: torch.cat([t, t])[::2]), ("bcsrRowPtr", lambda t: t[:2]),
-                        ("bcsrRowPtr", lambda t: t.long())):
+                        ("bcsrRowPtr", lambda t: t.long()), ("bcsrColIdx", lambda t: t[:2]), ("bcsrColIdx", lambda t: t.cpu())):
         A = S.SparseMatrix.from_bcsr(32, 48, rowptr, colidx, np.ones(768, np.float16))
         setattr(A, name, spoil(getattr(A, name)))
         with pytest.raises(S.SmatError) as e:
